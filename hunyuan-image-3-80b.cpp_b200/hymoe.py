@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("HYMOE_LIB") or os.path.join(HERE, "libhymoe.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "hymoe.h")
 
-TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0 = 0, 1, 2, 8
+TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_BF16 = 0, 1, 2, 8, 30
 HOST_PTRS = 1
 USE_GRAPH = 2
 PRE_NORM = 4
@@ -32,7 +32,7 @@ EXPORTS = ["hymoe_version", "hymoe_nccl_unique_id", "hymoe_create", "hymoe_destr
            "hymoe_gguf_open", "hymoe_gguf_close", "hymoe_gguf_last_error", "hymoe_gguf_tensor",
            "hymoe_gguf_get_u32", "hymoe_gguf_moe_tensors", "hymoe_load_layer_gguf",
            "hymoe_set_norm", "hymoe_set_routing", "hymoe_load_layer_async", "hymoe_wait_layer",
-           "hymoe_load_layer_gguf_async"]
+           "hymoe_load_layer_gguf_async", "hymoe_route", "hymoe_route_backward"]
 
 PHASES = ["router", "plan", "dispatch", "gate_up", "down", "combine", "ep_dispatch",
           "ep_combine", "copy_in", "copy_out"]
@@ -54,6 +54,16 @@ class Routing(C.Structure):
     _fields_ = [("group_limited_greedy", C.c_int32), ("n_group", C.c_uint32), ("topk_group", C.c_uint32),
                 ("drop_tokens", C.c_int32), ("capacity_factor", C.c_float), ("min_capacity", C.c_uint32),
                 ("norm_topk_prob", C.c_int32), ("routed_scaling_factor", C.c_float)]
+
+
+class Mat(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("type", C.c_int32), ("ld", C.c_int64)]
+
+
+class GateSpec(C.Structure):
+    _fields_ = [("score", C.c_int32), ("n_group", C.c_uint32), ("topk_group", C.c_uint32),
+                ("group_score", C.c_int32), ("norm_topk_prob", C.c_int32),
+                ("routed_scaling_factor", C.c_float)]
 
 
 class Debug(C.Structure):
@@ -116,6 +126,9 @@ def lib() -> C.CDLL:
         L.hymoe_load_layer_gguf_async.argtypes = [vp, u32, vp, u32]
         L.hymoe_set_norm.argtypes = [vp, u32, vp, C.c_float, C.c_int]
         L.hymoe_set_routing.argtypes = [vp, C.POINTER(Routing)]
+        L.hymoe_route.argtypes = [C.POINTER(GateSpec), C.POINTER(Mat), vp, u32, u32, u32, vp, vp, vp, vp, vp]
+        L.hymoe_route_backward.argtypes = [C.POINTER(GateSpec), C.POINTER(Mat), vp, vp, vp, u32, u32, u32,
+                                           C.POINTER(Mat), vp]
         for f in EXPORTS:
             if f not in ("hymoe_version", "hymoe_destroy", "hymoe_last_error", "hymoe_gguf_close",
                          "hymoe_gguf_last_error"):
@@ -372,6 +385,117 @@ class MoE:
         flags = (HOST_PTRS if host else 0) | (USE_GRAPH if graph else 0) | (PRE_NORM if pre_norm else 0)
         self._check(self.L.hymoe_forward(self.h, layer, x_ptr, resid_ptr, out_ptr, T, bias_ptr,
                                          C.byref(dbg) if dbg else None, flags))
+
+
+# ---- Operators on the caller's device buffers: torch CUDA tensors in, torch CUDA tensors out,
+# on the current stream of the tensors' device.
+
+
+def _check_entry(st: int) -> None:
+    if st != 0:
+        raise HymoeError(st, lib().hymoe_last_error(None).decode(errors="replace"))
+
+
+def _torch_types() -> dict:
+    import torch
+    return {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+
+
+def _mat(t, rows: int, cols: int, what: str) -> Mat:
+    """A [rows, cols] CUDA tensor whose rows are contiguous, as an hymoe_mat (rows may be strided)."""
+    if tuple(t.shape) != (rows, cols):
+        raise ValueError(f"{what} must be [{rows}, {cols}], got {tuple(t.shape)}")
+    code = _torch_types().get(t.dtype)
+    if code is None or not t.is_cuda:
+        raise ValueError(f"{what} must be a float32, float16 or bfloat16 CUDA tensor, got {t.dtype} on {t.device}")
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what} must have contiguous rows, got strides {t.stride()}")
+    return Mat(t.data_ptr(), code, t.stride(0) if rows > 1 else max(cols, 1))
+
+
+def _vec(t, shape: tuple, dtype, device, what: str):
+    """Pointer of a contiguous tensor of this shape, type and device (None stays None)."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} {list(shape)} on {device}, got {t.dtype} "
+                         f"{list(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+class _on:
+    """The device of the tensors made current, and its current stream."""
+
+    def __init__(self, device):
+        import torch
+        self.guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
+        self.stream = torch.cuda.current_stream(device).cuda_stream
+
+    def __enter__(self):
+        if self.guard:
+            self.guard.__enter__()
+        return self.stream
+
+    def __exit__(self, *exc):
+        if self.guard:
+            self.guard.__exit__(*exc)
+
+
+class Gate:
+    """Routing of tokens to experts from their logits (hymoe_route): score "softmax" or "sigmoid";
+    group = (n_group, topk_group) with group_score "max" or "top2"."""
+
+    SCORES = {"softmax": 0, "sigmoid": 1}
+    GROUPS = {"max": 0, "top2": 1}
+
+    def __init__(self, n_experts: int, topk: int, score: str = "softmax", group=None, group_score: str = "max",
+                 norm_topk_prob: bool = True, scale: float = 1.0):
+        self.L = lib()
+        self.E, self.K = n_experts, topk
+        if score not in self.SCORES or group_score not in self.GROUPS:
+            raise ValueError(f"score {score!r} is one of {list(self.SCORES)}, group_score {group_score!r} one of "
+                             f"{list(self.GROUPS)}")
+        ng, tg = group if group else (0, 0)
+        self.spec = GateSpec(self.SCORES[score], ng, tg, self.GROUPS[group_score], 1 if norm_topk_prob else 0, scale)
+        # the library checks the gate itself: a call without tokens does only that
+        _check_entry(self.L.hymoe_route_backward(C.byref(self.spec), None, None, None, None, 0, n_experts, topk,
+                                                 None, None))
+
+    def route(self, logits, bias=None, scores: bool = False, counts: bool = False) -> dict:
+        """logits [T, E] (float32, float16 or bfloat16; rows may be strided), bias [E] float32.
+        Returns idx int32 [T, K] (-1: no expert left), weights float32 [T, K] and on request
+        scores float32 [T, E] and counts int32 [E]."""
+        import torch
+        T, dev = logits.shape[0], logits.device
+        m = _mat(logits, T, self.E, "logits")
+        b = _vec(bias, (self.E,), torch.float32, dev, "bias")
+        out = {"idx": torch.empty((T, self.K), dtype=torch.int32, device=dev),
+               "weights": torch.empty((T, self.K), dtype=torch.float32, device=dev)}
+        if counts:
+            out["counts"] = torch.empty((self.E,), dtype=torch.int32, device=dev)
+        if scores:
+            out["scores"] = torch.empty((T, self.E), dtype=torch.float32, device=dev)
+        with _on(dev) as st:
+            _check_entry(self.L.hymoe_route(C.byref(self.spec), C.byref(m), b, T, self.E, self.K,
+                                            out["idx"].data_ptr(), out["weights"].data_ptr(),
+                                            out["scores"].data_ptr() if scores else None,
+                                            out["counts"].data_ptr() if counts else None, st))
+        return out
+
+    def backward(self, logits, idx, d_weights, d_scores=None):
+        """Gradient to the logits [T, E] (their type) for the selections idx of route()."""
+        import torch
+        T, dev = logits.shape[0], logits.device
+        m = _mat(logits, T, self.E, "logits")
+        i = _vec(idx, (T, self.K), torch.int32, dev, "idx")
+        dw = _vec(d_weights, (T, self.K), torch.float32, dev, "d_weights")
+        ds = _vec(d_scores, (T, self.E), torch.float32, dev, "d_scores")
+        d = torch.empty((T, self.E), dtype=logits.dtype, device=dev)
+        dm = Mat(d.data_ptr(), m.type, self.E)
+        with _on(dev) as st:
+            _check_entry(self.L.hymoe_route_backward(C.byref(self.spec), C.byref(m), i, dw, ds, T, self.E, self.K,
+                                                     C.byref(dm), st))
+        return d
 
 
 def zipf_router_bias(seed: int, E: int, s: float = 1.1):

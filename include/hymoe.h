@@ -41,7 +41,8 @@ enum {
     HYMOE_TYPE_F32 = 0,
     HYMOE_TYPE_F16 = 1,
     HYMOE_TYPE_Q4_0 = 2, /* 32-element blocks: fp16 d, 16 bytes of nibbles; x = (q-8)*d */
-    HYMOE_TYPE_Q8_0 = 8  /* 32-element blocks: fp16 d, 32 int8;            x = q*d     */
+    HYMOE_TYPE_Q8_0 = 8, /* 32-element blocks: fp16 d, 32 int8;            x = q*d     */
+    HYMOE_TYPE_BF16 = 30 /* hymoe_mat arguments only (hymoe_route and the following calls) */
 };
 
 /* flags for hymoe_load_layer / hymoe_forward */
@@ -305,6 +306,67 @@ hymoe_status hymoe_profile_read(hymoe_ctx* ctx, float* total_ms, int32_t* launch
  * that overlap on the GPU (unordered streams) race and give wrong results. */
 hymoe_status hymoe_ffn_noalloc(const hymoe_tensor* gate_up, const hymoe_tensor* down,
                                const float* x, float* y, uint32_t n_tokens, void* stream);
+
+/* ---- Operators on the caller's device buffers.  Like hymoe_ffn_noalloc they need no context
+ * and allocate nothing; every pointer is device memory of the current device (or managed
+ * memory), each call is asynchronous on `stream` (a cudaStream_t, NULL = legacy default stream)
+ * and may be captured into a CUDA graph, and hymoe_last_error(NULL) has the message of this
+ * thread's last failing call.  Calls on different streams share nothing. */
+
+/* A row-major matrix in device memory: element (i, j) is data[i * ld + j], ld >= columns in
+ * elements, type HYMOE_TYPE_F32 / F16 / BF16, data aligned to its element. */
+typedef struct {
+    void* data;
+    int32_t type;
+    int64_t ld;
+} hymoe_mat;
+
+enum { HYMOE_SCORE_SOFTMAX = 0, HYMOE_SCORE_SIGMOID = 1 };
+enum { HYMOE_GROUP_MAX = 0, HYMOE_GROUP_TOP2 = 1 };
+
+/* How a router's logits become a token's experts and weights (hymoe_route):
+ *   z  = logit; NaN and -inf close the expert for the token, +inf counts as FLT_MAX
+ *   s  = softmax of z over the open experts, or sigmoid(z); 0 for a closed expert
+ *   c  = s + bias: decides the selection only.  Without a bias the order is that of z.  A bias
+ *        of -inf or NaN closes the expert for the selection (not for the softmax), +inf counts
+ *        as FLT_MAX.
+ *   n_group > 0: experts in n_group groups of consecutive experts, each valued by its largest c
+ *        (HYMOE_GROUP_MAX) or the sum of its two largest (HYMOE_GROUP_TOP2; its only one where one
+ *        is open); the topk_group best groups (ties: lower group) stay selectable
+ *   the topk largest c in order (ties: lower expert); where fewer are selectable the remaining
+ *        entries get index -1 and weight 0
+ *   w  = routed_scaling_factor * s, over the sum of the selected s with norm_topk_prob
+ * c and the group values are compared as in double precision, whatever the logits' type. */
+typedef struct {
+    int32_t score;        /* HYMOE_SCORE_*                              */
+    uint32_t n_group;     /* 0: no groups; else <= 32 and divides n_experts */
+    uint32_t topk_group;  /* 1..n_group                                 */
+    int32_t group_score;  /* HYMOE_GROUP_*                              */
+    int32_t norm_topk_prob;
+    float routed_scaling_factor;
+} hymoe_gate;
+
+#define HYMOE_GATE_MAX_EXPERTS 512
+#define HYMOE_GATE_MAX_TOPK 32
+
+/* Routes n_tokens tokens over n_experts <= HYMOE_GATE_MAX_EXPERTS experts, topk <=
+ * HYMOE_GATE_MAX_TOPK of them each.  logits [n_tokens, n_experts]; bias [n_experts] (nullable);
+ * idx, weights [n_tokens, topk]; scores [n_tokens, n_experts] (nullable): every s; counts
+ * [n_experts] (nullable): tokens that selected each expert, overwritten.  The routing of
+ * moe_forward_cpu (src/attention.cpp:224-275) is the softmax gate with norm_topk_prob. */
+hymoe_status hymoe_route(const hymoe_gate* gate, const hymoe_mat* logits, const float* bias,
+                         uint32_t n_tokens, uint32_t n_experts, uint32_t topk, int32_t* idx,
+                         float* weights, float* scores, int32_t* counts, void* stream);
+
+/* Gradient of hymoe_route to the logits, for given selections: d_logits [n_tokens, n_experts]
+ * (the logits' type; every element written, closed experts 0) from d_weights [n_tokens, topk]
+ * and d_scores [n_tokens, n_experts] (nullable).  idx as hymoe_route wrote it; entries outside
+ * [0, n_experts) and entries of closed experts take no part.  The selection has no gradient.
+ * d_logits may be the logits' own buffer. */
+hymoe_status hymoe_route_backward(const hymoe_gate* gate, const hymoe_mat* logits, const int32_t* idx,
+                                  const float* d_weights, const float* d_scores, uint32_t n_tokens,
+                                  uint32_t n_experts, uint32_t topk, const hymoe_mat* d_logits,
+                                  void* stream);
 
 /* ---- GGUF weight files (replaces HunyuanGGUFLoader, src/hunyuan_gguf_loader.h:20-71, for
  * the MoE tensors).  A file (GGUF version 2 or 3) is parsed by the library and mapped
