@@ -32,7 +32,8 @@ EXPORTS = ["hymoe_version", "hymoe_nccl_unique_id", "hymoe_create", "hymoe_destr
            "hymoe_gguf_open", "hymoe_gguf_close", "hymoe_gguf_last_error", "hymoe_gguf_tensor",
            "hymoe_gguf_get_u32", "hymoe_gguf_moe_tensors", "hymoe_load_layer_gguf",
            "hymoe_set_norm", "hymoe_set_routing", "hymoe_load_layer_async", "hymoe_wait_layer",
-           "hymoe_load_layer_gguf_async", "hymoe_route", "hymoe_route_backward"]
+           "hymoe_load_layer_gguf_async", "hymoe_route", "hymoe_route_backward",
+           "hymoe_adapt_workspace", "hymoe_adapt", "hymoe_adapt_backward"]
 
 PHASES = ["router", "plan", "dispatch", "gate_up", "down", "combine", "ep_dispatch",
           "ep_combine", "copy_in", "copy_out"]
@@ -64,6 +65,12 @@ class GateSpec(C.Structure):
     _fields_ = [("score", C.c_int32), ("n_group", C.c_uint32), ("topk_group", C.c_uint32),
                 ("group_score", C.c_int32), ("norm_topk_prob", C.c_int32),
                 ("routed_scaling_factor", C.c_float)]
+
+
+class AdapterSpec(C.Structure):
+    _fields_ = [("n_adapters", C.c_uint32), ("rank", C.c_uint32), ("in_features", C.c_uint32),
+                ("out_features", C.c_uint32), ("type", C.c_int32), ("a", C.c_void_p), ("b", C.c_void_p),
+                ("scale", C.c_void_p)]
 
 
 class Debug(C.Structure):
@@ -129,6 +136,11 @@ def lib() -> C.CDLL:
         L.hymoe_route.argtypes = [C.POINTER(GateSpec), C.POINTER(Mat), vp, u32, u32, u32, vp, vp, vp, vp, vp]
         L.hymoe_route_backward.argtypes = [C.POINTER(GateSpec), C.POINTER(Mat), vp, vp, vp, u32, u32, u32,
                                            C.POINTER(Mat), vp]
+        L.hymoe_adapt_workspace.argtypes = [C.POINTER(AdapterSpec), u32, C.c_int, C.POINTER(C.c_size_t)]
+        L.hymoe_adapt.argtypes = [C.POINTER(AdapterSpec), C.POINTER(Mat), vp, u32, C.POINTER(Mat), C.POINTER(Mat), vp,
+                                  C.c_size_t, vp]
+        L.hymoe_adapt_backward.argtypes = [C.POINTER(AdapterSpec), C.POINTER(Mat), C.POINTER(Mat), vp, u32,
+                                           C.POINTER(Mat), C.POINTER(Mat), vp, vp, vp, C.c_size_t, vp]
         for f in EXPORTS:
             if f not in ("hymoe_version", "hymoe_destroy", "hymoe_last_error", "hymoe_gguf_close",
                          "hymoe_gguf_last_error"):
@@ -496,6 +508,89 @@ class Gate:
             _check_entry(self.L.hymoe_route_backward(C.byref(self.spec), C.byref(m), i, dw, ds, T, self.E, self.K,
                                                      C.byref(dm), st))
         return d
+
+
+class Adapters:
+    """Low-rank adapters of many requests beside one projection (hymoe_adapt): a [n, rank, in] and
+    b [n, out, rank] of one 16-bit type, scale [n] float32 (None: 1)."""
+
+    def __init__(self, a, b, scale=None):
+        import torch
+        self.L = lib()
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError(f"adapters must be a [n, rank, in] and b [n, out, rank], got {tuple(a.shape)} and "
+                             f"{tuple(b.shape)}")
+        if a.dtype not in (torch.float16, torch.bfloat16) or not a.is_cuda:
+            raise ValueError(f"adapters must be float16 or bfloat16 CUDA tensors, got {a.dtype} on {a.device}")
+        self.n, self.rank, self.n_in, self.n_out = a.shape[0], a.shape[1], a.shape[2], b.shape[1]
+        self.device = a.device
+        self.spec = AdapterSpec(self.n, self.rank, self.n_in, self.n_out, _torch_types()[a.dtype],
+                                _vec(a, tuple(a.shape), a.dtype, a.device, "a"),
+                                _vec(b, tuple(b.shape), a.dtype, a.device, "b"),
+                                _vec(scale, (self.n,), torch.float32, a.device, "scale"))
+        self._keep = (a, b, scale)
+        self._bytes = {}
+        self._workspace_bytes(0, False)  # the library checks the sizes
+
+    def _workspace_bytes(self, T: int, backward: bool) -> int:
+        got = self._bytes.get((T, backward))
+        if got is None:
+            n = C.c_size_t()
+            _check_entry(self.L.hymoe_adapt_workspace(C.byref(self.spec), T, 1 if backward else 0, C.byref(n)))
+            got = self._bytes[(T, backward)] = n.value
+        return got
+
+    def _workspace(self, T: int, backward: bool):
+        import torch
+        n = self._workspace_bytes(T, backward)
+        return (torch.empty(n, dtype=torch.uint8, device=self.device) if n else None), n
+
+    def _rows(self, t, T: int, cols: int, what: str):
+        if t is None:
+            return None
+        if t.device != self.device:
+            raise ValueError(f"{what} must be on {self.device}, got {t.device}")
+        return _mat(t, T, cols, what)
+
+    def apply(self, x, ids=None, base=None, out=None):
+        """out[t] = base[t] + scale * B (A x[t]) of adapter ids[t] (int32; outside [0, n): none; None:
+        adapter 0).  base None: zeros.  out: written in place (may be base); None: a new tensor of
+        base's type, x's without a base."""
+        import torch
+        T = x.shape[0]
+        mx, mb = self._rows(x, T, self.n_in, "x"), self._rows(base, T, self.n_out, "base")
+        i = _vec(ids, (T,), torch.int32, self.device, "ids")
+        if out is None:
+            out = torch.empty((T, self.n_out), dtype=x.dtype if base is None else base.dtype, device=self.device)
+        mo = self._rows(out, T, self.n_out, "out")
+        with _on(self.device) as st:
+            ws, n = self._workspace(T, False)
+            _check_entry(self.L.hymoe_adapt(C.byref(self.spec), C.byref(mx), i, T, C.byref(mb) if mb else None,
+                                            C.byref(mo), ws.data_ptr() if n else None, n, st))
+        return out
+
+    def backward(self, x, dy, ids=None, base=None, want=("dx", "da", "db")) -> dict:
+        """Gradients for dy [T, out]: dx (x's type, base added where given), da and db (float32, every
+        adapter's).  want: the ones to compute."""
+        import torch
+        T = x.shape[0]
+        mx, my = self._rows(x, T, self.n_in, "x"), self._rows(dy, T, self.n_out, "dy")
+        mb, i = self._rows(base, T, self.n_in, "base"), _vec(ids, (T,), torch.int32, self.device, "ids")
+        res = {}
+        if "dx" in want:
+            res["dx"] = torch.empty((T, self.n_in), dtype=x.dtype, device=self.device)
+        if "da" in want:
+            res["da"] = torch.empty((self.n, self.rank, self.n_in), dtype=torch.float32, device=self.device)
+        if "db" in want:
+            res["db"] = torch.empty((self.n, self.n_out, self.rank), dtype=torch.float32, device=self.device)
+        md = self._rows(res.get("dx"), T, self.n_in, "dx")
+        with _on(self.device) as st:
+            ws, n = self._workspace(T, True)
+            _check_entry(self.L.hymoe_adapt_backward(
+                C.byref(self.spec), C.byref(mx), C.byref(my), i, T, C.byref(mb) if mb else None,
+                C.byref(md) if md else None, res["da"].data_ptr() if "da" in res else None,
+                res["db"].data_ptr() if "db" in res else None, ws.data_ptr() if n else None, n, st))
+        return res
 
 
 def zipf_router_bias(seed: int, E: int, s: float = 1.1):

@@ -368,6 +368,59 @@ hymoe_status hymoe_route_backward(const hymoe_gate* gate, const hymoe_mat* logit
                                   uint32_t n_experts, uint32_t topk, const hymoe_mat* d_logits,
                                   void* stream);
 
+/* Low-rank adapters of many requests beside one projection: adapter a adds
+ *   scale[a] * B_a (A_a x)
+ * to the projection's result.  a [n_adapters, rank, in_features] and b [n_adapters,
+ * out_features, rank] are contiguous, of `type` HYMOE_TYPE_F16 or HYMOE_TYPE_BF16; scale
+ * [n_adapters] F32 (NULL: 1).  Adapters of a smaller rank are padded with zero rows of A (zero
+ * columns of B). */
+typedef struct {
+    uint32_t n_adapters;   /* 1..HYMOE_ADAPT_MAX_ADAPTERS          */
+    uint32_t rank;         /* 1..HYMOE_ADAPT_MAX_RANK              */
+    uint32_t in_features;  /* 1..HYMOE_ADAPT_MAX_FEATURES          */
+    uint32_t out_features; /* 1..HYMOE_ADAPT_MAX_FEATURES          */
+    int32_t type;
+    const void* a;
+    const void* b;
+    const float* scale;
+} hymoe_adapters;
+
+#define HYMOE_ADAPT_MAX_ADAPTERS 4096
+#define HYMOE_ADAPT_MAX_RANK 128
+#define HYMOE_ADAPT_MAX_FEATURES 1048576
+#define HYMOE_ADAPT_MAX_TOKENS 16777216
+
+/* Bytes of workspace that hymoe_adapt (backward == 0) or hymoe_adapt_backward (backward != 0)
+ * needs for up to n_tokens tokens; 0 is possible. */
+hymoe_status hymoe_adapt_workspace(const hymoe_adapters* adapters, uint32_t n_tokens, int backward,
+                                   size_t* bytes);
+
+/* out[t] = base[t] + scale[a] * B_a (A_a x[t]), a = ids[t], for t < n_tokens.
+ *   x [n_tokens, in_features], of the adapters' type or F32
+ *   ids [n_tokens] in any order; a token whose id is outside [0, n_adapters) has no adapter:
+ *     its row is the base's.  ids == NULL: adapter 0 for every token
+ *   base, out [n_tokens, out_features], both of the adapters' type or both F32.  base == NULL
+ *     counts as zeros; out may be base itself (same data and ld), else nothing may overlap
+ *   workspace: hymoe_adapt_workspace bytes, 256-byte aligned, used by this call alone until it
+ *     has run (NULL where none is needed)
+ * Products are summed in fp32, the intermediate A x is kept in fp32 or in parts that add up to
+ * it, and the result is rounded once. */
+hymoe_status hymoe_adapt(const hymoe_adapters* adapters, const hymoe_mat* x, const int32_t* ids,
+                         uint32_t n_tokens, const hymoe_mat* base, const hymoe_mat* out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Gradients of hymoe_adapt for dy [n_tokens, out_features] (adapters' type or F32):
+ *   dx[t]  = base[t] + scale[a] * A_a^T (B_a^T dy[t])   (dx, base: x's type; base nullable, dx may
+ *            be base itself; dx == NULL: not computed)
+ *   da[a]  = scale[a] * sum over a's tokens of (B_a^T dy[t]) x[t]^T   [n_adapters, rank, in_features]
+ *   db[a]  = scale[a] * sum over a's tokens of dy[t] (A_a x[t])^T     [n_adapters, out_features, rank]
+ * da and db are F32, overwritten for every adapter (0 where it has no tokens), nullable.  The
+ * sums' order depends on the ids alone: equal inputs give equal bits. */
+hymoe_status hymoe_adapt_backward(const hymoe_adapters* adapters, const hymoe_mat* x, const hymoe_mat* dy,
+                                  const int32_t* ids, uint32_t n_tokens, const hymoe_mat* base,
+                                  const hymoe_mat* dx, float* da, float* db, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 /* ---- GGUF weight files (replaces HunyuanGGUFLoader, src/hunyuan_gguf_loader.h:20-71, for
  * the MoE tensors).  A file (GGUF version 2 or 3) is parsed by the library and mapped
  * read-only; tensors are views of their raw GGUF blocks in the mapping, valid until
