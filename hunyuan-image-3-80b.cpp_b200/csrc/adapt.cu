@@ -4,122 +4,218 @@
 //   low[t]  = scale[a] * A_a x[t]          (a = ids[t]; backward also scale[a] * B_a^T dy[t])
 //   out[t]  = base[t] + B_a low[t]         (backward: dx[t] = base[t] + A_a^T low_dy[t])
 //   dA_a    = sum_t low_dy[t] x[t]^T,  dB_a = sum_t dy[t] low_x[t]^T
+//
+// This file: the plan (tokens sorted by adapter, tiles of 64 rows of one adapter, gradient
+// items), the checks and the order of the launches.  adapt_low.cu, adapt_wide.cu and
+// adapt_grad.cu hold the three products.
 #include <initializer_list>
 
-#include "common.cuh"
-#include "entry.h"
+#include "adapt.cuh"
+#include "kernels.h"
 
 namespace hymoe {
 namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanSmem = 220 * 1024;
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void from_f(float& d, float v) { d = v; }
-__device__ __forceinline__ void from_f(__half& d, float v) { d = __float2half_rn(v); }
-__device__ __forceinline__ void from_f(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
-
-__device__ __forceinline__ int adapter_of(const int* ids, int t, int n) {
-    const int a = ids != nullptr ? __ldg(ids + t) : 0;
-    return a >= 0 && a < n ? a : -1;
+// Warps of the plan that count and place tokens: one row of counters each, beside five lists.
+__host__ __device__ constexpr int plan_rows(int n) {
+    const int fit = (kPlanSmem / 4 - 5 * (n + 2)) / (n + 1);
+    return fit < 32 ? fit : 32;
 }
 
-// low[t, j] = scale * sum_i x[t, i] W[a][j * wj + i * wi]; one warp per (token, j).
-template <typename TX, typename TW>
-__global__ void low_kernel(const TX* __restrict__ x, size_t ldx, const int* __restrict__ ids, int T, int n, int R,
-                           int K, const TW* __restrict__ w, size_t wj, size_t wi, const float* __restrict__ scale,
-                           float* __restrict__ low) {
-    const size_t id = (static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
-    const int t = static_cast<int>(id / R), j = static_cast<int>(id % R), lane = threadIdx.x & 31;
-    if (t >= T) return;
-    const int a = adapter_of(ids, t, n);
-    float s = 0.f;
-    if (a >= 0) {
-        const TW* wr = w + static_cast<size_t>(a) * R * K + j * wj;
-        for (int i = lane; i < K; i += 32) s = fmaf(to_f(x[t * ldx + i]), to_f(wr[i * wi]), s);
+// Exclusive prefix sum of v[0, n) in place, v[n] = the sum; all threads of the CTA.
+__device__ void block_scan(int* v, int n) {
+    __shared__ int wsum[33];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (n + kPlanThreads - 1) / kPlanThreads, lo = min(n, tid * per), hi = min(n, lo + per);
+    __syncthreads();
+    int s = 0;
+    for (int i = lo; i < hi; ++i) s += v[i];
+    int inc = s;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
-        if (scale != nullptr) s *= __ldg(scale + a);
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kAll, inc, o);
+        if (lane >= o) inc += u;
     }
-    if (lane == 0) low[static_cast<size_t>(t) * R + j] = s;
-}
-
-// out[t, o] = base[t, o] + sum_j low[t, j] W[a][j * wj + o * wo]; one thread per element.
-template <typename TY, typename TW>
-__global__ void wide_kernel(const float* __restrict__ low, const int* __restrict__ ids, int T, int n, int R, int N,
-                            const TW* __restrict__ w, size_t wj, size_t wo, const TY* base, size_t ldb, TY* out,
-                            size_t ldo) {
-    const size_t id = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int t = static_cast<int>(id / N), o = static_cast<int>(id % N);
-    if (t >= T) return;
-    const int a = adapter_of(ids, t, n);
-    float s = 0.f;
-    if (a >= 0) {
-        const TW* wr = w + static_cast<size_t>(a) * R * N + o * wo;
-        for (int j = 0; j < R; ++j) s = fmaf(low[static_cast<size_t>(t) * R + j], to_f(wr[j * wj]), s);
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    if (warp == 0) {
+        const int w = wsum[lane];
+        int winc = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(kAll, winc, o);
+            if (lane >= o) winc += u;
+        }
+        wsum[lane] = winc - w;
+        if (lane == 31) wsum[32] = winc;
     }
-    if (base != nullptr) s += to_f(base[t * ldb + o]);
-    from_f(out[t * ldo + o], s);
+    __syncthreads();
+    int run = wsum[warp] + inc - s;
+    for (int i = lo; i < hi; ++i) {
+        const int x = v[i];
+        v[i] = run;
+        run += x;
+    }
+    if (tid == 0) v[n] = wsum[32];
+    __syncthreads();
 }
 
-// g[a][j * gj + m * gm] = sum over a's tokens of low[t, j] x[t, m]; one thread per element.
-template <typename TX>
-__global__ void outer_kernel(const float* __restrict__ low, const TX* __restrict__ x, size_t ldx,
-                             const int* __restrict__ ids, int T, int n, int R, int M, float* __restrict__ g, size_t gj,
-                             size_t gm) {
-    const size_t id = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int m = static_cast<int>(id % M), j = static_cast<int>(id / M % R), a = static_cast<int>(id / M / R);
-    if (a >= n) return;
-    float s = 0.f;
-    for (int t = 0; t < T; ++t)
-        if (adapter_of(ids, t, n) == a) s = fmaf(low[static_cast<size_t>(t) * R + j], to_f(x[t * ldx + m]), s);
-    g[static_cast<size_t>(a) * R * M + j * gj + m * gm] = s;
+// Largest b with pre[b] <= i, of pre[0..n] ascending, pre[n] > i.
+__device__ __forceinline__ int bucket_of(const int* pre, int n, int i) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= i) lo = mid;
+        else hi = mid;
+    }
+    return lo;
 }
 
-unsigned blocks(size_t threads) { return static_cast<unsigned>((threads + 255) / 256); }
+// Stable counting sort of the tokens by adapter and the lists over the sorted rows, by one CTA:
+// each counting warp owns a run of tokens (in order) and a row of counters, 32 tokens a step; the
+// lanes of equal adapters find one another by a warp match.  8192 tokens take 8 steps, twice.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restrict__ ids, int T, int n, AdaptPlan p,
+                                                            int chunk) {
+    extern __shared__ int sm[];
+    griddep_launch_dependents();
+    const int nb = n + 1;  // the last bucket: no adapter
+    int *off = sm, *tpre = off + n + 2, *ipre = tpre + n + 2, *spre = ipre + n + 2, *tot = spre + n + 2;
+    int* cnt = tot + n + 2;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, W = plan_rows(n);
+    for (int i = tid; i < W * nb; i += kPlanThreads) cnt[i] = 0;
+    __syncthreads();
+    const int per = ((T + W - 1) / W + 31) / 32 * 32;
+    const int64_t lo64 = static_cast<int64_t>(warp) * per;
+    const int t_lo = lo64 < T ? static_cast<int>(lo64) : T, t_hi = warp < W ? min(T, t_lo + per) : t_lo;
+    int* mine = cnt + (warp < W ? warp : 0) * nb;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int t0 = t_lo; t0 < t_hi; t0 += 32 * 8) {
+            int b[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int t = t0 + 32 * i + lane;
+                int v = ids != nullptr && t < t_hi ? __ldg(ids + t) : 0;
+                if (v < 0 || v >= n) v = n;
+                b[i] = t < t_hi ? v : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (t0 + 32 * i >= t_hi) break;
+                const unsigned same = __match_any_sync(kAll, b[i]);
+                const int before = __popc(same & ((1u << lane) - 1u));
+                if (pass == 0) {
+                    if (b[i] >= 0 && before == 0) mine[b[i]] += __popc(same);
+                } else {
+                    const int at = b[i] >= 0 ? mine[b[i]] + before : 0;
+                    __syncwarp();
+                    if (b[i] >= 0) {
+                        p.perm[at] = t0 + 32 * i + lane;
+                        if (before == 0) mine[b[i]] = at + __popc(same);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (pass == 1) break;
+        __syncthreads();
+        for (int a = tid; a < nb; a += kPlanThreads) {
+            int c = 0;
+            for (int w = 0; w < W; ++w) c += cnt[w * nb + a];
+            tot[a] = c;
+            off[a] = c;
+            tpre[a] = (c + kAdRows - 1) / kAdRows;
+            const int pieces = a < n ? max(1, (c + chunk - 1) / chunk) : 0;
+            ipre[a] = pieces;
+            spre[a] = pieces > 1 ? pieces : 0;
+        }
+        block_scan(off, nb);
+        block_scan(tpre, nb);
+        block_scan(ipre, n);
+        block_scan(spre, n);
+        for (int a = tid; a < nb; a += kPlanThreads) {
+            int run = off[a];
+            for (int w = 0; w < W; ++w) {
+                const int c = cnt[w * nb + a];
+                cnt[w * nb + a] = run;
+                run += c;
+            }
+        }
+        __syncthreads();
+    }
+    const int n_tiles = tpre[nb];
+    for (int i = tid; i < n_tiles; i += kPlanThreads) {
+        const int a = bucket_of(tpre, nb, i), r = (i - tpre[a]) * kAdRows;
+        p.tiles[i] = make_int4(a < n ? a : -1, off[a] + r, min(kAdRows, tot[a] - r), 0);
+    }
+    if (p.items != nullptr) {
+        const int n_items = ipre[n];
+        for (int i = tid; i < n_items; i += kPlanThreads) {
+            const int a = bucket_of(ipre, n, i), q = i - ipre[a], r = q * chunk;
+            const bool several = ipre[a + 1] - ipre[a] > 1;
+            p.items[i] = make_int4(a, off[a] + r, min(chunk, tot[a] - r), several ? spre[a] + q : -1);
+        }
+        for (int a = tid; a <= n; a += kPlanThreads) p.pieces[a] = ipre[a];
+        if (tid == 0) p.n_lists[1] = n_items;
+    }
+    if (tid == 0) p.n_lists[0] = n_tiles;
+}
 
-template <typename TW>
-cudaError_t run_low(const hymoe_mat& x, const int* ids, int T, int n, int R, int K, const void* w, size_t wj, size_t wi,
-                    const float* scale, float* low, cudaStream_t st) {
-    const TW* wp = static_cast<const TW*>(w);
-    const unsigned g = blocks(static_cast<size_t>(T) * R * 32);
-    if (x.type == HYMOE_TYPE_F32)
-        low_kernel<float, TW><<<g, 256, 0, st>>>(static_cast<const float*>(x.data), x.ld, ids, T, n, R, K, wp, wj, wi, scale, low);
-    else
-        low_kernel<TW, TW><<<g, 256, 0, st>>>(static_cast<const TW*>(x.data), x.ld, ids, T, n, R, K, wp, wj, wi, scale, low);
+cudaError_t launch_plan_adapt(const int* ids, int T, int n, const AdaptPlan& p, cudaStream_t st) {
+    const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanSmem);
+    if (e != cudaSuccess) return e;
+    const size_t smem = sizeof(int) * (5 * (static_cast<size_t>(n) + 2) + static_cast<size_t>(plan_rows(n)) * (n + 1));
+    plan_kernel<<<1, kPlanThreads, smem, st>>>(ids, T, n, p, adapt_chunk(T));
     return cudaGetLastError();
 }
 
-template <typename TW>
-cudaError_t run_wide(const float* low, const int* ids, int T, int n, int R, int N, const void* w, size_t wj, size_t wo,
-                     const hymoe_mat* base, const hymoe_mat& out, cudaStream_t st) {
-    const TW* wp = static_cast<const TW*>(w);
-    const unsigned g = blocks(static_cast<size_t>(T) * N);
-    const void* bp = base ? base->data : nullptr;
-    const size_t ldb = base ? base->ld : 0;
-    if (out.type == HYMOE_TYPE_F32)
-        wide_kernel<float, TW><<<g, 256, 0, st>>>(low, ids, T, n, R, N, wp, wj, wo, static_cast<const float*>(bp), ldb,
-                                                  static_cast<float*>(out.data), out.ld);
-    else
-        wide_kernel<TW, TW><<<g, 256, 0, st>>>(low, ids, T, n, R, N, wp, wj, wo, static_cast<const TW*>(bp), ldb,
-                                               static_cast<TW*>(out.data), out.ld);
-    return cudaGetLastError();
+// The workspace: every part starts on 256 bytes.
+struct AdaptLayout {
+    size_t perm, tiles, items, pieces, lists, low, low2, part, bytes;
+    int max_tiles, max_items;
+};
+AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward) {
+    AdaptLayout l{};
+    const size_t n = ad->n_adapters;
+    auto take = [&](size_t bytes) {
+        const size_t at = l.bytes;
+        l.bytes += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    if (T == 0) return l;
+    const size_t long_pieces = T / 1024 < 32 ? T / 1024 : 32;  // T / adapt_chunk(T) at most
+    l.max_tiles = static_cast<int>(T / kAdRows + (n + 1 < T ? n + 1 : T));
+    l.max_items = static_cast<int>(n + long_pieces);
+    l.lists = take(2 * sizeof(int));
+    l.perm = take(T * sizeof(int));
+    l.tiles = take(static_cast<size_t>(l.max_tiles) * sizeof(int4));
+    l.low = take(T * adapt_rp(ad->rank) * sizeof(float));
+    if (backward) {
+        l.items = take(static_cast<size_t>(l.max_items) * sizeof(int4));
+        l.pieces = take((n + 1) * sizeof(int));
+        l.low2 = take(T * adapt_rp(ad->rank) * sizeof(float));
+        // an adapter of c tokens in p > 1 pieces: p < 2 c / chunk
+        l.part = take(2 * long_pieces * ad->rank * (static_cast<size_t>(ad->in_features) + ad->out_features) * sizeof(float));
+    }
+    return l;
+}
+AdaptPlan plan_in(const AdaptLayout& l, char* ws, bool backward) {
+    AdaptPlan p{};
+    p.perm = reinterpret_cast<int*>(ws + l.perm);
+    p.tiles = reinterpret_cast<int4*>(ws + l.tiles);
+    p.items = backward ? reinterpret_cast<int4*>(ws + l.items) : nullptr;
+    p.pieces = backward ? reinterpret_cast<int*>(ws + l.pieces) : nullptr;
+    p.n_lists = reinterpret_cast<int*>(ws + l.lists);
+    p.max_tiles = l.max_tiles;
+    p.max_items = l.max_items;
+    return p;
 }
 
-template <typename TW>
-cudaError_t run_outer(const float* low, const hymoe_mat& x, const int* ids, int T, int n, int R, int M, float* g,
-                      size_t gj, size_t gm, cudaStream_t st) {
-    const unsigned b = blocks(static_cast<size_t>(n) * R * M);
-    if (x.type == HYMOE_TYPE_F32)
-        outer_kernel<float><<<b, 256, 0, st>>>(low, static_cast<const float*>(x.data), x.ld, ids, T, n, R, M, g, gj, gm);
-    else
-        outer_kernel<TW><<<b, 256, 0, st>>>(low, static_cast<const TW*>(x.data), x.ld, ids, T, n, R, M, g, gj, gm);
-    return cudaGetLastError();
-}
-
-size_t low_bytes(const hymoe_adapters* ad, size_t T) { return (T * ad->rank * 4 + 255) / 256 * 256; }
+// Rows of `ld` elements of `es` bytes that all start on 16-byte boundaries.
+bool rows_vec(const void* p, size_t ld, size_t es) { return entry_aligned(p, 16) && ld * es % 16 == 0; }
 
 const char* adapters_problem(const hymoe_adapters* ad) {
     if (!ad) return "null adapters";
@@ -156,7 +252,7 @@ extern "C" hymoe_status hymoe_adapt_workspace(const hymoe_adapters* ad, uint32_t
     if (const char* why = adapters_problem(ad)) return entry_fail(HYMOE_ERR_INVALID_ARG, why);
     if (!bytes) return entry_fail(HYMOE_ERR_INVALID_ARG, "null bytes");
     if (n_tokens > HYMOE_ADAPT_MAX_TOKENS) return entry_fail(HYMOE_ERR_INVALID_ARG, "n_tokens must be at most 16777216");
-    *bytes = low_bytes(ad, n_tokens) * (backward ? 2 : 1);
+    *bytes = adapt_layout(ad, n_tokens, backward != 0).bytes;
     return HYMOE_OK;
 }
 
@@ -179,6 +275,59 @@ hymoe_status current_device(int* dev) {
     return entry_fail(HYMOE_ERR_CUDA, "cudaGetDevice failed");
 }
 
+cudaError_t run_low(const AdaptPlan& plan, const hymoe_mat& x, const void* w, int type_w, bool trans, const float* scale,
+                    float* low, int T, int R, int K, int n_sms, cudaStream_t st) {
+    AdaptLow a{};
+    a.plan = plan;
+    a.x = x.data;
+    a.ldx = static_cast<size_t>(x.ld);
+    a.w = w;
+    a.scale = scale;
+    a.low = low;
+    a.K = K;
+    a.R = R;
+    a.vec_x = rows_vec(x.data, a.ldx, elem_bytes(x.type));
+    a.vec_w = rows_vec(w, trans ? R : K, 2);
+    return launch_adapt_low(a, x.type, type_w, trans, T, n_sms, st);
+}
+
+cudaError_t run_wide(const AdaptPlan& plan, const float* low, const void* w, int type_w, bool trans, const hymoe_mat* base,
+                     const hymoe_mat& out, int T, int R, int N, int n_sms, cudaStream_t st) {
+    const size_t es = elem_bytes(out.type);
+    AdaptWide a{};
+    a.plan = plan;
+    a.low = low;
+    a.w = w;
+    a.base = base ? base->data : nullptr;
+    a.out = out.data;
+    a.ldb = base ? static_cast<size_t>(base->ld) : 0;
+    a.ldo = static_cast<size_t>(out.ld);
+    a.N = N;
+    a.R = R;
+    a.vec_w = rows_vec(w, trans ? N : R, 2);
+    a.vec_b = base ? rows_vec(base->data, a.ldb, es) : 0;
+    a.vec_o = rows_vec(out.data, a.ldo, es);
+    a.in_place = base && base->data == out.data;
+    return launch_adapt_wide(a, out.type, type_w, trans, T, n_sms, st);
+}
+
+cudaError_t run_grad(const AdaptPlan& plan, const float* low, const hymoe_mat& x, float* g, float* part, int T, int n,
+                     int R, int M, int gm, int gj, cudaStream_t st) {
+    AdaptGrad a{};
+    a.plan = plan;
+    a.low = low;
+    a.x = x.data;
+    a.ldx = static_cast<size_t>(x.ld);
+    a.g = g;
+    a.part = part;
+    a.M = M;
+    a.R = R;
+    a.gm = gm;
+    a.gj = gj;
+    a.vec_x = rows_vec(x.data, a.ldx, elem_bytes(x.type));
+    return launch_adapt_grad(a, x.type, T, n, st);
+}
+
 bool all_on(int dev, std::initializer_list<const void*> ps) {
     for (const void* p : ps)
         if (p && !entry_on_device(p, dev)) return false;
@@ -193,7 +342,8 @@ extern "C" hymoe_status hymoe_adapt(const hymoe_adapters* ad, const hymoe_mat* x
     set_thread_error("");
     if (const char* why = adapters_problem(ad)) return entry_fail(HYMOE_ERR_INVALID_ARG, why);
     if (n_tokens == 0) return HYMOE_OK;
-    if (const char* why = common_problem(ad, ids, n_tokens, workspace, workspace_bytes, low_bytes(ad, n_tokens)))
+    if (const char* why = common_problem(ad, ids, n_tokens, workspace, workspace_bytes,
+                                         adapt_layout(ad, n_tokens, false).bytes))
         return entry_fail(HYMOE_ERR_INVALID_ARG, why);
     const uint32_t T = n_tokens, I = ad->in_features, O = ad->out_features;
     if (!rows_ok(x, I, ad->type) || !rows_ok(out, O, ad->type) || (base && (!rows_ok(base, O, ad->type) || base->type != out->type)))
@@ -216,14 +366,15 @@ extern "C" hymoe_status hymoe_adapt(const hymoe_adapters* ad, const hymoe_mat* x
         return entry_fail(HYMOE_ERR_INVALID_ARG, "hymoe_adapt: every pointer must be memory of the current device");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int n = static_cast<int>(ad->n_adapters), R = static_cast<int>(ad->rank), t = static_cast<int>(T);
-    float* low = static_cast<float*>(workspace);
-    auto go = [&](auto tag) {
-        using TW = decltype(tag);
-        cudaError_t e = run_low<TW>(*x, ids, t, n, R, static_cast<int>(I), ad->a, I, 1, ad->scale, low, st);
-        if (e == cudaSuccess) e = run_wide<TW>(low, ids, t, n, R, static_cast<int>(O), ad->b, 1, R, base, *out, st);
-        return e;
-    };
-    const cudaError_t e = ad->type == HYMOE_TYPE_F16 ? go(__half{}) : go(__nv_bfloat16{});
+    int n_sms = 0;
+    cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, dev);
+    const AdaptLayout l = adapt_layout(ad, T, false);
+    char* ws = static_cast<char*>(workspace);
+    const AdaptPlan plan = plan_in(l, ws, false);
+    float* low = reinterpret_cast<float*>(ws + l.low);
+    cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
+    if (e == cudaSuccess) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low, t, R, static_cast<int>(I), n_sms, st);
+    if (e == cudaSuccess) e = run_wide(plan, low, ad->b, ad->type, false, base, *out, t, R, static_cast<int>(O), n_sms, st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt: kernel launch failed");
     return HYMOE_OK;
 }
@@ -239,7 +390,7 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
     if (!entry_aligned(da, 4) || !entry_aligned(db, 4))
         return entry_fail(HYMOE_ERR_INVALID_ARG, "hymoe_adapt_backward: da and db must be 4-byte aligned");
     if (T > 0) {
-        if (const char* why = common_problem(ad, ids, T, workspace, workspace_bytes, 2 * low_bytes(ad, T)))
+        if (const char* why = common_problem(ad, ids, T, workspace, workspace_bytes, adapt_layout(ad, T, true).bytes))
             return entry_fail(HYMOE_ERR_INVALID_ARG, why);
         if (!rows_ok(x, I, ad->type) || !rows_ok(dy, O, ad->type) || (dx && (!rows_ok(dx, I, ad->type) || dx->type != x->type)) ||
             (base && (!dx || !rows_ok(base, I, ad->type) || base->type != dx->type)))
@@ -279,20 +430,21 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
         }
         return HYMOE_OK;
     }
-    float* low_x = static_cast<float*>(workspace);
-    float* low_dy = low_x + low_bytes(ad, T) / 4;
+    int n_sms = 0;
+    cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, dev);
+    const AdaptLayout l = adapt_layout(ad, T, true);
+    char* ws = static_cast<char*>(workspace);
+    const AdaptPlan plan = plan_in(l, ws, true);
+    float* low_dy = reinterpret_cast<float*>(ws + l.low);
+    float* low_x = reinterpret_cast<float*>(ws + l.low2);
+    float* part = reinterpret_cast<float*>(ws + l.part);
     const int i = static_cast<int>(I), o = static_cast<int>(O);
-    auto go = [&](auto tag) {
-        using TW = decltype(tag);
-        cudaError_t e = cudaSuccess;
-        if (db) e = run_low<TW>(*x, ids, t, n, R, i, ad->a, I, 1, ad->scale, low_x, st);
-        if (e == cudaSuccess && (dx || da)) e = run_low<TW>(*dy, ids, t, n, R, o, ad->b, 1, R, ad->scale, low_dy, st);
-        if (e == cudaSuccess && dx) e = run_wide<TW>(low_dy, ids, t, n, R, i, ad->a, I, 1, base, *dx, st);
-        if (e == cudaSuccess && da) e = run_outer<TW>(low_dy, *x, ids, t, n, R, i, da, I, 1, st);
-        if (e == cudaSuccess && db) e = run_outer<TW>(low_x, *dy, ids, t, n, R, o, db, 1, R, st);
-        return e;
-    };
-    const cudaError_t e = ad->type == HYMOE_TYPE_F16 ? go(__half{}) : go(__nv_bfloat16{});
+    cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
+    if (e == cudaSuccess && (dx || da)) e = run_low(plan, *dy, ad->b, ad->type, true, ad->scale, low_dy, t, R, o, n_sms, st);
+    if (e == cudaSuccess && dx) e = run_wide(plan, low_dy, ad->a, ad->type, true, base, *dx, t, R, i, n_sms, st);
+    if (e == cudaSuccess && db) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low_x, t, R, i, n_sms, st);
+    if (e == cudaSuccess && da) e = run_grad(plan, low_dy, *x, da, part, t, n, R, i, 1, i, st);
+    if (e == cudaSuccess && db) e = run_grad(plan, low_x, *dy, db, part, t, n, R, o, R, 1, st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt_backward: kernel launch failed");
     return HYMOE_OK;
 }

@@ -1,0 +1,176 @@
+// adapt.cuh — shared by the adapter kernels (adapt.cu, adapt_low.cu, adapt_wide.cu,
+// adapt_grad.cu): the plan's lists, shared-memory tiles, mma.sync wrappers and the splitting of
+// fp32 operands.
+//
+// Tiles in shared memory have rows padded so that a row is an odd number of 16-byte pieces (fp32
+// tiles read in 8-byte pairs: 32 bytes of padding): the eight rows of an ldmatrix, and the rows of
+// a fragment access, fall into different banks.
+//
+// Fragment layouts are those of mma.sync (thread g = lane / 4, t = lane % 4).  An m16n8k16
+// fragment of 16-bit values holds k = 2t, 2t+1 in one register; taken as the k = t and t + 4 of an
+// m16n8k8 tf32 fragment on both operands, the same registers feed a tf32 product: the sum over k
+// does not mind the order.  Every 16-bit value is exact in tf32, and an fp32 value is the sum of two
+// tf32 parts to 2^-22.
+#pragma once
+
+#include "common.cuh"
+#include "entry.h"
+
+namespace hymoe {
+
+constexpr int kAdRows = 64;         // token rows of a tile
+constexpr int kAdThreads = 128;     // four warps of 16 rows
+constexpr int kAdGradCols = 128;    // columns of a gradient tile
+
+// Rank padded to the kernels' sizes.
+__host__ __device__ constexpr int adapt_rp(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
+
+// Tokens of one gradient item: long adapters are split so that their pieces run side by side (the
+// pieces' sums are added in order by a second kernel); at most about 64 pieces in all.
+__host__ __device__ constexpr int adapt_chunk(int T) {
+    return T <= 32768 ? 1024 : ((T + 31) / 32 + 63) / 64 * 64;
+}
+
+// What the plan kernel writes: tokens in the order of their adapters (stable; those without one
+// last) and the work lists over that order.
+struct AdaptPlan {
+    int* perm;       // [T] token of each sorted row
+    int4* tiles;     // {adapter or -1, first row, rows, 0} of at most kAdRows rows
+    int4* items;     // gradients: {adapter, first row, rows, partial slot or -1}; every adapter has one
+    int* pieces;     // gradients: [n + 1] first item of each adapter (items are adapter-major)
+    int* n_lists;    // [0] tiles, [1] items
+    int max_tiles, max_items;
+};
+
+struct AdaptLow {      // low[row, j] = scale[a] * sum_k X[perm[row], k] W_a(j, k), rows in sorted order
+    AdaptPlan plan;
+    const void* x;
+    size_t ldx;        // elements
+    const void* w;     // [n] matrices of R x K (trans: K x R)
+    const float* scale;
+    float* low;        // [T, RP]
+    int K, R;
+    int vec_x, vec_w;  // rows start on 16-byte boundaries
+};
+struct AdaptWide {     // out[t, o] = base[t, o] + sum_j low[row, j] W_a(o, j)
+    AdaptPlan plan;
+    const float* low;
+    const void* w;     // [n] matrices of N x R (trans: R x N)
+    const void* base;  // nullptr: zeros
+    void* out;
+    size_t ldb, ldo;
+    int N, R;
+    int vec_w, vec_b, vec_o;
+    int in_place;      // base is out: rows without an adapter need no copy
+};
+struct AdaptGrad {     // G_a(m, j) = sum over a's rows of X[perm[row], m] low[row, j]
+    AdaptPlan plan;
+    const float* low;  // [T, RP]
+    const void* x;
+    size_t ldx;
+    float* g;          // [n] matrices: element (m, j) at m * gm + j * gj
+    float* part;       // partial slots of M * R
+    int M, R, gm, gj;
+    int vec_x;
+};
+
+// type_x: HYMOE_TYPE_F32 or type_w; trans: the weight matrix has the rank as its fast dimension
+// (low) or the columns as its fast dimension (wide).
+cudaError_t launch_adapt_low(const AdaptLow& a, int type_x, int type_w, bool trans, int T, int n_sms, cudaStream_t st);
+cudaError_t launch_adapt_wide(const AdaptWide& a, int type_y, int type_w, bool trans, int T, int n_sms, cudaStream_t st);
+cudaError_t launch_adapt_grad(const AdaptGrad& a, int type_x, int T, int n, cudaStream_t st);
+
+#ifdef __CUDACC__
+
+constexpr int ad_pad16(int bytes) { return (bytes / 16 % 2 == 0) ? bytes + 16 : bytes; }  // odd number of pieces
+
+__device__ __forceinline__ void cp_async16_part(void* dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+
+// One 16-byte piece of a row into shared memory: `n` of its elements exist (the rest become 0).
+// src must be a valid address also where n == 0.
+template <int ES>
+__device__ __forceinline__ void ad_copy_piece(char* dst, const char* src, int n, bool vec) {
+    constexpr int P = 16 / ES;
+    n = n < 0 ? 0 : n > P ? P : n;
+    if (vec) {
+        cp_async16_part(dst, src, n * ES);
+    } else {
+        uint32_t v[4] = {0u, 0u, 0u, 0u};
+        if constexpr (ES == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < n) v[i] = reinterpret_cast<const uint32_t*>(src)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < n) v[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(src)[i]) << (16 * (i & 1));
+        }
+        *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+template <typename W>
+struct AdType;
+template <>
+struct AdType<__half> {
+    static constexpr bool kScaled = true;  // a row of fp32 values needs a power of two before it is split
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    // the two values of a register as fp32
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+template <>
+struct AdType<__nv_bfloat16> {
+    static constexpr bool kScaled = false;
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// v = hi + lo, both tf32 (their low 13 bits are 0, or ignored by the product): lo is exact in fp32.
+__device__ __forceinline__ void split_tf32(float v, uint32_t& hi, uint32_t& lo) {
+    hi = __float_as_uint(v) & 0xffffe000u;
+    lo = __float_as_uint(v - __uint_as_float(hi));
+}
+
+#endif  // __CUDACC__
+
+}  // namespace hymoe
