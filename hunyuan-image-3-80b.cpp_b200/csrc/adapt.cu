@@ -26,42 +26,22 @@ __host__ __device__ constexpr int plan_rows(int n) {
     return fit < 32 ? fit : 32;
 }
 
-// Exclusive prefix sum of v[0, n) in place, v[n] = the sum; all threads of the CTA.
-__device__ void block_scan(int* v, int n) {
-    __shared__ int wsum[33];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (n + kPlanThreads - 1) / kPlanThreads, lo = min(n, tid * per), hi = min(n, lo + per);
-    __syncthreads();
-    int s = 0;
-    for (int i = lo; i < hi; ++i) s += v[i];
-    int inc = s;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(kAll, inc, o);
-        if (lane >= o) inc += u;
-    }
-    if (lane == 31) wsum[warp] = inc;
-    __syncthreads();
-    if (warp == 0) {
-        const int w = wsum[lane];
-        int winc = w;
+// Exclusive prefix sum of v[0, n) in place, v[n] = the sum; one warp.
+__device__ void warp_scan(int* v, int n) {
+    const int lane = threadIdx.x & 31;
+    int run = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int x = i0 + lane < n ? v[i0 + lane] : 0;
+        int inc = x;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(kAll, winc, o);
-            if (lane >= o) winc += u;
+            const int u = __shfl_up_sync(kAll, inc, o);
+            if (lane >= o) inc += u;
         }
-        wsum[lane] = winc - w;
-        if (lane == 31) wsum[32] = winc;
+        if (i0 + lane < n) v[i0 + lane] = run + inc - x;
+        run += __shfl_sync(kAll, inc, 31);
     }
-    __syncthreads();
-    int run = wsum[warp] + inc - s;
-    for (int i = lo; i < hi; ++i) {
-        const int x = v[i];
-        v[i] = run;
-        run += x;
-    }
-    if (tid == 0) v[n] = wsum[32];
-    __syncthreads();
+    if (lane == 0) v[n] = run;
 }
 
 // Largest b with pre[b] <= i, of pre[0..n] ascending, pre[n] > i.
@@ -77,7 +57,9 @@ __device__ __forceinline__ int bucket_of(const int* pre, int n, int i) {
 
 // Stable counting sort of the tokens by adapter and the lists over the sorted rows, by one CTA:
 // each counting warp owns a run of tokens (in order) and a row of counters, 32 tokens a step; the
-// lanes of equal adapters find one another by a warp match.  8192 tokens take 8 steps, twice.
+// lanes of equal adapters find one another by a ballot for every bit of the adapter's number (a
+// warp match takes a step for every distinct adapter: 16 us instead of 6 at 8192 tokens of 16).
+// Up to 8192 tokens the adapters stay in registers between counting and placing.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restrict__ ids, int T, int n, AdaptPlan p,
                                                             int chunk) {
     extern __shared__ int sm[];
@@ -86,65 +68,85 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
     int *off = sm, *tpre = off + n + 2, *ipre = tpre + n + 2, *spre = ipre + n + 2, *tot = spre + n + 2;
     int* cnt = tot + n + 2;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, W = plan_rows(n);
-    for (int i = tid; i < W * nb; i += kPlanThreads) cnt[i] = 0;
-    __syncthreads();
     const int per = ((T + W - 1) / W + 31) / 32 * 32;
     const int64_t lo64 = static_cast<int64_t>(warp) * per;
     const int t_lo = lo64 < T ? static_cast<int>(lo64) : T, t_hi = warp < W ? min(T, t_lo + per) : t_lo;
-    int* mine = cnt + (warp < W ? warp : 0) * nb;
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int t0 = t_lo; t0 < t_hi; t0 += 32 * 8) {
-            int b[8];
+    const int bits = 32 - __clz(n);
+    int b[8];
+    auto fetch = [&](int t0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int t = t0 + 32 * i + lane;
-                int v = ids != nullptr && t < t_hi ? __ldg(ids + t) : 0;
-                if (v < 0 || v >= n) v = n;
-                b[i] = t < t_hi ? v : -1;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (t0 + 32 * i >= t_hi) break;
-                const unsigned same = __match_any_sync(kAll, b[i]);
-                const int before = __popc(same & ((1u << lane) - 1u));
-                if (pass == 0) {
-                    if (b[i] >= 0 && before == 0) mine[b[i]] += __popc(same);
-                } else {
-                    const int at = b[i] >= 0 ? mine[b[i]] + before : 0;
-                    __syncwarp();
-                    if (b[i] >= 0) {
-                        p.perm[at] = t0 + 32 * i + lane;
-                        if (before == 0) mine[b[i]] = at + __popc(same);
-                    }
-                }
-                __syncwarp();
-            }
+        for (int i = 0; i < 8; ++i) {
+            const int t = t0 + 32 * i + lane;
+            int v = ids != nullptr && t < t_hi ? __ldg(ids + t) : 0;
+            if (v < 0 || v >= n) v = n;
+            b[i] = t < t_hi ? v : -1;
         }
-        if (pass == 1) break;
-        __syncthreads();
-        for (int a = tid; a < nb; a += kPlanThreads) {
-            int c = 0;
-            for (int w = 0; w < W; ++w) c += cnt[w * nb + a];
-            tot[a] = c;
-            off[a] = c;
-            tpre[a] = (c + kAdRows - 1) / kAdRows;
-            const int pieces = a < n ? max(1, (c + chunk - 1) / chunk) : 0;
+    };
+    auto equals = [&](int v) {  // lanes with the same v
+        unsigned same = __ballot_sync(kAll, v >= 0);
+        if (v < 0) same = ~same;
+        for (int k = 0; k < bits; ++k) {
+            const unsigned one = __ballot_sync(kAll, v >> k & 1);
+            same &= v >> k & 1 ? one : ~one;
+        }
+        return same;
+    };
+    fetch(t_lo);
+    for (int i = tid; i < W * nb; i += kPlanThreads) cnt[i] = 0;
+    for (int i = tid; i < p.max_tiles; i += kPlanThreads) p.counters[i] = 0u;
+    __syncthreads();
+    int* mine = cnt + (warp < W ? warp : 0) * nb;
+    for (int t0 = t_lo; t0 < t_hi; t0 += 256) {
+        if (t0 > t_lo) fetch(t0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (t0 + 32 * i >= t_hi) break;
+            const unsigned same = equals(b[i]);
+            if (b[i] >= 0 && (same & ((1u << lane) - 1u)) == 0) mine[b[i]] += __popc(same);
+            __syncwarp();
+        }
+    }
+    __syncthreads();
+    for (int a = warp; a < nb; a += kPlanThreads / 32) {  // every run's start among the adapter's tokens
+        const int c = lane < W ? cnt[lane * nb + a] : 0;
+        int inc = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(kAll, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (lane < W) cnt[lane * nb + a] = inc - c;
+        if (lane == 31) {
+            tot[a] = inc;
+            off[a] = inc;
+            tpre[a] = (inc + kAdRows - 1) / kAdRows;
+            const int pieces = a < n ? max(1, (inc + chunk - 1) / chunk) : 0;
             ipre[a] = pieces;
             spre[a] = pieces > 1 ? pieces : 0;
         }
-        block_scan(off, nb);
-        block_scan(tpre, nb);
-        block_scan(ipre, n);
-        block_scan(spre, n);
-        for (int a = tid; a < nb; a += kPlanThreads) {
-            int run = off[a];
-            for (int w = 0; w < W; ++w) {
-                const int c = cnt[w * nb + a];
-                cnt[w * nb + a] = run;
-                run += c;
+    }
+    __syncthreads();
+    if (warp == 0) warp_scan(off, nb);
+    if (warp == 1) warp_scan(tpre, nb);
+    if (warp == 2) warp_scan(ipre, n);
+    if (warp == 3) warp_scan(spre, n);
+    __syncthreads();
+    if (t_hi - t_lo > 256) fetch(t_lo);
+    for (int t0 = t_lo; t0 < t_hi; t0 += 256) {
+        if (t0 > t_lo) fetch(t0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (t0 + 32 * i >= t_hi) break;
+            const unsigned same = equals(b[i]);
+            const int before = __popc(same & ((1u << lane) - 1u));
+            const int at = b[i] >= 0 ? mine[b[i]] : 0;
+            __syncwarp();
+            if (b[i] >= 0) {
+                p.perm[off[b[i]] + at + before] = t0 + 32 * i + lane;
+                if (before == 0) mine[b[i]] = at + __popc(same);
             }
+            __syncwarp();
         }
-        __syncthreads();
     }
     const int n_tiles = tpre[nb];
     for (int i = tid; i < n_tiles; i += kPlanThreads) {
@@ -168,13 +170,13 @@ cudaError_t launch_plan_adapt(const int* ids, int T, int n, const AdaptPlan& p, 
     const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanSmem);
     if (e != cudaSuccess) return e;
     const size_t smem = sizeof(int) * (5 * (static_cast<size_t>(n) + 2) + static_cast<size_t>(plan_rows(n)) * (n + 1));
-    plan_kernel<<<1, kPlanThreads, smem, st>>>(ids, T, n, p, adapt_chunk(T));
+    plan_kernel<<<1, kPlanThreads, smem, st>>>(ids, T, n, p, adapt_chunk(T, n));
     return cudaGetLastError();
 }
 
 // The workspace: every part starts on 256 bytes.
 struct AdaptLayout {
-    size_t perm, tiles, items, pieces, lists, low, low2, part, bytes;
+    size_t perm, tiles, items, pieces, lists, counters, low, low2, low_part, part, bytes;
     int max_tiles, max_items;
 };
 AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward) {
@@ -186,13 +188,16 @@ AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward) {
         return at;
     };
     if (T == 0) return l;
-    const size_t long_pieces = T / 1024 < 32 ? T / 1024 : 32;  // T / adapt_chunk(T) at most
+    const size_t long_pieces = T / kAdMinChunk < kAdMaxPieces ? T / kAdMinChunk : kAdMaxPieces;  // T / adapt_chunk at most
     l.max_tiles = static_cast<int>(T / kAdRows + (n + 1 < T ? n + 1 : T));
     l.max_items = static_cast<int>(n + long_pieces);
     l.lists = take(2 * sizeof(int));
     l.perm = take(T * sizeof(int));
     l.tiles = take(static_cast<size_t>(l.max_tiles) * sizeof(int4));
+    l.counters = take(static_cast<size_t>(l.max_tiles) * sizeof(unsigned));
     l.low = take(T * adapt_rp(ad->rank) * sizeof(float));
+    const size_t shared_tiles = static_cast<size_t>(l.max_tiles) * kAdMaxSplits;
+    l.low_part = take((shared_tiles < kAdMaxSlots ? shared_tiles : kAdMaxSlots) * kAdRows * adapt_rp(ad->rank) * sizeof(float));
     if (backward) {
         l.items = take(static_cast<size_t>(l.max_items) * sizeof(int4));
         l.pieces = take((n + 1) * sizeof(int));
@@ -209,6 +214,7 @@ AdaptPlan plan_in(const AdaptLayout& l, char* ws, bool backward) {
     p.items = backward ? reinterpret_cast<int4*>(ws + l.items) : nullptr;
     p.pieces = backward ? reinterpret_cast<int*>(ws + l.pieces) : nullptr;
     p.n_lists = reinterpret_cast<int*>(ws + l.lists);
+    p.counters = reinterpret_cast<unsigned*>(ws + l.counters);
     p.max_tiles = l.max_tiles;
     p.max_items = l.max_items;
     return p;
@@ -275,8 +281,15 @@ hymoe_status current_device(int* dev) {
     return entry_fail(HYMOE_ERR_CUDA, "cudaGetDevice failed");
 }
 
+// SMs that the launches are sized for (the workspace's bound on partial sums assumes at most this).
+int sm_count(int dev) {
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n < 1 ? 1 : n < kAdMaxSlots / 4 ? n : kAdMaxSlots / 4;
+}
+
 cudaError_t run_low(const AdaptPlan& plan, const hymoe_mat& x, const void* w, int type_w, bool trans, const float* scale,
-                    float* low, int T, int R, int K, int n_sms, cudaStream_t st) {
+                    float* low, float* part, int R, int K, int n_sms, cudaStream_t st) {
     AdaptLow a{};
     a.plan = plan;
     a.x = x.data;
@@ -284,15 +297,16 @@ cudaError_t run_low(const AdaptPlan& plan, const hymoe_mat& x, const void* w, in
     a.w = w;
     a.scale = scale;
     a.low = low;
+    a.part = part;
     a.K = K;
     a.R = R;
     a.vec_x = rows_vec(x.data, a.ldx, elem_bytes(x.type));
     a.vec_w = rows_vec(w, trans ? R : K, 2);
-    return launch_adapt_low(a, x.type, type_w, trans, T, n_sms, st);
+    return launch_adapt_low(a, x.type, type_w, trans, n_sms, st);
 }
 
 cudaError_t run_wide(const AdaptPlan& plan, const float* low, const void* w, int type_w, bool trans, const hymoe_mat* base,
-                     const hymoe_mat& out, int T, int R, int N, int n_sms, cudaStream_t st) {
+                     const hymoe_mat& out, int R, int N, int n_sms, cudaStream_t st) {
     const size_t es = elem_bytes(out.type);
     AdaptWide a{};
     a.plan = plan;
@@ -308,7 +322,7 @@ cudaError_t run_wide(const AdaptPlan& plan, const float* low, const void* w, int
     a.vec_b = base ? rows_vec(base->data, a.ldb, es) : 0;
     a.vec_o = rows_vec(out.data, a.ldo, es);
     a.in_place = base && base->data == out.data;
-    return launch_adapt_wide(a, out.type, type_w, trans, T, n_sms, st);
+    return launch_adapt_wide(a, out.type, type_w, trans, n_sms, st);
 }
 
 cudaError_t run_grad(const AdaptPlan& plan, const float* low, const hymoe_mat& x, float* g, float* part, int T, int n,
@@ -366,15 +380,15 @@ extern "C" hymoe_status hymoe_adapt(const hymoe_adapters* ad, const hymoe_mat* x
         return entry_fail(HYMOE_ERR_INVALID_ARG, "hymoe_adapt: every pointer must be memory of the current device");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int n = static_cast<int>(ad->n_adapters), R = static_cast<int>(ad->rank), t = static_cast<int>(T);
-    int n_sms = 0;
-    cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, dev);
+    const int n_sms = sm_count(dev);
     const AdaptLayout l = adapt_layout(ad, T, false);
     char* ws = static_cast<char*>(workspace);
     const AdaptPlan plan = plan_in(l, ws, false);
     float* low = reinterpret_cast<float*>(ws + l.low);
+    float* low_part = reinterpret_cast<float*>(ws + l.low_part);
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
-    if (e == cudaSuccess) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low, t, R, static_cast<int>(I), n_sms, st);
-    if (e == cudaSuccess) e = run_wide(plan, low, ad->b, ad->type, false, base, *out, t, R, static_cast<int>(O), n_sms, st);
+    if (e == cudaSuccess) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low, low_part, R, static_cast<int>(I), n_sms, st);
+    if (e == cudaSuccess) e = run_wide(plan, low, ad->b, ad->type, false, base, *out, R, static_cast<int>(O), n_sms, st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt: kernel launch failed");
     return HYMOE_OK;
 }
@@ -430,19 +444,19 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
         }
         return HYMOE_OK;
     }
-    int n_sms = 0;
-    cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, dev);
+    const int n_sms = sm_count(dev);
     const AdaptLayout l = adapt_layout(ad, T, true);
     char* ws = static_cast<char*>(workspace);
     const AdaptPlan plan = plan_in(l, ws, true);
     float* low_dy = reinterpret_cast<float*>(ws + l.low);
     float* low_x = reinterpret_cast<float*>(ws + l.low2);
+    float* low_part = reinterpret_cast<float*>(ws + l.low_part);
     float* part = reinterpret_cast<float*>(ws + l.part);
     const int i = static_cast<int>(I), o = static_cast<int>(O);
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
-    if (e == cudaSuccess && (dx || da)) e = run_low(plan, *dy, ad->b, ad->type, true, ad->scale, low_dy, t, R, o, n_sms, st);
-    if (e == cudaSuccess && dx) e = run_wide(plan, low_dy, ad->a, ad->type, true, base, *dx, t, R, i, n_sms, st);
-    if (e == cudaSuccess && db) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low_x, t, R, i, n_sms, st);
+    if (e == cudaSuccess && (dx || da)) e = run_low(plan, *dy, ad->b, ad->type, true, ad->scale, low_dy, low_part, R, o, n_sms, st);
+    if (e == cudaSuccess && dx) e = run_wide(plan, low_dy, ad->a, ad->type, true, base, *dx, R, i, n_sms, st);
+    if (e == cudaSuccess && db) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low_x, low_part, R, i, n_sms, st);
     if (e == cudaSuccess && da) e = run_grad(plan, low_dy, *x, da, part, t, n, R, i, 1, i, st);
     if (e == cudaSuccess && db) e = run_grad(plan, low_x, *dy, db, part, t, n, R, o, R, 1, st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt_backward: kernel launch failed");

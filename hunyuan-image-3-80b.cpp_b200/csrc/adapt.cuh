@@ -25,10 +25,28 @@ constexpr int kAdGradCols = 128;    // columns of a gradient tile
 // Rank padded to the kernels' sizes.
 __host__ __device__ constexpr int adapt_rp(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
-// Tokens of one gradient item: long adapters are split so that their pieces run side by side (the
-// pieces' sums are added in order by a second kernel); at most about 64 pieces in all.
-__host__ __device__ constexpr int adapt_chunk(int T) {
-    return T <= 32768 ? 1024 : ((T + 31) / 32 + 63) / 64 * 64;
+// Tokens of one gradient item.  An adapter of average length stays whole; a long one is cut into
+// pieces that run side by side (their sums are added in order by a second kernel), five where it
+// has all the tokens, at most eight.
+constexpr int kAdMinChunk = 512, kAdMaxPieces = 8;
+__host__ __device__ constexpr int adapt_chunk(int T, int n) {
+    const int avg = static_cast<int>(static_cast<int64_t>(T) * 3 / (2 * static_cast<int64_t>(n))), fifth = T / 5;
+    int c = avg < fifth ? avg : fifth;
+    const int least = (T + kAdMaxPieces - 1) / kAdMaxPieces;
+    c = c < least ? least : c;
+    c = c < kAdMinChunk ? kAdMinChunk : c;
+    return (c + 63) / 64 * 64;
+}
+
+// CTAs that share a tile of the narrow product over K columns: as many as the `slots` of the GPU
+// leave for each of `tiles` tiles, each with two blocks of 64 columns at least.
+constexpr int kAdMaxSplits = 16;
+constexpr int kAdMaxSlots = 640;  // CTAs that a GPU is taken to hold at most (four on each of 160 SMs)
+__host__ __device__ constexpr int adapt_splits(int tiles, int K, int slots) {
+    const int nk = (K + 63) / 64;
+    int s = slots / tiles < nk / 2 ? slots / tiles : nk / 2;
+    s = s < kAdMaxSplits ? s : kAdMaxSplits;
+    return s < 1 ? 1 : s;
 }
 
 // What the plan kernel writes: tokens in the order of their adapters (stable; those without one
@@ -39,6 +57,7 @@ struct AdaptPlan {
     int4* items;     // gradients: {adapter, first row, rows, partial slot or -1}; every adapter has one
     int* pieces;     // gradients: [n + 1] first item of each adapter (items are adapter-major)
     int* n_lists;    // [0] tiles, [1] items
+    unsigned* counters;  // [max_tiles] CTAs of a tile that have left their partial sums (0 between launches)
     int max_tiles, max_items;
 };
 
@@ -49,6 +68,7 @@ struct AdaptLow {      // low[row, j] = scale[a] * sum_k X[perm[row], k] W_a(j, 
     const void* w;     // [n] matrices of R x K (trans: K x R)
     const float* scale;
     float* low;        // [T, RP]
+    float* part;       // [max_tiles * S] partial sums of 64 x RP
     int K, R;
     int vec_x, vec_w;  // rows start on 16-byte boundaries
 };
@@ -76,8 +96,8 @@ struct AdaptGrad {     // G_a(m, j) = sum over a's rows of X[perm[row], m] low[r
 
 // type_x: HYMOE_TYPE_F32 or type_w; trans: the weight matrix has the rank as its fast dimension
 // (low) or the columns as its fast dimension (wide).
-cudaError_t launch_adapt_low(const AdaptLow& a, int type_x, int type_w, bool trans, int T, int n_sms, cudaStream_t st);
-cudaError_t launch_adapt_wide(const AdaptWide& a, int type_y, int type_w, bool trans, int T, int n_sms, cudaStream_t st);
+cudaError_t launch_adapt_low(const AdaptLow& a, int type_x, int type_w, bool trans, int n_sms, cudaStream_t st);
+cudaError_t launch_adapt_wide(const AdaptWide& a, int type_y, int type_w, bool trans, int n_sms, cudaStream_t st);
 cudaError_t launch_adapt_grad(const AdaptGrad& a, int type_x, int T, int n, cudaStream_t st);
 
 #ifdef __CUDACC__

@@ -1,10 +1,14 @@
 // adapt_grad.cu — the adapters' gradients: for every adapter, the sum over its tokens of the outer
 // products of a long row (x or dy) and its narrow counterpart (low).
 //
-// A CTA takes 128 columns of the long rows and one item of the plan (an adapter's tokens, or 1024
-// of them), 32 tokens at a time; the matrix pipe sums over the tokens.  low is held in two tf32
-// parts, so that the fp32 results keep fp32's digits.  Items that are pieces of one adapter write
-// partial sums, which a second kernel adds in order.
+// A CTA takes 128 columns of the long rows and one item of the plan (an adapter's tokens, or a
+// piece of a long adapter's), 32 tokens at a time; the matrix pipe sums over the 32 tokens, and
+// the sums of the blocks are added in fp32 outside it: the pipe truncates what it adds, which over
+// a thousand tokens cost 5e-6 of the result instead of 1e-6.  low is held in two bf16 parts beside
+// bf16 rows (2^-17 of each value), in two tf32 parts beside others.  Items that are pieces of one
+// adapter write partial sums, which a second kernel adds in order.
+#include <type_traits>
+
 #include "adapt.cuh"
 #include "kernels.h"
 
@@ -22,7 +26,10 @@ struct GradTile {
     static constexpr int kXBytes = kGradTok * kXRow;
     static constexpr int kLBytes = kGradTok * kLRow;
     static constexpr int kStage = kXBytes + kLBytes;
-    static constexpr int kSmem = kStage * kGradStages;
+    static constexpr bool kParts = std::is_same<X, __nv_bfloat16>::value;  // 16-bit parts of low
+    static constexpr int kPRow = ad_pad16(RP * 2);
+    static constexpr int kPBytes = kGradTok * kPRow;  // one part of a block
+    static constexpr int kSmem = kStage * kGradStages + (kParts ? 2 * kPBytes : 0);
 };
 
 template <typename X, int RP>
@@ -62,13 +69,13 @@ __global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant_
         }
     };
 
-    float acc[2][RP / 8][4];  // this warp's 32 columns m x RP
+    float sum[2][RP / 8][4];  // this warp's 32 columns m x RP
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < RP / 8; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.f;
+            for (int q = 0; q < 4; ++q) sum[i][j][q] = 0.f;
 
 #pragma unroll
     for (int s = 0; s < kGradStages - 1; ++s) {
@@ -84,6 +91,47 @@ __global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant_
         cp_async_commit();
         const char* xs = smem + stage * L::kStage;
         const float* ls = reinterpret_cast<const float*>(xs + L::kXBytes);
+        float acc[2][RP / 8][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.f;
+        if constexpr (L::kParts) {
+            char* ps = smem + kGradStages * L::kStage;
+#pragma unroll
+            for (int i = 0; i < kGradTok * RP / 4 / kAdThreads; ++i) {
+                const int p = tid + i * kAdThreads, r = p / (RP / 4), c = p % (RP / 4) * 4;
+                const float4 v = *reinterpret_cast<const float4*>(ls + r * (RP + 4) + c);
+                const uint32_t h0 = AdType<X>::pack(v.x, v.y), h1 = AdType<X>::pack(v.z, v.w);
+                const float2 b0 = AdType<X>::unpack(h0), b1 = AdType<X>::unpack(h1);
+                *reinterpret_cast<uint2*>(ps + r * L::kPRow + c * 2) = make_uint2(h0, h1);
+                *reinterpret_cast<uint2*>(ps + L::kPBytes + r * L::kPRow + c * 2) =
+                    make_uint2(AdType<X>::pack(v.x - b0.x, v.y - b0.y), AdType<X>::pack(v.z - b1.x, v.w - b1.y));
+            }
+            __syncthreads();
+#pragma unroll
+            for (int kk = 0; kk < kGradTok / 16; ++kk) {
+                uint32_t af[2][4];  // X^T: rows m, k = tokens
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    ldsm4_t(af[i], smem_u32(xs) + (kk * 16 + (lane >> 4) * 8 + (lane & 7)) * L::kXRow +
+                                       (warp * 32 + i * 16 + (lane >> 3 & 1) * 8) * 2);
+#pragma unroll
+                for (int j = 0; j < RP / 16; ++j)
+#pragma unroll
+                    for (int part = 1; part >= 0; --part) {
+                        uint32_t bf[4];
+                        ldsm4_t(bf, smem_u32(ps) + part * L::kPBytes + (kk * 16 + (lane & 15)) * L::kPRow + (j * 16 + (lane >> 4) * 8) * 2);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            AdType<X>::mma(acc[i][2 * j], af[i], bf[0], bf[1]);
+                            AdType<X>::mma(acc[i][2 * j + 1], af[i], bf[2], bf[3]);
+                        }
+                    }
+            }
+        } else {
 #pragma unroll
         for (int kk = 0; kk < kGradTok / 16; ++kk) {
             // A: X^T, rows m, k = tokens; v[i][h][q]: tokens 8h + 2t, 2t + 1 of column m = 16 i + g + 8 q
@@ -135,6 +183,13 @@ __global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant_
                 }
             }
         }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) sum[i][j][q] += acc[i][j][q];
     }
     cp_async_wait<0>();
     float* out = item.w >= 0 ? a.part + static_cast<size_t>(item.w) * a.M * a.R : a.g + static_cast<size_t>(item.x) * a.M * a.R;
@@ -145,7 +200,7 @@ __global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant_
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int m = m0 + warp * 32 + i * 16 + g + 8 * (q >> 1), c = j * 8 + 2 * t + (q & 1);
-                if (m < a.M && c < a.R) out[static_cast<size_t>(m) * a.gm + static_cast<size_t>(c) * a.gj] = acc[i][j][q];
+                if (m < a.M && c < a.R) out[static_cast<size_t>(m) * a.gm + static_cast<size_t>(c) * a.gj] = sum[i][j][q];
             }
 }
 
@@ -170,7 +225,7 @@ cudaError_t launch_t(const AdaptGrad& a, int T, int n, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
     e = launch_kernel(true, kern, dim3(a.plan.max_items, (a.M + kAdGradCols - 1) / kAdGradCols), dim3(kAdThreads), L::kSmem, st, a);
-    if (e != cudaSuccess || T <= adapt_chunk(T)) return e;  // no adapter can have two pieces
+    if (e != cudaSuccess || T <= adapt_chunk(T, n)) return e;  // no adapter can have two pieces
     const size_t size = static_cast<size_t>(a.M) * a.R, blk = (size + 255) / 256;
     return launch_kernel(true, grad_join_kernel, dim3(static_cast<unsigned>(blk < 1024 ? blk : 1024), n), dim3(256), 0, st, a);
 }

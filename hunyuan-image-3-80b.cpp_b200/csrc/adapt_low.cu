@@ -1,9 +1,10 @@
 // adapt_low.cu — the adapters' narrow product: low[row] = scale[a] * W_a x[token of row].
 //
-// A tile of 64 sorted rows of one adapter is one cluster of S CTAs (S = 1, 2, 4, 8), each over a
-// part of the long dimension; the S partial sums [64, RP] meet in distributed shared memory, where
-// every CTA adds its share of the rows in the order of the ranks.  Bound by reading x (the weights,
-// RP / 64 of its bytes per tile, come from L2): four stages of 64 columns are in flight per CTA.
+// A tile of 64 sorted rows of one adapter is shared by S CTAs, each over a part of the long
+// dimension.  Every CTA leaves its partial sums [64, RP] in the workspace; the last one of a tile to
+// arrive adds them in the order of the parts.  Bound by reading x (the weights, RP / 64 of its
+// bytes per tile, come from L2): four stages of 64 columns are in flight per CTA, and S is chosen
+// so that the CTAs fill the GPU once.
 #include "adapt.cuh"
 #include "kernels.h"
 
@@ -21,27 +22,19 @@ struct LowTile {
     static constexpr int kXBytes = kAdRows * kXRow;
     static constexpr int kWBytes = (TRANS ? kLowK : RP) * kWRow;
     static constexpr int kStage = kXBytes + kWBytes;
-    static constexpr int kRed = kAdRows * (RP + 4) * 4;  // partial sums
-    static constexpr int kSmem = kStage * kLowStages > kRed ? kStage * kLowStages : kRed;
+    static constexpr int kSmem = kStage * kLowStages;
+    static constexpr int kPerSm = 226 * 1024 / (kSmem + 1024) < 4 ? 226 * 1024 / (kSmem + 1024) : 4;  // CTAs on an SM
 };
 
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-
 template <typename X, typename W, int RP, bool TRANS>
-__global__ __launch_bounds__(kAdThreads) void low_kernel(const __grid_constant__ AdaptLow a, int S) {
+__global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void low_kernel(
+    const __grid_constant__ AdaptLow a, int S) {
     using L = LowTile<X, W, RP, TRANS>;
     extern __shared__ __align__(128) char smem[];
     griddep_wait();
     griddep_launch_dependents();
     const int tile_id = blockIdx.x / S, rank = blockIdx.x % S;
-    if (tile_id >= a.plan.n_lists[0]) return;  // the whole cluster
+    if (tile_id >= a.plan.n_lists[0]) return;
     const int4 tile = a.plan.tiles[tile_id];
     if (tile.x < 0) return;  // rows without an adapter
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -49,48 +42,64 @@ __global__ __launch_bounds__(kAdThreads) void low_kernel(const __grid_constant__
     const int k_lo = static_cast<int>(static_cast<int64_t>(nk) * rank / S);
     const int k_hi = static_cast<int>(static_cast<int64_t>(nk) * (rank + 1) / S);
 
-    // this thread's pieces of every stage's x tile: piece xc of rows xr0 + i * (128 / pieces)
-    constexpr int kXPieces = kLowK * static_cast<int>(sizeof(X)) / 16, kXIter = kAdRows * kXPieces / kAdThreads;
+    // this thread's pieces of every stage: piece xc of rows xr0 + i * (128 / pieces) of x, and piece
+    // p % kWPieces of row p / kWPieces of the weights, p = tid + i * 128
+    constexpr int P = 16 / static_cast<int>(sizeof(X));
+    constexpr int kXPieces = kLowK / P, kXIter = kAdRows * kXPieces / kAdThreads;
+    constexpr int kWPieces = TRANS ? RP / 8 : kLowK / 8, kWAll = (TRANS ? kLowK : RP) * kWPieces;
+    constexpr int kWIter = kWAll / kAdThreads;
+    static_assert(kWAll % kAdThreads == 0, "whole rounds of pieces");
     const int xc = tid % kXPieces, xr0 = tid / kXPieces;
-    const char* xp[kXIter];
-    unsigned xok = 0;
+    const char* xp[kXIter];  // the piece in column 0; rows that do not exist have no bytes
+    int xn[kXIter];
 #pragma unroll
     for (int i = 0; i < kXIter; ++i) {
         const int r = xr0 + i * (kAdThreads / kXPieces);
         const bool ok = r < tile.z;
         const int tok = ok ? __ldg(a.plan.perm + tile.y + r) : 0;
-        xp[i] = static_cast<const char*>(a.x) + static_cast<size_t>(tok) * a.ldx * sizeof(X);
-        if (ok) xok |= 1u << i;
+        xp[i] = static_cast<const char*>(a.x) + (static_cast<size_t>(tok) * a.ldx + (ok ? xc * P : 0)) * sizeof(X);
+        xn[i] = ok ? 16 : 0;
     }
     const char* wbase = static_cast<const char*>(a.w) + static_cast<size_t>(tile.x) * a.R * a.K * 2;
+    const char* wp[kWIter];
+    int wn[kWIter];
+#pragma unroll
+    for (int i = 0; i < kWIter; ++i) {
+        const int p = tid + i * kAdThreads, r = p / kWPieces, c = p % kWPieces * 8;
+        const bool ok = TRANS ? c < a.R : r < a.R;  // trans: row = k, columns = rank; else row = rank, columns = k
+        wp[i] = ok ? wbase + (static_cast<size_t>(r) * (TRANS ? a.R : a.K) + c) * 2 : wbase;
+        wn[i] = !ok ? 0 : TRANS ? min(16, (a.R - c) * 2) : 16;
+    }
+    const bool vec = a.vec_x && a.vec_w;
     auto load = [&](int stage, int kb) {
         char* xs = smem + stage * L::kStage;
         char* ws = xs + L::kXBytes;
         const int k0 = kb * kLowK;
-        constexpr int P = 16 / static_cast<int>(sizeof(X));
+        if (vec && k0 + kLowK <= a.K) {  // a whole block of aligned rows
+#pragma unroll
+            for (int i = 0; i < kXIter; ++i)
+                cp_async16_part(xs + (xr0 + i * (kAdThreads / kXPieces)) * L::kXRow + xc * 16,
+                                xp[i] + static_cast<size_t>(k0) * sizeof(X), xn[i]);
+            const size_t adv = static_cast<size_t>(k0) * (TRANS ? a.R : 1) * 2;
+#pragma unroll
+            for (int i = 0; i < kWIter; ++i) {
+                const int p = tid + i * kAdThreads;
+                cp_async16_part(ws + p / kWPieces * L::kWRow + p % kWPieces * 16, wn[i] ? wp[i] + adv : wbase, wn[i]);
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < kXIter; ++i) {
-            const int r = xr0 + i * (kAdThreads / kXPieces), k = k0 + xc * P;
-            const int n = (xok >> i & 1) ? a.K - k : 0;
+            const int r = xr0 + i * (kAdThreads / kXPieces), n = xn[i] ? a.K - (k0 + xc * P) : 0;
             ad_copy_piece<sizeof(X)>(xs + r * L::kXRow + xc * 16,
-                                     n > 0 ? xp[i] + static_cast<size_t>(k) * sizeof(X) : static_cast<const char*>(a.x), n, a.vec_x);
+                                     n > 0 ? xp[i] + static_cast<size_t>(k0) * sizeof(X) : static_cast<const char*>(a.x), n, a.vec_x);
         }
-        constexpr int kWPieces = TRANS ? RP / 8 : kLowK / 8, kWAll = (TRANS ? kLowK : RP) * kWPieces;
 #pragma unroll
-        for (int i = 0; i < (kWAll + kAdThreads - 1) / kAdThreads; ++i) {
-            const int p = tid + i * kAdThreads;
-            if (kWAll % kAdThreads != 0 && p >= kWAll) break;
-            const int r = p / kWPieces, c = p % kWPieces;
-            int n;
-            size_t off;
-            if (TRANS) {  // row = k, columns = rank
-                n = k0 + r < a.K ? a.R - c * 8 : 0;
-                off = static_cast<size_t>(k0 + r) * a.R + c * 8;
-            } else {      // row = rank, columns = k
-                n = r < a.R ? a.K - (k0 + c * 8) : 0;
-                off = static_cast<size_t>(r) * a.K + k0 + c * 8;
-            }
-            ad_copy_piece<2>(ws + r * L::kWRow + c * 16, n > 0 ? wbase + off * 2 : wbase, n, a.vec_w);
+        for (int i = 0; i < kWIter; ++i) {
+            const int p = tid + i * kAdThreads, r = p / kWPieces, c = p % kWPieces;
+            const int n = wn[i] == 0 ? 0 : TRANS ? (k0 + r < a.K ? a.R - c * 8 : 0) : a.K - (k0 + c * 8);
+            ad_copy_piece<2>(ws + r * L::kWRow + c * 16,
+                             n > 0 ? wp[i] + static_cast<size_t>(k0) * (TRANS ? a.R : 1) * 2 : wbase, n, a.vec_w);
         }
     };
 
@@ -161,81 +170,72 @@ __global__ __launch_bounds__(kAdThreads) void low_kernel(const __grid_constant__
         }
     }
     cp_async_wait<0>();
-    __syncthreads();  // the stages become the partial sums
-    {
-        float* red = reinterpret_cast<float*>(smem);
-        const int g = lane >> 2, t = lane & 3;
+    const float f = a.scale != nullptr ? __ldg(a.scale + tile.x) : 1.f;
+    const int g = lane >> 2, t = lane & 3;
+    float* dst = S == 1 ? a.low + static_cast<size_t>(tile.y) * RP
+                        : a.part + (static_cast<size_t>(tile_id) * S + rank) * (kAdRows * RP);
+    const float f1 = S == 1 ? f : 1.f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int r = warp * 16 + g + 8 * q;
+        if (r >= tile.z) continue;
 #pragma unroll
         for (int j = 0; j < RP / 8; ++j)
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-                *reinterpret_cast<float2*>(red + (warp * 16 + g + 8 * q) * (RP + 4) + j * 8 + 2 * t) =
-                    make_float2(acc[j][2 * q], acc[j][2 * q + 1]);
+            *reinterpret_cast<float2*>(dst + static_cast<size_t>(r) * RP + j * 8 + 2 * t) =
+                make_float2(acc[j][2 * q] * f1, acc[j][2 * q + 1] * f1);
     }
-    cluster_sync();
-    const float f = a.scale != nullptr ? __ldg(a.scale + tile.x) : 1.f;
-    const int rows = kAdRows / S;
-    for (int p = tid; p < rows * (RP / 4); p += kAdThreads) {
-        const int r = rank * rows + p / (RP / 4), c = p % (RP / 4) * 4;
-        if (r >= tile.z) continue;
+    if (S == 1) return;
+    // The tile's last CTA adds the parts.  Its counter wraps back to 0 for the next call.
+    __shared__ int last;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) last = atomicInc(a.plan.counters + tile_id, S - 1) == static_cast<unsigned>(S - 1);
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    const float* part = a.part + static_cast<size_t>(tile_id) * S * (kAdRows * RP);
+    for (int p = tid; p < tile.z * (RP / 4); p += kAdThreads) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int q = 0; q < S; ++q) {
-            const float4 v = ld_cluster4(mapa_shared(smem + (r * (RP + 4) + c) * 4, q));
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + static_cast<size_t>(q) * (kAdRows * RP)) + p);
             s.x += v.x;
             s.y += v.y;
             s.z += v.z;
             s.w += v.w;
         }
-        *reinterpret_cast<float4*>(a.low + static_cast<size_t>(tile.y + r) * RP + c) =
-            make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+        reinterpret_cast<float4*>(a.low + static_cast<size_t>(tile.y) * RP)[p] = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
     }
-    cluster_sync();  // no CTA leaves while another reads its sums
 }
 
 template <typename X, typename W, int RP, bool TRANS>
-cudaError_t launch_t(const AdaptLow& a, int T, int n_sms, cudaStream_t st) {
+cudaError_t launch_t(const AdaptLow& a, int n_sms, cudaStream_t st) {
     using L = LowTile<X, W, RP, TRANS>;
     auto kern = low_kernel<X, W, RP, TRANS>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
-    // enough CTAs for two on every SM, each with at least four stages of columns
-    const int tiles = (T + kAdRows - 1) / kAdRows, nk = (a.K + kLowK - 1) / kLowK;
-    int S = 1;
-    while (S < 8 && tiles * S < 2 * n_sms && nk / (2 * S) >= kLowStages) S *= 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(a.plan.max_tiles) * S);
-    cfg.blockDim = dim3(kAdThreads);
-    cfg.dynamicSmemBytes = L::kSmem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = S;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kern, a, S);
+    const int S = adapt_splits(a.plan.max_tiles, a.K, L::kPerSm * n_sms);
+    return launch_kernel(true, kern, dim3(static_cast<unsigned>(a.plan.max_tiles) * S), dim3(kAdThreads), L::kSmem, st, a, S);
 }
 
 template <typename X, typename W>
-cudaError_t launch_x(const AdaptLow& a, bool trans, int T, int n_sms, cudaStream_t st) {
+cudaError_t launch_x(const AdaptLow& a, bool trans, int n_sms, cudaStream_t st) {
     switch (adapt_rp(a.R)) {
-        case 16: return trans ? launch_t<X, W, 16, true>(a, T, n_sms, st) : launch_t<X, W, 16, false>(a, T, n_sms, st);
-        case 32: return trans ? launch_t<X, W, 32, true>(a, T, n_sms, st) : launch_t<X, W, 32, false>(a, T, n_sms, st);
-        case 64: return trans ? launch_t<X, W, 64, true>(a, T, n_sms, st) : launch_t<X, W, 64, false>(a, T, n_sms, st);
-        default: return trans ? launch_t<X, W, 128, true>(a, T, n_sms, st) : launch_t<X, W, 128, false>(a, T, n_sms, st);
+        case 16: return trans ? launch_t<X, W, 16, true>(a, n_sms, st) : launch_t<X, W, 16, false>(a, n_sms, st);
+        case 32: return trans ? launch_t<X, W, 32, true>(a, n_sms, st) : launch_t<X, W, 32, false>(a, n_sms, st);
+        case 64: return trans ? launch_t<X, W, 64, true>(a, n_sms, st) : launch_t<X, W, 64, false>(a, n_sms, st);
+        default: return trans ? launch_t<X, W, 128, true>(a, n_sms, st) : launch_t<X, W, 128, false>(a, n_sms, st);
     }
 }
 
 }  // namespace
 
-cudaError_t launch_adapt_low(const AdaptLow& a, int type_x, int type_w, bool trans, int T, int n_sms, cudaStream_t st) {
+cudaError_t launch_adapt_low(const AdaptLow& a, int type_x, int type_w, bool trans, int n_sms, cudaStream_t st) {
     if (type_w == HYMOE_TYPE_F16)
-        return type_x == HYMOE_TYPE_F32 ? launch_x<float, __half>(a, trans, T, n_sms, st)
-                                        : launch_x<__half, __half>(a, trans, T, n_sms, st);
-    return type_x == HYMOE_TYPE_F32 ? launch_x<float, __nv_bfloat16>(a, trans, T, n_sms, st)
-                                    : launch_x<__nv_bfloat16, __nv_bfloat16>(a, trans, T, n_sms, st);
+        return type_x == HYMOE_TYPE_F32 ? launch_x<float, __half>(a, trans, n_sms, st)
+                                        : launch_x<__half, __half>(a, trans, n_sms, st);
+    return type_x == HYMOE_TYPE_F32 ? launch_x<float, __nv_bfloat16>(a, trans, n_sms, st)
+                                    : launch_x<__nv_bfloat16, __nv_bfloat16>(a, trans, n_sms, st);
 }
 
 }  // namespace hymoe

@@ -25,6 +25,7 @@ struct WideTile {
     static constexpr int kWBytes = (TRANS ? RP : kWideCols) * kWRow;
     static constexpr int kStage = kYBytes + kWBytes;
     static constexpr int kSmem = kStage * kWideStages;
+    static constexpr int kPerSm = 226 * 1024 / (kSmem + 1024) < 4 ? 226 * 1024 / (kSmem + 1024) : 4;  // CTAs on an SM
 };
 
 // The 16-bit parts of a pair of fp32 values; bf16 has fp32's range, fp16 rows are scaled before.
@@ -40,7 +41,8 @@ __device__ __forceinline__ void split16(float x, float y, uint32_t (&p)[NP]) {
 }
 
 template <typename Y, typename W, int RP, bool TRANS>
-__global__ __launch_bounds__(kAdThreads) void wide_kernel(const __grid_constant__ AdaptWide a, int cols_per_cta) {
+__global__ __launch_bounds__(kAdThreads, WideTile<Y, RP, TRANS>::kPerSm) void wide_kernel(
+    const __grid_constant__ AdaptWide a, int cols_per_cta) {
     using L = WideTile<Y, RP, TRANS>;
     constexpr bool kScaled = AdType<W>::kScaled;
     constexpr int NP = L::kF32 && !kScaled ? 3 : 2;  // bf16 parts of 8 bits, fp16 parts of 11
@@ -60,44 +62,65 @@ __global__ __launch_bounds__(kAdThreads) void wide_kernel(const __grid_constant_
     constexpr int kYRows = 32 / kYPieces;                  // rows that a warp covers at once
     constexpr int kYIter = 16 / kYRows;                    // a warp loads and stores its own 16 rows
     const int yc = lane % kYPieces, yr0 = warp * 16 + lane / kYPieces;
-    int tok[kYIter];
+    const char* bp[kYIter];  // this thread's pieces of the base's and the result's rows, in column 0
+    char* op[kYIter];
+    int yn[kYIter];          // bytes of a whole piece: none where the row does not exist
 #pragma unroll
     for (int i = 0; i < kYIter; ++i) {
         const int r = yr0 + i * kYRows;
-        tok[i] = r < tile.z ? __ldg(a.plan.perm + tile.y + r) : -1;
+        const bool ok = r < tile.z;
+        const int tok = ok ? __ldg(a.plan.perm + tile.y + r) : 0;
+        yn[i] = ok ? 16 : 0;
+        bp[i] = static_cast<const char*>(a.base) + (static_cast<size_t>(tok) * a.ldb + (ok ? yc * P : 0)) * sizeof(Y);
+        op[i] = static_cast<char*>(a.out) + (static_cast<size_t>(tok) * a.ldo + yc * P) * sizeof(Y);
     }
+    constexpr int kWPieces = TRANS ? kWideCols / 8 : RP / 8, kWAll = (TRANS ? RP : kWideCols) * kWPieces;
+    constexpr int kWIter = kWAll / kAdThreads;
+    static_assert(kWAll % kAdThreads == 0, "whole rounds of pieces");
     const char* wbase = static_cast<const char*>(a.w) + static_cast<size_t>(mul ? tile.x : 0) * a.R * a.N * 2;
+    const char* wp[kWIter];
+    int wn[kWIter];
+#pragma unroll
+    for (int i = 0; i < kWIter; ++i) {
+        const int p = tid + i * kAdThreads, r = p / kWPieces, c = p % kWPieces * 8;
+        const bool ok = TRANS ? r < a.R : c < a.R;  // trans: row = rank, columns = out; else row = out, columns = rank
+        wp[i] = ok ? wbase + (static_cast<size_t>(r) * (TRANS ? a.N : a.R) + c) * 2 : wbase;
+        wn[i] = !ok ? 0 : TRANS ? 16 : min(16, (a.R - c) * 2);
+    }
     auto load = [&](int stage, int blk) {
         char* ys = smem + stage * L::kStage;
         char* ws = ys + L::kYBytes;
         const int c0 = c_lo + blk * kWideCols;
+        const bool whole = c0 + kWideCols <= c_hi;
         if (a.base != nullptr) {
+            if (whole && a.vec_b) {
 #pragma unroll
-            for (int i = 0; i < kYIter; ++i) {
-                const int r = yr0 + i * kYRows, c = c0 + yc * P;
-                const int n = tok[i] >= 0 ? c_hi - c : 0;
-                const char* src = static_cast<const char*>(a.base);
-                if (n > 0) src += (static_cast<size_t>(tok[i]) * a.ldb + c) * sizeof(Y);
-                ad_copy_piece<sizeof(Y)>(ys + r * L::kYRow + yc * 16, src, n, a.vec_b);
+                for (int i = 0; i < kYIter; ++i)
+                    cp_async16_part(ys + (yr0 + i * kYRows) * L::kYRow + yc * 16, yn[i] ? bp[i] + static_cast<size_t>(c0) * sizeof(Y) : bp[i], yn[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kYIter; ++i) {
+                    const int n = yn[i] ? c_hi - (c0 + yc * P) : 0;
+                    ad_copy_piece<sizeof(Y)>(ys + (yr0 + i * kYRows) * L::kYRow + yc * 16,
+                                             n > 0 ? bp[i] + static_cast<size_t>(c0) * sizeof(Y) : static_cast<const char*>(a.base), n, a.vec_b);
+                }
             }
         }
         if (mul) {
-            constexpr int kWPieces = TRANS ? kWideCols / 8 : RP / 8, kWAll = (TRANS ? RP : kWideCols) * kWPieces;
+            const size_t adv = static_cast<size_t>(c0) * (TRANS ? 1 : a.R) * 2;
+            if (whole && a.vec_w) {
 #pragma unroll
-            for (int i = 0; i < (kWAll + kAdThreads - 1) / kAdThreads; ++i) {
-                const int p = tid + i * kAdThreads;
-                if (kWAll % kAdThreads != 0 && p >= kWAll) break;
-                const int r = p / kWPieces, c = p % kWPieces;
-                int n;
-                size_t off;
-                if (TRANS) {  // row = rank, columns = out columns
-                    n = r < a.R ? a.N - (c0 + c * 8) : 0;
-                    off = static_cast<size_t>(r) * a.N + c0 + c * 8;
-                } else {      // row = out column, columns = rank
-                    n = c0 + r < a.N ? a.R - c * 8 : 0;
-                    off = static_cast<size_t>(c0 + r) * a.R + c * 8;
+                for (int i = 0; i < kWIter; ++i) {
+                    const int p = tid + i * kAdThreads;
+                    cp_async16_part(ws + p / kWPieces * L::kWRow + p % kWPieces * 16, wn[i] ? wp[i] + adv : wbase, wn[i]);
                 }
-                ad_copy_piece<2>(ws + r * L::kWRow + c * 16, n > 0 ? wbase + off * 2 : wbase, n, a.vec_w);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kWIter; ++i) {
+                    const int p = tid + i * kAdThreads, r = p / kWPieces, c = p % kWPieces;
+                    const int n = wn[i] == 0 ? 0 : TRANS ? a.N - (c0 + c * 8) : (c0 + r < a.N ? a.R - c * 8 : 0);
+                    ad_copy_piece<2>(ws + r * L::kWRow + c * 16, n > 0 ? wp[i] + adv : wbase, n, a.vec_w);
+                }
             }
         }
     };
@@ -195,7 +218,11 @@ __global__ __launch_bounds__(kAdThreads) void wide_kernel(const __grid_constant_
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     char* at = ys + (warp * 16 + g + 8 * q) * L::kYRow + (j * 8 + 2 * t) * static_cast<int>(sizeof(Y));
-                    float x = acc[j][2 * q] * back[q], y = acc[j][2 * q + 1] * back[q];
+                    float x = acc[j][2 * q], y = acc[j][2 * q + 1];
+                    if (kScaled) {
+                        x *= back[q];
+                        y *= back[q];
+                    }
                     if constexpr (L::kF32) {
                         if (a.base != nullptr) {
                             const float2 b = *reinterpret_cast<const float2*>(at);
@@ -215,17 +242,19 @@ __global__ __launch_bounds__(kAdThreads) void wide_kernel(const __grid_constant_
             __syncwarp();
         }
         const int c0 = c_lo + blk * kWideCols;
+        if (c0 + kWideCols <= c_hi && a.vec_o) {
 #pragma unroll
-        for (int i = 0; i < kYIter; ++i) {
-            const int r = yr0 + i * kYRows, c = c0 + yc * P;
-            if (tok[i] < 0 || c >= c_hi) continue;
-            const char* src = ys + r * L::kYRow + yc * 16;
-            char* dst = static_cast<char*>(a.out) + (static_cast<size_t>(tok[i]) * a.ldo + c) * sizeof(Y);
-            if (a.vec_o && c + P <= c_hi) {
-                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-            } else {
-                const Y* s = reinterpret_cast<const Y*>(src);
-                for (int j = 0; j < P && c + j < c_hi; ++j) reinterpret_cast<Y*>(dst)[j] = s[j];
+            for (int i = 0; i < kYIter; ++i)
+                if (yn[i])
+                    *reinterpret_cast<uint4*>(op[i] + static_cast<size_t>(c0) * sizeof(Y)) =
+                        *reinterpret_cast<const uint4*>(ys + (yr0 + i * kYRows) * L::kYRow + yc * 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kYIter; ++i) {
+                const Y* src = reinterpret_cast<const Y*>(ys + (yr0 + i * kYRows) * L::kYRow + yc * 16);
+                Y* dst = reinterpret_cast<Y*>(op[i]) + c0;
+                if (yn[i])
+                    for (int j = 0; j < P && c0 + yc * P + j < c_hi; ++j) dst[j] = src[j];
             }
         }
     }
@@ -233,36 +262,36 @@ __global__ __launch_bounds__(kAdThreads) void wide_kernel(const __grid_constant_
 }
 
 template <typename Y, typename W, int RP, bool TRANS>
-cudaError_t launch_t(const AdaptWide& a, int T, int n_sms, cudaStream_t st) {
+cudaError_t launch_t(const AdaptWide& a, int n_sms, cudaStream_t st) {
     using L = WideTile<Y, RP, TRANS>;
     auto kern = wide_kernel<Y, W, RP, TRANS>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
-    // runs of columns: about four CTAs on every SM, each with as many columns as that leaves
-    const int tiles = (T + kAdRows - 1) / kAdRows, blks = (a.N + kWideCols - 1) / kWideCols;
-    const int want = (4 * n_sms + tiles - 1) / tiles, parts = want < blks ? want : blks;
+    // runs of columns: as many as fill the GPU once
+    const int blks = (a.N + kWideCols - 1) / kWideCols, fit = L::kPerSm * n_sms / a.plan.max_tiles;
+    const int parts = fit < 1 ? 1 : fit < blks ? fit : blks;
     const int cols = (blks + parts - 1) / parts * kWideCols;
     return launch_kernel(true, kern, dim3(a.plan.max_tiles, (a.N + cols - 1) / cols), dim3(kAdThreads), L::kSmem, st, a, cols);
 }
 
 template <typename Y, typename W>
-cudaError_t launch_y(const AdaptWide& a, bool trans, int T, int n_sms, cudaStream_t st) {
+cudaError_t launch_y(const AdaptWide& a, bool trans, int n_sms, cudaStream_t st) {
     switch (adapt_rp(a.R)) {
-        case 16: return trans ? launch_t<Y, W, 16, true>(a, T, n_sms, st) : launch_t<Y, W, 16, false>(a, T, n_sms, st);
-        case 32: return trans ? launch_t<Y, W, 32, true>(a, T, n_sms, st) : launch_t<Y, W, 32, false>(a, T, n_sms, st);
-        case 64: return trans ? launch_t<Y, W, 64, true>(a, T, n_sms, st) : launch_t<Y, W, 64, false>(a, T, n_sms, st);
-        default: return trans ? launch_t<Y, W, 128, true>(a, T, n_sms, st) : launch_t<Y, W, 128, false>(a, T, n_sms, st);
+        case 16: return trans ? launch_t<Y, W, 16, true>(a, n_sms, st) : launch_t<Y, W, 16, false>(a, n_sms, st);
+        case 32: return trans ? launch_t<Y, W, 32, true>(a, n_sms, st) : launch_t<Y, W, 32, false>(a, n_sms, st);
+        case 64: return trans ? launch_t<Y, W, 64, true>(a, n_sms, st) : launch_t<Y, W, 64, false>(a, n_sms, st);
+        default: return trans ? launch_t<Y, W, 128, true>(a, n_sms, st) : launch_t<Y, W, 128, false>(a, n_sms, st);
     }
 }
 
 }  // namespace
 
-cudaError_t launch_adapt_wide(const AdaptWide& a, int type_y, int type_w, bool trans, int T, int n_sms, cudaStream_t st) {
+cudaError_t launch_adapt_wide(const AdaptWide& a, int type_y, int type_w, bool trans, int n_sms, cudaStream_t st) {
     if (type_w == HYMOE_TYPE_F16)
-        return type_y == HYMOE_TYPE_F32 ? launch_y<float, __half>(a, trans, T, n_sms, st)
-                                        : launch_y<__half, __half>(a, trans, T, n_sms, st);
-    return type_y == HYMOE_TYPE_F32 ? launch_y<float, __nv_bfloat16>(a, trans, T, n_sms, st)
-                                    : launch_y<__nv_bfloat16, __nv_bfloat16>(a, trans, T, n_sms, st);
+        return type_y == HYMOE_TYPE_F32 ? launch_y<float, __half>(a, trans, n_sms, st)
+                                        : launch_y<__half, __half>(a, trans, n_sms, st);
+    return type_y == HYMOE_TYPE_F32 ? launch_y<float, __nv_bfloat16>(a, trans, n_sms, st)
+                                    : launch_y<__nv_bfloat16, __nv_bfloat16>(a, trans, n_sms, st);
 }
 
 }  // namespace hymoe
