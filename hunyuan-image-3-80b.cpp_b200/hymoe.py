@@ -408,49 +408,57 @@ def _check_entry(st: int) -> None:
         raise HymoeError(st, lib().hymoe_last_error(None).decode(errors="replace"))
 
 
-def _torch_types() -> dict:
-    import torch
-    return {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+_TORCH = None
+
+
+def _torch():
+    """torch, the type codes of its element types, and the calls that give the current device and
+    its current stream's handle (torch's own thin ones where it has them)."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+        current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+        stream = (getattr(torch._C, "_cuda_getCurrentRawStream", None)
+                  or (lambda index: torch.cuda.current_stream(index).cuda_stream))
+        _TORCH = torch, types, current, stream
+    return _TORCH
 
 
 def _mat(t, rows: int, cols: int, what: str) -> Mat:
     """A [rows, cols] CUDA tensor whose rows are contiguous, as an hymoe_mat (rows may be strided)."""
-    if tuple(t.shape) != (rows, cols):
+    if t.shape != (rows, cols):
         raise ValueError(f"{what} must be [{rows}, {cols}], got {tuple(t.shape)}")
-    code = _torch_types().get(t.dtype)
+    code = _torch()[1].get(t.dtype)
     if code is None or not t.is_cuda:
         raise ValueError(f"{what} must be a float32, float16 or bfloat16 CUDA tensor, got {t.dtype} on {t.device}")
-    if cols > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
         raise ValueError(f"{what} must have contiguous rows, got strides {t.stride()}")
-    return Mat(t.data_ptr(), code, t.stride(0) if rows > 1 else max(cols, 1))
+    return Mat(t.data_ptr(), code, ld if rows > 1 else max(cols, 1))
 
 
 def _vec(t, shape: tuple, dtype, device, what: str):
     """Pointer of a contiguous tensor of this shape, type and device (None stays None)."""
     if t is None:
         return None
-    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} {list(shape)} on {device}, got {t.dtype} "
                          f"{list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-class _on:
-    """The device of the tensors made current, and its current stream."""
-
-    def __init__(self, device):
-        import torch
-        self.guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
-        self.stream = torch.cuda.current_stream(device).cuda_stream
-
-    def __enter__(self):
-        if self.guard:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self.guard:
-            self.guard.__exit__(*exc)
+def _call(device, fn, *args):
+    """fn(*args, stream) with `device` current, on its current stream; raises on a bad status."""
+    torch, _, current, stream = _torch()
+    index = device.index
+    if current() == index:
+        st = fn(*args, stream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, stream(index))
+    if st != 0:
+        _check_entry(st)
 
 
 class Gate:
@@ -469,6 +477,7 @@ class Gate:
                              f"{list(self.GROUPS)}")
         ng, tg = group if group else (0, 0)
         self.spec = GateSpec(self.SCORES[score], ng, tg, self.GROUPS[group_score], 1 if norm_topk_prob else 0, scale)
+        self._spec = C.byref(self.spec)
         # the library checks the gate itself: a call without tokens does only that
         _check_entry(self.L.hymoe_route_backward(C.byref(self.spec), None, None, None, None, 0, n_experts, topk,
                                                  None, None))
@@ -477,36 +486,31 @@ class Gate:
         """logits [T, E] (float32, float16 or bfloat16; rows may be strided), bias [E] float32.
         Returns idx int32 [T, K] (-1: no expert left), weights float32 [T, K] and on request
         scores float32 [T, E] and counts int32 [E]."""
-        import torch
-        T, dev = logits.shape[0], logits.device
-        m = _mat(logits, T, self.E, "logits")
-        b = _vec(bias, (self.E,), torch.float32, dev, "bias")
-        out = {"idx": torch.empty((T, self.K), dtype=torch.int32, device=dev),
-               "weights": torch.empty((T, self.K), dtype=torch.float32, device=dev)}
+        torch = _torch()[0]
+        T, E, K, dev = logits.shape[0], self.E, self.K, logits.device
+        m = _mat(logits, T, E, "logits")
+        b = _vec(bias, (E,), torch.float32, dev, "bias")
+        idx, w = logits.new_empty((T, K), dtype=torch.int32), logits.new_empty((T, K), dtype=torch.float32)
+        out = {"idx": idx, "weights": w}
+        c = s = None
         if counts:
-            out["counts"] = torch.empty((self.E,), dtype=torch.int32, device=dev)
+            out["counts"] = c = logits.new_empty((E,), dtype=torch.int32)
         if scores:
-            out["scores"] = torch.empty((T, self.E), dtype=torch.float32, device=dev)
-        with _on(dev) as st:
-            _check_entry(self.L.hymoe_route(C.byref(self.spec), C.byref(m), b, T, self.E, self.K,
-                                            out["idx"].data_ptr(), out["weights"].data_ptr(),
-                                            out["scores"].data_ptr() if scores else None,
-                                            out["counts"].data_ptr() if counts else None, st))
+            out["scores"] = s = logits.new_empty((T, E), dtype=torch.float32)
+        _call(dev, self.L.hymoe_route, self._spec, m, b, T, E, K, idx.data_ptr(), w.data_ptr(),
+              None if s is None else s.data_ptr(), None if c is None else c.data_ptr())
         return out
 
     def backward(self, logits, idx, d_weights, d_scores=None):
         """Gradient to the logits [T, E] (their type) for the selections idx of route()."""
-        import torch
-        T, dev = logits.shape[0], logits.device
-        m = _mat(logits, T, self.E, "logits")
-        i = _vec(idx, (T, self.K), torch.int32, dev, "idx")
-        dw = _vec(d_weights, (T, self.K), torch.float32, dev, "d_weights")
-        ds = _vec(d_scores, (T, self.E), torch.float32, dev, "d_scores")
-        d = torch.empty((T, self.E), dtype=logits.dtype, device=dev)
-        dm = Mat(d.data_ptr(), m.type, self.E)
-        with _on(dev) as st:
-            _check_entry(self.L.hymoe_route_backward(C.byref(self.spec), C.byref(m), i, dw, ds, T, self.E, self.K,
-                                                     C.byref(dm), st))
+        torch = _torch()[0]
+        T, E, K, dev = logits.shape[0], self.E, self.K, logits.device
+        m = _mat(logits, T, E, "logits")
+        i = _vec(idx, (T, K), torch.int32, dev, "idx")
+        dw = _vec(d_weights, (T, K), torch.float32, dev, "d_weights")
+        ds = _vec(d_scores, (T, E), torch.float32, dev, "d_scores")
+        d = logits.new_empty((T, E))
+        _call(dev, self.L.hymoe_route_backward, self._spec, m, i, dw, ds, T, E, K, Mat(d.data_ptr(), m.type, E))
         return d
 
 
@@ -524,10 +528,11 @@ class Adapters:
             raise ValueError(f"adapters must be float16 or bfloat16 CUDA tensors, got {a.dtype} on {a.device}")
         self.n, self.rank, self.n_in, self.n_out = a.shape[0], a.shape[1], a.shape[2], b.shape[1]
         self.device = a.device
-        self.spec = AdapterSpec(self.n, self.rank, self.n_in, self.n_out, _torch_types()[a.dtype],
+        self.spec = AdapterSpec(self.n, self.rank, self.n_in, self.n_out, _torch()[1][a.dtype],
                                 _vec(a, tuple(a.shape), a.dtype, a.device, "a"),
                                 _vec(b, tuple(b.shape), a.dtype, a.device, "b"),
                                 _vec(scale, (self.n,), torch.float32, a.device, "scale"))
+        self._spec = C.byref(self.spec)
         self._keep = (a, b, scale)
         self._bytes = {}
         self._workspace_bytes(0, False)  # the library checks the sizes
@@ -540,11 +545,6 @@ class Adapters:
             got = self._bytes[(T, backward)] = n.value
         return got
 
-    def _workspace(self, T: int, backward: bool):
-        import torch
-        n = self._workspace_bytes(T, backward)
-        return (torch.empty(n, dtype=torch.uint8, device=self.device) if n else None), n
-
     def _rows(self, t, T: int, cols: int, what: str):
         if t is None:
             return None
@@ -556,40 +556,38 @@ class Adapters:
         """out[t] = base[t] + scale * B (A x[t]) of adapter ids[t] (int32; outside [0, n): none; None:
         adapter 0).  base None: zeros.  out: written in place (may be base); None: a new tensor of
         base's type, x's without a base."""
-        import torch
+        torch = _torch()[0]
         T = x.shape[0]
         mx, mb = self._rows(x, T, self.n_in, "x"), self._rows(base, T, self.n_out, "base")
         i = _vec(ids, (T,), torch.int32, self.device, "ids")
         if out is None:
-            out = torch.empty((T, self.n_out), dtype=x.dtype if base is None else base.dtype, device=self.device)
+            out = (x if base is None else base).new_empty((T, self.n_out))
         mo = self._rows(out, T, self.n_out, "out")
-        with _on(self.device) as st:
-            ws, n = self._workspace(T, False)
-            _check_entry(self.L.hymoe_adapt(C.byref(self.spec), C.byref(mx), i, T, C.byref(mb) if mb else None,
-                                            C.byref(mo), ws.data_ptr() if n else None, n, st))
+        n = self._workspace_bytes(T, False)
+        ws = x.new_empty((n,), dtype=torch.uint8) if n else None
+        _call(self.device, self.L.hymoe_adapt, self._spec, mx, i, T, mb, mo, ws.data_ptr() if n else None, n)
         return out
 
     def backward(self, x, dy, ids=None, base=None, want=("dx", "da", "db")) -> dict:
         """Gradients for dy [T, out]: dx (x's type, base added where given), da and db (float32, every
         adapter's).  want: the ones to compute."""
-        import torch
+        torch = _torch()[0]
         T = x.shape[0]
         mx, my = self._rows(x, T, self.n_in, "x"), self._rows(dy, T, self.n_out, "dy")
         mb, i = self._rows(base, T, self.n_in, "base"), _vec(ids, (T,), torch.int32, self.device, "ids")
         res = {}
         if "dx" in want:
-            res["dx"] = torch.empty((T, self.n_in), dtype=x.dtype, device=self.device)
+            res["dx"] = x.new_empty((T, self.n_in))
         if "da" in want:
-            res["da"] = torch.empty((self.n, self.rank, self.n_in), dtype=torch.float32, device=self.device)
+            res["da"] = x.new_empty((self.n, self.rank, self.n_in), dtype=torch.float32)
         if "db" in want:
-            res["db"] = torch.empty((self.n, self.n_out, self.rank), dtype=torch.float32, device=self.device)
+            res["db"] = x.new_empty((self.n, self.n_out, self.rank), dtype=torch.float32)
         md = self._rows(res.get("dx"), T, self.n_in, "dx")
-        with _on(self.device) as st:
-            ws, n = self._workspace(T, True)
-            _check_entry(self.L.hymoe_adapt_backward(
-                C.byref(self.spec), C.byref(mx), C.byref(my), i, T, C.byref(mb) if mb else None,
-                C.byref(md) if md else None, res["da"].data_ptr() if "da" in res else None,
-                res["db"].data_ptr() if "db" in res else None, ws.data_ptr() if n else None, n, st))
+        n = self._workspace_bytes(T, True)
+        ws = x.new_empty((n,), dtype=torch.uint8) if n else None
+        _call(self.device, self.L.hymoe_adapt_backward, self._spec, mx, my, i, T, mb, md,
+              res["da"].data_ptr() if "da" in res else None, res["db"].data_ptr() if "db" in res else None,
+              ws.data_ptr() if n else None, n)
         return res
 
 

@@ -156,6 +156,21 @@ def test_ties_with_equal_biases():
                 check_route(z, b, K, got, score=score, group=group, group_score=gs)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("E", [40, 64, 512])
+def test_zeros_of_both_signs_and_neighbours(dtype, E):
+    """-0 ties with 0; neighbouring numbers of the type do not tie."""
+    g = torch.Generator().manual_seed(11)
+    z = torch.where(torch.rand(30, E, generator=g) < 0.5, 0.0, -0.0)
+    z[10:20] = 1.0 + torch.randint(0, 3, (10, E), generator=g) * torch.finfo(dtype).eps
+    z[20:] = -(3.0 + torch.randint(0, 9, (10, E), generator=g) * 2 * torch.finfo(dtype).eps)
+    z = z.to(dtype)
+    for score in ("softmax", "sigmoid"):
+        for group in (None, (4, 2)):
+            gate = hymoe.Gate(E, 8, score=score, group=group)
+            check_route(z, None, 8, gate.route(z.cuda(), counts=True), score=score, group=group)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("E,off,ld", [(64, 0, 64), (64, 1, 65), (64, 8, 96), (256, 3, 300), (60, 0, 60), (48, 4, 52)])
 def test_strides_and_alignment(dtype, E, off, ld):
