@@ -310,6 +310,7 @@ __global__ void ep_segments_fused_kernel(const int* __restrict__ C, int ld, int 
 __global__ void unmap_slots_kernel(int* __restrict__ idx, const int* __restrict__ expert_of_slot, int n) {
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
+    if (idx[i] < 0) return;
     const int slot = idx[i] & ~kDroppedPair;
     idx[i] = expert_of_slot != nullptr ? __ldg(expert_of_slot + slot) : slot;
 }

@@ -9,8 +9,7 @@ extern template cudaError_t launch_gate_grad<float>(const hymoe_mat&, const hymo
 extern template cudaError_t launch_gate_grad<__half>(const hymoe_mat&, const hymoe_mat&, uint32_t, const GateGradArgs&, cudaStream_t);
 extern template cudaError_t launch_gate_grad<__nv_bfloat16>(const hymoe_mat&, const hymoe_mat&, uint32_t, const GateGradArgs&, cudaStream_t);
 
-namespace {
-
+// Why a gate cannot route E experts, K of them to a token; nullptr where it can.
 const char* gate_problem(const hymoe_gate* g, uint32_t E, uint32_t K) {
     if (!g) return "null gate";
     if (E == 0 || E > HYMOE_GATE_MAX_EXPERTS) return "n_experts must be 1..HYMOE_GATE_MAX_EXPERTS (512)";
@@ -22,6 +21,8 @@ const char* gate_problem(const hymoe_gate* g, uint32_t E, uint32_t K) {
     if (!isfinite(g->routed_scaling_factor)) return "routed_scaling_factor is not finite";
     return nullptr;
 }
+
+namespace {
 
 bool any_overlap(const EntrySpan* out, int n_out, const EntrySpan* in, int n_in) {
     for (int i = 0; i < n_out; ++i) {
@@ -77,7 +78,7 @@ extern "C" hymoe_status hymoe_route(const hymoe_gate* gate, const hymoe_mat* log
     if (T == 0) return HYMOE_OK;
     GateArgs a{bias, static_cast<int>(E), static_cast<int>(K), gate->score, static_cast<int>(gate->n_group),
                static_cast<int>(gate->topk_group), gate->group_score, gate->norm_topk_prob != 0, 0u,
-               gate->routed_scaling_factor, idx, weights, scores, counts};
+               gate->routed_scaling_factor, idx, weights, scores, counts, nullptr};
     while (a.mask + 1 < n_experts) a.mask = 2 * a.mask + 1;
     const cudaError_t e = logits->type == HYMOE_TYPE_F32   ? launch_gate<float>(*logits, n_tokens, a, st)
                           : logits->type == HYMOE_TYPE_F16 ? launch_gate<__half>(*logits, n_tokens, a, st)

@@ -44,6 +44,7 @@ struct GateArgs {
     float* weights;
     float* scores;
     int* counts;
+    const int* slot_of;  // in the block: expert -> placement slot, what idx and the counts then hold
 };
 struct GateGradArgs {
     const int* idx;
@@ -317,10 +318,19 @@ __device__ int select_exact(const T* __restrict__ row, const GateArgs& a) {
     return sel;
 }
 
+// Lane k's selection of token t to memory; cnt: the CTA's counters, or nullptr.
+__device__ __forceinline__ void put_choice(const GateArgs& a, size_t t, int sel, float w, int* cnt) {
+    const int lane = threadIdx.x & 31;
+    if (lane >= a.K) return;
+    if (a.slot_of != nullptr && sel >= 0) sel = __ldg(a.slot_of + sel);
+    a.idx[t * a.K + lane] = sel;
+    a.weights[t * a.K + lane] = w;
+    if (cnt != nullptr && sel >= 0) atomicAdd(cnt + sel, 1);
+}
+
 // A token in double precision where its order could not be proven in fp32: outputs and counts.
 template <typename T, int EPL, bool SIG>
 __device__ __noinline__ void route_exact(const T* __restrict__ row, size_t t, const GateArgs& a, int* cnt) {
-    const int lane = threadIdx.x & 31;
     const int sel = select_exact<T, EPL>(row, a);
     const float z = sel >= 0 ? clean_logit(gate_value(row[sel])) : -INFINITY;
     float m = 0.f, sum = 0.f;
@@ -338,12 +348,7 @@ __device__ __noinline__ void route_exact(const T* __restrict__ row, size_t t, co
         for (int i = 0; i < EPL; ++i) sum += expf(c[i] - m);
         sum = warp_sum(sum);
     }
-    const float w = gate_weight<SIG>(z, a.norm, m, sum, a.scale);
-    if (lane < a.K) {
-        a.idx[t * a.K + lane] = sel;
-        a.weights[t * a.K + lane] = w;
-        if (cnt != nullptr && sel >= 0) atomicAdd(cnt + sel, 1);
-    }
+    put_choice(a, t, sel, gate_weight<SIG>(z, a.norm, m, sum, a.scale), cnt);
 }
 
 // One token: lane k gets its k-th expert (-1: none left) and weight; false where the selection has
@@ -532,7 +537,7 @@ __global__ __launch_bounds__(32 * kGateWarps, EPL <= 2 ? 6 : EPL == 4 ? 5 : EPL 
     const T* __restrict__ logits, size_t ld, uint32_t n_tok, const __grid_constant__ GateArgs a) {
     extern __shared__ float gbuf[];  // groups with spread experts only: [kGateWarps][E]
     __shared__ int cnt[HYMOE_GATE_MAX_EXPERTS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int warp = threadIdx.x >> 5;
     if (a.counts != nullptr) {
         for (int e = threadIdx.x; e < a.E; e += blockDim.x) cnt[e] = 0;
         __syncthreads();
@@ -552,10 +557,8 @@ __global__ __launch_bounds__(32 * kGateWarps, EPL <= 2 ? 6 : EPL == 4 ? 5 : EPL 
             if (!route_token<T, EPL, RUN, SIG, VALUED>(logits + t * ld, raw, VALUED && a.scores != nullptr ? a.scores + t * a.E : nullptr,
                                                        a, bias, gbuf + static_cast<size_t>(warp) * a.E, sel, w)) {
                 again |= 1u << i;
-            } else if (lane < a.K) {
-                a.idx[t * a.K + lane] = sel;
-                a.weights[t * a.K + lane] = w;
-                if (a.counts != nullptr && sel >= 0) atomicAdd(&cnt[sel], 1);
+            } else {
+                put_choice(a, t, sel, w, a.counts != nullptr ? cnt : nullptr);
             }
         }
         for (; again != 0; again &= again - 1) {

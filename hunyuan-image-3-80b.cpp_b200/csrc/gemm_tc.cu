@@ -526,6 +526,16 @@ __global__ void __launch_bounds__(EP ? kEpThreads : kThreads, 1)
                 // matching up rows.  Lanes < 16 finish tokens 0-15 of the chunk, lanes >= 16
                 // tokens 16-31; one shuffle per token pair swaps the missing halves.
                 const bool gate_lane = lane < 16;
+                if (a.glu_add != nullptr && row0 < a.shared_rows) {
+                    // the shared expert's adapters: this lane's gate or up column of every token
+                    const float* add = a.glu_add + static_cast<size_t>(row0 + ch * 32) * 2 * a.out_ld +
+                                       (gate_lane ? 0 : a.out_ld) + rb * kGluHalf + 16 * q + (lane & 15);
+                    const int na = min(32, nrows - ch * 32);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j < na)
+                            v[j] = __float_as_uint(__uint_as_float(v[j]) + __ldg(add + static_cast<size_t>(j) * 2 * a.out_ld));
+                }
                 __half* o = static_cast<__half*>(a.out) + static_cast<size_t>(row0 + ch * 32) * a.out_ld +
                             rb * kGluHalf + 16 * q + (lane & 15);
                 const int nj = min(32, nrows - ch * 32);

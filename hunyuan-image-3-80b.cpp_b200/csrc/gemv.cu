@@ -46,6 +46,7 @@ struct GemvItem {
     void* out;
     __half* out_r;    // down projection: routed rows (>= shared_rows), fp16
     int shared_rows;
+    const float* glu_add;  // gate_up: added to the sums of rows below shared_rows ([row][2 out_ld]: gate, up), or nullptr
     int* err;
 };
 
@@ -165,8 +166,14 @@ __device__ __forceinline__ void run_item(const GemvItem& p, uint8_t* base, uint6
         __half* o = static_cast<__half*>(p.out);
         for (int i = tid; i < kGluHalf * nrows; i += kGemvThreads) {
             const int j = i % kGluHalf, n = i / kGluHalf;
-            o[static_cast<size_t>(p.row0 + n) * p.out_ld + p.rb * kGluHalf + j] =
-                __float2half_rn(silu_mul(G[glu_gate_row(j) * kGL + n], G[glu_up_row(j) * kGL + n]));
+            const size_t at = static_cast<size_t>(p.row0 + n) * p.out_ld + p.rb * kGluHalf + j;
+            float gt = G[glu_gate_row(j) * kGL + n], up = G[glu_up_row(j) * kGL + n];
+            if (p.glu_add != nullptr && p.row0 < p.shared_rows) {
+                const float* add = p.glu_add + at + static_cast<size_t>(p.row0 + n) * p.out_ld;
+                gt += add[0];
+                up += add[p.out_ld];
+            }
+            o[at] = __float2half_rn(silu_mul(gt, up));
         }
     } else if (p.row0 < p.shared_rows) {
         float* o = static_cast<float*>(p.out);
@@ -190,7 +197,7 @@ __global__ __launch_bounds__(kGemvThreads, 3) void gemv_kernel(const __grid_cons
                                                             int n_ks, int glu, int slots, int xb_max,
                                                             void* __restrict__ out, int out_ld,
                                                             __half* __restrict__ out_r, int shared_rows,
-                                                            int* err) {
+                                                            const float* __restrict__ glu_add, int* err) {
     griddep_wait();
     griddep_launch_dependents();
     constexpr int TB = tile_bytes(WT);
@@ -219,6 +226,7 @@ __global__ __launch_bounds__(kGemvThreads, 3) void gemv_kernel(const __grid_cons
     p.out = out;
     p.out_r = out_r;
     p.shared_rows = shared_rows;
+    p.glu_add = glu_add;
     p.err = err;
     if (threadIdx.x == 0) {
         for (int s = 0; s < slots; ++s) mbar_init(&full[s], 1);
@@ -249,7 +257,7 @@ template <int WT, int R>
 __global__ __launch_bounds__(kGemvThreads, 1) void gemv_stream_kernel(
     const __grid_constant__ GemvMaps maps, const int4* __restrict__ items, const int* __restrict__ n_items,
     const uint8_t* const* __restrict__ wtiles, int n_ks, int glu, void* __restrict__ out, int out_ld,
-    __half* __restrict__ out_r, int shared_rows, int* err) {
+    __half* __restrict__ out_r, int shared_rows, const float* __restrict__ glu_add, int* err) {
     // Programmatic dependent launch: everything up to griddep_wait reads only what was complete
     // before this grid could be scheduled (the work list, written by the plan two or more
     // launches back, and the weights); the activation rows come from the predecessor.
@@ -387,8 +395,14 @@ __global__ __launch_bounds__(kGemvThreads, 1) void gemv_stream_kernel(
             __half* o = static_cast<__half*>(out);
             for (int e = tid; e < kGluHalf * nrows; e += kGemvThreads) {
                 const int j = e % kGluHalf, n = e / kGluHalf;
-                o[static_cast<size_t>(row0 + n) * out_ld + rb * kGluHalf + j] =
-                    __float2half_rn(silu_mul(sum(glu_gate_row(j), n), sum(glu_up_row(j), n)));
+                const size_t at = static_cast<size_t>(row0 + n) * out_ld + rb * kGluHalf + j;
+                float gt = sum(glu_gate_row(j), n), up = sum(glu_up_row(j), n);
+                if (glu_add != nullptr && row0 < shared_rows) {
+                    const float* add = glu_add + at + static_cast<size_t>(row0 + n) * out_ld;
+                    gt += add[0];
+                    up += add[out_ld];
+                }
+                o[at] = __float2half_rn(silu_mul(gt, up));
             }
         } else if (row0 < shared_rows) {
             float* o = static_cast<float*>(out);
@@ -421,13 +435,13 @@ size_t stream_smem() {
 template <int WT, int R>
 cudaError_t launch_stream(const GemvMaps& maps, const int4* items, const int* n_items, int n_sms,
                           const uint8_t* const* wtiles, int n_ks, int glu, void* out, int out_ld, __half* out_r,
-                          int shared_rows, int* err, cudaStream_t st, bool pdl) {
+                          int shared_rows, const float* glu_add, int* err, cudaStream_t st, bool pdl) {
     const size_t smem = stream_smem<WT, R>();
     cudaError_t e = cudaFuncSetAttribute(gemv_stream_kernel<WT, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     return launch_kernel(pdl, gemv_stream_kernel<WT, R>, dim3(n_sms), dim3(kGemvThreads), smem, st, maps, items,
-                         n_items, wtiles, n_ks, glu, out, out_ld, out_r, shared_rows, err);
+                         n_items, wtiles, n_ks, glu, out, out_ld, out_r, shared_rows, glu_add, err);
 }
 
 // Stages per CTA: as many as fit in ~72 KB (three CTAs per SM), at least 2 and at most 4;
@@ -447,7 +461,8 @@ void gemv_smem(int max_box, int* slots, int* xb_max, size_t* smem) {
 template <int WT>
 cudaError_t launch_t(const GemvMaps& maps, const int4* items, const int* n_items, int max_items,
                      const uint8_t* const* wtiles, int n_ks, int glu, int max_rows, void* out,
-                     int out_ld, __half* out_r, int shared_rows, int* err, cudaStream_t st, bool pdl) {
+                     int out_ld, __half* out_r, int shared_rows, const float* glu_add, int* err, cudaStream_t st,
+                     bool pdl) {
     int slots = 0, xb_max = 0;
     size_t smem = 0;
     gemv_smem<WT>(box_index(max_rows), &slots, &xb_max, &smem);
@@ -455,7 +470,7 @@ cudaError_t launch_t(const GemvMaps& maps, const int4* items, const int* n_items
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     return launch_kernel(pdl, gemv_kernel<WT>, dim3(max_items), dim3(kGemvThreads), smem, st, maps, items, n_items,
-                         wtiles, n_ks, glu, slots, xb_max, out, out_ld, out_r, shared_rows, err);
+                         wtiles, n_ks, glu, slots, xb_max, out, out_ld, out_r, shared_rows, glu_add, err);
 }
 
 }  // namespace
@@ -463,19 +478,19 @@ cudaError_t launch_t(const GemvMaps& maps, const int4* items, const int* n_items
 cudaError_t launch_gemv(const GemvMaps& maps, const int4* items, const int* n_items, int max_items,
                         const uint8_t* const* wtiles, int wtype, int n_ks, int glu, int max_rows,
                         void* out, int out_ld, __half* out_r, int shared_rows, int* err, int n_sms,
-                        cudaStream_t st, bool pdl) {
+                        cudaStream_t st, bool pdl, const float* glu_add) {
     if (max_items <= 0) return cudaSuccess;
     if (max_rows < 1 || max_rows > kGemvMaxRows) return cudaErrorInvalidValue;
     if (max_rows <= 8 && wtype == W_Q8_0)
-        return launch_stream<W_Q8_0, 2>(maps, items, n_items, n_sms, wtiles, n_ks, glu, out, out_ld, out_r, shared_rows, err, st,
-                                        pdl);
+        return launch_stream<W_Q8_0, 2>(maps, items, n_items, n_sms, wtiles, n_ks, glu, out, out_ld, out_r, shared_rows, glu_add, err,
+                                        st, pdl);
     if (max_rows <= 8 && wtype == W_Q4_0)
-        return launch_stream<W_Q4_0, 3>(maps, items, n_items, n_sms, wtiles, n_ks, glu, out, out_ld, out_r, shared_rows, err, st,
-                                        pdl);
+        return launch_stream<W_Q4_0, 3>(maps, items, n_items, n_sms, wtiles, n_ks, glu, out, out_ld, out_r, shared_rows, glu_add, err,
+                                        st, pdl);
     switch (wtype) {
-        case W_Q4_0: return launch_t<W_Q4_0>(maps, items, n_items, max_items, wtiles, n_ks, glu, max_rows, out, out_ld, out_r, shared_rows, err, st, pdl);
-        case W_Q8_0: return launch_t<W_Q8_0>(maps, items, n_items, max_items, wtiles, n_ks, glu, max_rows, out, out_ld, out_r, shared_rows, err, st, pdl);
-        default: return launch_t<W_F16>(maps, items, n_items, max_items, wtiles, n_ks, glu, max_rows, out, out_ld, out_r, shared_rows, err, st, pdl);
+        case W_Q4_0: return launch_t<W_Q4_0>(maps, items, n_items, max_items, wtiles, n_ks, glu, max_rows, out, out_ld, out_r, shared_rows, glu_add, err, st, pdl);
+        case W_Q8_0: return launch_t<W_Q8_0>(maps, items, n_items, max_items, wtiles, n_ks, glu, max_rows, out, out_ld, out_r, shared_rows, glu_add, err, st, pdl);
+        default: return launch_t<W_F16>(maps, items, n_items, max_items, wtiles, n_ks, glu, max_rows, out, out_ld, out_r, shared_rows, glu_add, err, st, pdl);
     }
 }
 

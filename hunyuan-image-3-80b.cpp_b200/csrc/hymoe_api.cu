@@ -144,18 +144,19 @@ bool allocation_base(const void* p, uintptr_t* base) {
 
 namespace hymoe {
 void set_thread_error(const char* msg) { g_create_error = msg ? msg : ""; }
+const char* gate_problem(const hymoe_gate* g, uint32_t E, uint32_t K);  // gate.cu
 }  // namespace hymoe
 
 struct GraphKey {
     uint32_t layer, n_tokens;
-    const void* p[8];
+    const void* p[9];
     GraphKey(uint32_t l, uint32_t n, const void* a, const void* b, const void* c, const void* d,
-             const void* e, const void* f, const void* g, const void* h)
-        : layer(l), n_tokens(n), p{a, b, c, d, e, f, g, h} {}
+             const void* e, const void* f, const void* g, const void* h, const void* i)
+        : layer(l), n_tokens(n), p{a, b, c, d, e, f, g, h, i} {}
     bool operator<(const GraphKey& o) const {
         if (layer != o.layer) return layer < o.layer;
         if (n_tokens != o.n_tokens) return n_tokens < o.n_tokens;
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 9; ++i)
             if (p[i] != o.p[i]) return p[i] < o.p[i];
         return false;
     }
@@ -194,6 +195,17 @@ struct hymoe_ctx {
     std::vector<float> norm_eps;
     float* rms_buf = nullptr;
     RouteMode route;  // routing variant (hymoe_set_routing); default: moe_forward_cpu's
+    bool gated = false;  // the routing is `gate` (hymoe_set_gate) instead
+    hymoe_gate gate{};
+    std::vector<float*> gate_bias;  // per layer: [E] the gate's selection bias on the device, or nullptr
+    // Adapters of the shared expert per layer (hymoe_set_adapters); rank 0: none.  The weights are
+    // the caller's; the workspace, the gate_up deltas [max_tokens, 2I] F32 and the ids of host-pointer
+    // calls are the context's.
+    std::vector<hymoe_adapters> ad_gu, ad_dn;
+    char* ad_ws = nullptr;
+    size_t ad_ws_bytes = 0;
+    float* ad_delta = nullptr;
+    int32_t* ad_ids = nullptr;
     int expert_at(uint32_t layer, int slot) const {
         return expert_of_slot[layer].empty() ? slot : expert_of_slot[layer][slot];
     }
@@ -814,6 +826,9 @@ hymoe_status hymoe_create(const hymoe_config* cfg, hymoe_ctx** out) {
     c->place_dev.assign(cfg->num_layers, nullptr);
     c->norm_w.assign(cfg->num_layers, nullptr);
     c->norm_eps.assign(cfg->num_layers, 0.f);
+    c->gate_bias.assign(cfg->num_layers, nullptr);
+    c->ad_gu.assign(cfg->num_layers, hymoe_adapters{});
+    c->ad_dn.assign(cfg->num_layers, hymoe_adapters{});
     cudaDeviceGetAttribute(&c->n_sms, cudaDevAttrMultiProcessorCount, cfg->device);
 
     auto bail = [&](hymoe_status st) {
@@ -978,6 +993,10 @@ void hymoe_destroy(hymoe_ctx* c) {
     for (int* p : c->place_dev) cudaFree(p);
     for (float* p : c->norm_w) cudaFree(p);
     cudaFree(c->rms_buf);
+    for (float* p : c->gate_bias) cudaFree(p);
+    cudaFree(c->ad_ws);
+    cudaFree(c->ad_delta);
+    cudaFree(c->ad_ids);
     cudaFree(c->x_dev);
     cudaFree(c->resid_dev);
     cudaFree(c->out_dev);
@@ -1380,6 +1399,83 @@ hymoe_status hymoe_set_routing(hymoe_ctx* c, const hymoe_routing* r) {
     HY_CUDA(c, cudaStreamSynchronize(c->stream));
     c->clear_graphs();  // the mode is baked into captured launches
     c->route = m;
+    c->gated = false;
+    return HYMOE_OK;
+}
+
+hymoe_status hymoe_set_gate(hymoe_ctx* c, const hymoe_gate* gate) {
+    if (!c) return HYMOE_ERR_INVALID_ARG;
+    if (gate) {
+        if (c->cfg.ep_size > 1) return c->fail(HYMOE_ERR_UNSUPPORTED, "hymoe_set_gate: one GPU only");
+        if (const char* why = gate_problem(gate, static_cast<uint32_t>(c->E), static_cast<uint32_t>(c->K)))
+            return c->fail(HYMOE_ERR_INVALID_ARG, "hymoe_set_gate: %s", why);
+    }
+    HY_CUDA(c, cudaSetDevice(c->cfg.device));
+    HY_CUDA(c, cudaStreamSynchronize(c->stream));
+    c->clear_graphs();  // the gate is baked into captured launches
+    c->route = RouteMode{};
+    c->gated = gate != nullptr;
+    if (gate) c->gate = *gate;
+    return HYMOE_OK;
+}
+
+hymoe_status hymoe_set_balance_bias(hymoe_ctx* c, uint32_t layer, const float* bias, int flags) {
+    if (!c) return HYMOE_ERR_INVALID_ARG;
+    if (layer >= c->layers.size()) return c->fail(HYMOE_ERR_INVALID_ARG, "layer %u out of range", layer);
+    HY_CUDA(c, cudaSetDevice(c->cfg.device));
+    HY_CUDA(c, cudaStreamSynchronize(c->stream));  // no call still reads the old bias
+    if (!bias) {
+        c->clear_graphs();
+        cudaFree(c->gate_bias[layer]);
+        c->gate_bias[layer] = nullptr;
+        return HYMOE_OK;
+    }
+    if (!c->gate_bias[layer]) {
+        c->clear_graphs();  // captured launches have no bias
+        HY_CUDA(c, dalloc(&c->gate_bias[layer], static_cast<size_t>(c->E)));
+    }
+    const bool host = (flags & HYMOE_HOST_PTRS) != 0;
+    HY_CUDA(c, cudaMemcpy(c->gate_bias[layer], bias, sizeof(float) * c->E,
+                          host ? cudaMemcpyHostToDevice : cudaMemcpyDeviceToDevice));
+    return HYMOE_OK;
+}
+
+hymoe_status hymoe_set_adapters(hymoe_ctx* c, uint32_t layer, const hymoe_adapters* gate_up, const hymoe_adapters* down) {
+    if (!c) return HYMOE_ERR_INVALID_ARG;
+    if (layer >= c->layers.size()) return c->fail(HYMOE_ERR_INVALID_ARG, "layer %u out of range", layer);
+    if ((gate_up || down) && c->cfg.ep_size > 1) return c->fail(HYMOE_ERR_UNSUPPORTED, "hymoe_set_adapters: one GPU only");
+    const uint32_t H = static_cast<uint32_t>(c->H), I = static_cast<uint32_t>(c->I);
+    const hymoe_adapters* ads[2] = {gate_up, down};
+    const uint32_t in[2] = {H, I}, out[2] = {2 * I, H};
+    size_t need = 0;
+    for (int i = 0; i < 2; ++i) {
+        const hymoe_adapters* ad = ads[i];
+        if (!ad) continue;
+        if (ad->type != HYMOE_TYPE_F16)
+            return c->fail(HYMOE_ERR_UNSUPPORTED, "hymoe_set_adapters: the block's adapters are F16, like its activations");
+        if (ad->in_features != in[i] || ad->out_features != out[i] || !ad->a || !ad->b)
+            return c->fail(HYMOE_ERR_INVALID_ARG, "hymoe_set_adapters: gate_up adapters are H=%u -> 2I=%u, down adapters "
+                           "I=%u -> H=%u, with weights", H, 2 * I, I, H);
+        size_t bytes = 0;
+        const hymoe_status st = hymoe_adapt_workspace(ad, c->cfg.max_tokens, 0, &bytes);
+        if (st != HYMOE_OK) return c->fail(st, "hymoe_set_adapters: %s", hymoe_last_error(nullptr));
+        need = std::max(need, bytes);
+    }
+    HY_CUDA(c, cudaSetDevice(c->cfg.device));
+    HY_CUDA(c, cudaStreamSynchronize(c->stream));  // no call still uses the old ones
+    c->clear_graphs();
+    if (need > c->ad_ws_bytes) {
+        cudaFree(c->ad_ws);
+        c->ad_ws = nullptr;
+        c->ad_ws_bytes = 0;
+        HY_CUDA(c, dalloc(&c->ad_ws, need));
+        c->ad_ws_bytes = need;
+    }
+    if ((gate_up || down) && !c->ad_ids) HY_CUDA(c, dalloc(&c->ad_ids, static_cast<size_t>(c->cfg.max_tokens)));
+    if (gate_up && !c->ad_delta)
+        HY_CUDA(c, dalloc(&c->ad_delta, static_cast<size_t>(c->cfg.max_tokens) * 2 * c->I));
+    c->ad_gu[layer] = gate_up ? *gate_up : hymoe_adapters{};
+    c->ad_dn[layer] = down ? *down : hymoe_adapters{};
     return HYMOE_OK;
 }
 
@@ -1444,9 +1540,11 @@ hymoe_status hymoe_balance_placement(uint32_t n_experts, uint32_t ep_size, const
     return HYMOE_OK;
 }
 
-hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const float* residual,
-                           float* out, uint32_t n_tokens, const float* router_bias,
-                           hymoe_debug* dbg, int flags) {
+// hymoe_forward; adapted: with the layer's adapters, ids [n_tokens] (x's memory kind) naming each
+// token's (nullptr: adapter 0).
+static hymoe_status forward_call(hymoe_ctx* c, uint32_t layer, const float* x, const float* residual,
+                                 float* out, uint32_t n_tokens, const float* router_bias,
+                                 hymoe_debug* dbg, int flags, const int32_t* ids, bool adapted) {
     if (!c) return HYMOE_ERR_INVALID_ARG;
     if (layer >= c->layers.size() || !c->layers[layer].loaded)
         return c->fail(HYMOE_ERR_STATE, "layer %u not loaded", layer);
@@ -1527,6 +1625,11 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
             HY_CUDA(c, dalloc(&c->dbg_idx, static_cast<size_t>(max_tok) * K));
         }
         // both copy streams follow earlier work on the compute stream (they rewrite x_dev / out_dev)
+        const int32_t* dids = ids;
+        if (adapted && ids && T > 0) {
+            HY_CUDA(c, cudaMemcpyAsync(c->ad_ids, ids, sizeof(int32_t) * T, cudaMemcpyHostToDevice, st));
+            dids = c->ad_ids;
+        }
         std::vector<cudaEvent_t> evs;
         auto ev = [&]() {
             evs.push_back(c->take_event());
@@ -1560,8 +1663,8 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
                 d2.topk_weights = dbg->topk_weights ? c->dbg_w + static_cast<size_t>(t0) * K : nullptr;
                 d2.topk_indices = dbg->topk_indices ? c->dbg_idx + static_cast<size_t>(t0) * K : nullptr;
             }
-            result = hymoe_forward(c, layer, c->x_dev + off, r, c->out_dev + off, static_cast<uint32_t>(n), dbias,
-                                   dbg ? &d2 : nullptr, flags & ~HYMOE_HOST_PTRS);
+            result = forward_call(c, layer, c->x_dev + off, r, c->out_dev + off, static_cast<uint32_t>(n), dbias,
+                                  dbg ? &d2 : nullptr, flags & ~HYMOE_HOST_PTRS, dids ? dids + t0 : nullptr, adapted);
             cudaEvent_t done = ev();
             HY_CUDA(c, cudaEventRecord(done, st));
             HY_CUDA(c, cudaStreamWaitEvent(down, done, 0));
@@ -1610,7 +1713,13 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
         }
         if (dlog) dlog = c->logits;
         if (dprob) dprob = c->probs;
+        if (adapted && ids && T > 0) {
+            HY_CUDA(c, cudaMemcpyAsync(c->ad_ids, ids, sizeof(int32_t) * T, cudaMemcpyHostToDevice, st));
+            ids = c->ad_ids;
+        }
     }
+    const hymoe_adapters* ad_gu = adapted && c->ad_gu[layer].rank ? &c->ad_gu[layer] : nullptr;
+    const hymoe_adapters* ad_dn = adapted && c->ad_dn[layer].rank ? &c->ad_dn[layer] : nullptr;
     // A rank with no tokens still takes part in every collective of the exchange.
     if (T == 0 && !ep) return host ? hymoe_synchronize(c) : HYMOE_OK;
 
@@ -1674,7 +1783,7 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
         };
         // 1..8 tokens on one GPU (Q4_0 / Q8_0, no capacity drops): the whole block is one
         // cooperative kernel (decode.cu), timed as the gate_up phase.
-        if (c->dec_ok && !ep && T >= 1 && T <= kDecodeMaxT && !c->route.drop &&
+        if (c->dec_ok && !ep && T >= 1 && T <= kDecodeMaxT && !c->route.drop && !c->gated && !ad_gu && !ad_dn &&
             (L.wtype == W_Q4_0 || L.wtype == W_Q8_0) && K <= 8 && decode_smem(L.wtype, T, H, E) != 0) {
             DecodeArgs da{};
             da.x = dx;
@@ -1738,13 +1847,14 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
         // leaving SMs to them); the combine joins both streams.  From 4 tokens on the router's
         // chains last long enough to hide it (measured: T=8 0.357 -> 0.351 ms; at T=1 the fork
         // outlasted the front end and delayed the routed launch, 0.105 -> 0.119 ms).
-        const bool shared_apart = !ep && gemv && T >= 4 && T <= 8 && (L.wtype == W_Q4_0 || L.wtype == W_Q8_0);
+        // (Not with adapters, whose products join the shared expert's in this stream.)
+        const bool shared_apart = !ep && gemv && T >= 4 && T <= 8 && (L.wtype == W_Q4_0 || L.wtype == W_Q8_0) && !ad_gu && !ad_dn;
         // Decode-size chains on one GPU (1..64 tokens, weight-streaming kernels): router (and
         // top-K), plan, scatter, gate_up, down and combine are launched with programmatic
         // dependent launch, so each is scheduled while its predecessor finishes (every one of
         // these kernels waits for its predecessor's completion before it reads anything).
         const bool pdl = c->pdl && !ep && gemv && T >= 1 && T <= kGemvMaxRows && !c->route.drop &&
-                         (L.wtype == W_Q4_0 || L.wtype == W_Q8_0);
+                         (L.wtype == W_Q4_0 || L.wtype == W_Q8_0) && !ad_gu && !ad_dn;
         if (shared_apart) {
             cudaStream_t side = c->side_stream;
             HY_CUDA(c, cudaEventRecord(c->ev_fork, st));
@@ -1761,11 +1871,14 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
             const int n_chunks = (T + kRouterTok - 1) / kRouterTok;
             // T <= 16 (one router chunk): the top-K runs inside the plan launch (not with
             // capacity drops, which need every token's choices before the plan).
-            const bool fused = n_chunks == 1 && !c->route.drop;
+            const bool fused = n_chunks == 1 && !c->route.drop && !c->gated;
             c->phase_begin();
             HY_CUDA(c, launch_router(dxn, T, H, L.router, E, K, dbias, dlog ? dlog : c->logits, dprob,
-                                     c->topk_w, c->topk_idx, c->chunk_counts, slot_of, c->route, !fused, st,
+                                     c->topk_w, c->topk_idx, c->chunk_counts, slot_of, c->route, !fused && !c->gated, st,
                                      nrm, pdl));
+            if (c->gated)
+                HY_CUDA(c, launch_gate_block(dlog ? dlog : c->logits, T, E, K, c->gate, c->gate_bias[layer], dprob, c->topk_w,
+                                             c->topk_idx, c->chunk_counts, slot_of, st, pdl));
             c->phase_end(HYMOE_PHASE_ROUTER, fused ? 1 : 2);
             if (c->route.drop) {
                 // topkgating_full's capacity with drop_tokens (src/hunyuan_moe_full.cpp:205-224):
@@ -1941,13 +2054,25 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
             fuse.epoch = epoch;
             fuse.budget_ns = budget_ns;
         }
+        // The shared expert's adapters (rows [0, T) of xp and hbuf are its inputs): gate_up's go into
+        // the sums before the SwiGLU, down's onto its result.
+        auto adapt = [&](const hymoe_adapters* ad, __half* in, int n_in, const float* base, float* res, int n_out) -> hymoe_status {
+            const hymoe_mat mx{in, HYMOE_TYPE_F16, n_in}, mb{const_cast<float*>(base), HYMOE_TYPE_F32, n_out}, mo{res, HYMOE_TYPE_F32, n_out};
+            const hymoe_status sa = hymoe_adapt(ad, &mx, ids, n_tokens, base ? &mb : nullptr, &mo, c->ad_ws, c->ad_ws_bytes, st);
+            return sa == HYMOE_OK ? sa : c->fail(sa, "adapters: %s", hymoe_last_error(nullptr));
+        };
+        if (ad_gu) {
+            const hymoe_status sa = adapt(ad_gu, c->xp, H, nullptr, c->ad_delta, 2 * I);
+            if (sa != HYMOE_OK) return sa;
+        }
+        const float* glu_add = ad_gu ? c->ad_delta : nullptr;
         if (gemv) {
             const int max_it = static_cast<int>(std::min<size_t>(
                 c->max_items, static_cast<size_t>(tiles_gu) * ((rows_in_use + kGemvMaxRows - 1) / kGemvMaxRows + kMaxSegs)));
             c->phase_begin();
             const int mr = static_cast<int>(std::max<size_t>(1, gemv_rows));
             HY_CUDA(c, launch_gemv(c->gmaps_xp, c->items_gu, c->n_items, max_it, L.d_gu_ptrs, L.wtype, H / kTileK,
-                                   1, mr, c->hbuf, I, nullptr, 0, c->err_word, c->n_sms, st, pdl));
+                                   1, mr, c->hbuf, I, nullptr, glu_add ? T : 0, c->err_word, c->n_sms, st, pdl, glu_add));
             c->phase_end(HYMOE_PHASE_GATE_UP);
             c->phase_begin();
             HY_CUDA(c, launch_gemv(c->gmaps_h, c->items_dn, c->n_items + 1, max_it, L.d_dn_ptrs, L.wtype,
@@ -1969,6 +2094,8 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
             ga.n_rb = tiles_gu;
             ga.glu = 1;
             ga.out = c->hbuf;
+            ga.glu_add = glu_add;
+            ga.shared_rows = glu_add ? T : 0;
             ga.out_ld = I;
             ga.err = c->err_word;
             ga.ep_mode = p2p ? 1 : 0;  // fused: the remote rows leave and arrive during the GEMM
@@ -2021,6 +2148,10 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
             y_routed = c->y_ret;
         }
         if (shared_apart) HY_CUDA(c, cudaStreamWaitEvent(st, c->ev_join, 0));  // the shared expert's rows of y
+        if (ad_dn) {
+            const hymoe_status sa = adapt(ad_dn, c->hbuf, I, c->y, c->y, H);
+            if (sa != HYMOE_OK) return sa;
+        }
         if (T > 0) {
             c->phase_begin();
             HY_CUDA(c, launch_combine(c->y, y_routed, c->slot_pos, c->topk_w, dres, dout, T, H, K, st,
@@ -2039,7 +2170,8 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
     } else {
         // One captured graph per (layer, token count, buffers); replayed while they repeat.
         const GraphKey key{layer | (pre_norm ? 0x80000000u : 0u), n_tokens, dx, dres, dout, dbias, dlog, dprob,
-                           dbg ? dbg->topk_weights : nullptr, dbg ? dbg->topk_indices : nullptr};
+                           dbg ? dbg->topk_weights : nullptr, dbg ? dbg->topk_indices : nullptr,
+                           ad_gu || ad_dn ? (ids ? static_cast<const void*>(ids) : static_cast<const void*>(c)) : nullptr};
         auto hit = c->graphs.find(key);
         if (hit == c->graphs.end()) {
             if (c->graphs.size() >= 64) c->clear_graphs();
@@ -2065,6 +2197,22 @@ hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const f
         return hymoe_synchronize(c);
     }
     return HYMOE_OK;
+}
+
+hymoe_status hymoe_forward(hymoe_ctx* c, uint32_t layer, const float* x, const float* residual,
+                           float* out, uint32_t n_tokens, const float* router_bias,
+                           hymoe_debug* dbg, int flags) {
+    return forward_call(c, layer, x, residual, out, n_tokens, router_bias, dbg, flags, nullptr, false);
+}
+
+hymoe_status hymoe_forward_adapted(hymoe_ctx* c, uint32_t layer, const float* x, const float* residual,
+                                   float* out, uint32_t n_tokens, const float* router_bias,
+                                   const int32_t* adapter_ids, hymoe_debug* dbg, int flags) {
+    if (!c) return HYMOE_ERR_INVALID_ARG;
+    if (layer >= c->layers.size()) return c->fail(HYMOE_ERR_INVALID_ARG, "layer %u out of range", layer);
+    if (!c->ad_gu[layer].rank && !c->ad_dn[layer].rank)
+        return c->fail(HYMOE_ERR_STATE, "layer %u has no adapters (hymoe_set_adapters)", layer);
+    return forward_call(c, layer, x, residual, out, n_tokens, router_bias, dbg, flags, adapter_ids, true);
 }
 
 hymoe_status hymoe_profile(hymoe_ctx* c, int enable) {

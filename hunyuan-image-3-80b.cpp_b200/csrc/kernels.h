@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/hymoe.h"
+
 namespace hymoe {
 
 // ---- weights.cu
@@ -65,6 +67,13 @@ cudaError_t launch_router(const float* x, int T, int H, const float* Wr, int E, 
                           const RouteMode& mode, bool topk, cudaStream_t st, const RowNorm& nrm = {},
                           bool pdl = false);
 
+// ---- gate_f32.cu: a gate's routing (hymoe_set_gate) of the block's own logits [T, E], E <= 64: the
+// same outputs as launch_router's top-K step (entries without an expert: index -1, weight 0, not
+// counted).  probs: every score, or nullptr.  bias: the selection's, or nullptr.
+cudaError_t launch_gate_block(const float* logits, int T, int E, int K, const hymoe_gate& gate, const float* bias,
+                              float* probs, float* topk_w, int* topk_idx, int* chunk_counts, const int* slot_of,
+                              cudaStream_t st, bool pdl = false);
+
 // ---- dispatch.cu
 constexpr int kMaxSegs = 80;  // >= E + 1 (E <= 64)
 struct ItemsArgs {
@@ -114,6 +123,7 @@ cudaError_t launch_capacity_job(int* topk_idx, float* topk_w, int* chunk_counts,
                                 const int* recs, int N, int me, float cf, int min_capacity, cudaStream_t st);
 // idx[i] = expert_of_slot[idx[i]] for i < n (top-K slots back to expert ids for the caller);
 // the dropped-pair bit is cleared; expert_of_slot == nullptr: identity (only the bit is cleared).
+// Negative entries (no expert) stay.
 cudaError_t launch_unmap_slots(int* idx, const int* expert_of_slot, int n, cudaStream_t st);
 
 // xp_shared == nullptr: the shared expert's rows are written elsewhere (launch_shared_prep).
@@ -223,6 +233,8 @@ struct GemmArgs {
     void* out;                     // gate_up: fp16 [rows, out_ld]; down: fp32 rows [0, shared_rows)
     __half* out_r;                 // down: fp16 rows [shared_rows, ...) (routed results)
     int shared_rows;
+    const float* glu_add;          // gate_up: [shared_rows][2 out_ld] (gate half, up half) added to
+                                   // the sums of rows below shared_rows before the SwiGLU, or nullptr
     int out_ld;
     int* err;
     int ep_mode;                   // 0: none; 1: gate_up with the token-row sends; 2: down with
@@ -240,11 +252,12 @@ struct GemvMaps {
 // max_rows: the largest item (<= kGemvMaxRows); it sizes the activation stages.  Items of at
 // most 8 rows (Q4_0 / Q8_0) run on the persistent streaming variant with n_sms CTAs.
 // glu = 0 (down projection): rows below shared_rows go to `out` (fp32), the others to
-// `out_r` (fp16, routed results); glu = 1: `out` fp16.
+// `out_r` (fp16, routed results); glu = 1: `out` fp16, and glu_add [shared_rows][2 out_ld] (gate
+// half, up half; nullable) is added to the gate and up sums of rows below shared_rows first.
 cudaError_t launch_gemv(const GemvMaps& maps, const int4* items, const int* n_items, int max_items,
                         const uint8_t* const* wtiles, int wtype, int n_ks, int glu, int max_rows,
                         void* out, int out_ld, __half* out_r, int shared_rows, int* err, int n_sms,
-                        cudaStream_t st, bool pdl = false);
+                        cudaStream_t st, bool pdl = false, const float* glu_add = nullptr);
 
 // ---- decode.cu
 // The whole block for 1..8 tokens on one GPU (Q4_0 / Q8_0 weights) as one persistent

@@ -33,7 +33,8 @@ EXPORTS = ["hymoe_version", "hymoe_nccl_unique_id", "hymoe_create", "hymoe_destr
            "hymoe_gguf_get_u32", "hymoe_gguf_moe_tensors", "hymoe_load_layer_gguf",
            "hymoe_set_norm", "hymoe_set_routing", "hymoe_load_layer_async", "hymoe_wait_layer",
            "hymoe_load_layer_gguf_async", "hymoe_route", "hymoe_route_backward",
-           "hymoe_adapt_workspace", "hymoe_adapt", "hymoe_adapt_backward"]
+           "hymoe_adapt_workspace", "hymoe_adapt", "hymoe_adapt_backward", "hymoe_set_gate",
+           "hymoe_set_balance_bias", "hymoe_set_adapters", "hymoe_forward_adapted"]
 
 PHASES = ["router", "plan", "dispatch", "gate_up", "down", "combine", "ep_dispatch",
           "ep_combine", "copy_in", "copy_out"]
@@ -136,6 +137,10 @@ def lib() -> C.CDLL:
         L.hymoe_route.argtypes = [C.POINTER(GateSpec), C.POINTER(Mat), vp, u32, u32, u32, vp, vp, vp, vp, vp]
         L.hymoe_route_backward.argtypes = [C.POINTER(GateSpec), C.POINTER(Mat), vp, vp, vp, u32, u32, u32,
                                            C.POINTER(Mat), vp]
+        L.hymoe_set_gate.argtypes = [vp, C.POINTER(GateSpec)]
+        L.hymoe_set_balance_bias.argtypes = [vp, u32, vp, C.c_int]
+        L.hymoe_set_adapters.argtypes = [vp, u32, C.POINTER(AdapterSpec), C.POINTER(AdapterSpec)]
+        L.hymoe_forward_adapted.argtypes = [vp, u32, vp, vp, vp, u32, vp, vp, C.POINTER(Debug), C.c_int]
         L.hymoe_adapt_workspace.argtypes = [C.POINTER(AdapterSpec), u32, C.c_int, C.POINTER(C.c_size_t)]
         L.hymoe_adapt.argtypes = [C.POINTER(AdapterSpec), C.POINTER(Mat), vp, u32, C.POINTER(Mat), C.POINTER(Mat), vp,
                                   C.c_size_t, vp]
@@ -345,6 +350,30 @@ class MoE:
                     min_capacity, 1 if norm_topk_prob else 0, scale)
         self._check(self.L.hymoe_set_routing(self.h, C.byref(r)))
 
+    def set_gate(self, gate: "Gate | None") -> None:
+        """Routing by a gate (its experts and topk must be the context's); None: the default."""
+        if gate is not None and (gate.E, gate.K) != (self.E, self.K):
+            raise ValueError(f"gate of {gate.E} experts, topk {gate.K}; the context has {self.E} and {self.K}")
+        self._check(self.L.hymoe_set_gate(self.h, C.byref(gate.spec) if gate is not None else None))
+
+    def set_balance_bias(self, layer: int, bias) -> None:
+        """The gate's selection bias [E] of a layer (host numpy float32; None removes it)."""
+        import numpy as np
+        if bias is None:
+            self._check(self.L.hymoe_set_balance_bias(self.h, layer, None, HOST_PTRS))
+            return
+        b = np.ascontiguousarray(bias, dtype=np.float32)
+        if b.shape != (self.E,):
+            raise ValueError(f"balance bias must be [{self.E}], got {b.shape}")
+        self._check(self.L.hymoe_set_balance_bias(self.h, layer, b.ctypes.data, HOST_PTRS))
+
+    def set_adapters(self, layer: int, gate_up: "Adapters | None" = None, down: "Adapters | None" = None) -> None:
+        """Adapters of the layer's shared expert (kept alive by this object until replaced)."""
+        self._check(self.L.hymoe_set_adapters(self.h, layer, C.byref(gate_up.spec) if gate_up else None,
+                                              C.byref(down.spec) if down else None))
+        self._adapters = getattr(self, "_adapters", {})
+        self._adapters[layer] = (gate_up, down)
+
     def set_norm(self, layer: int, weight, eps: float) -> None:
         """Post-attention RMSNorm weights [H] (host numpy float32; None removes them)."""
         import numpy as np
@@ -364,9 +393,10 @@ class MoE:
         self._check(self.L.hymoe_synth_layer(self.h, layer, wtype, seed, std))
 
     def forward_host(self, layer: int, x, resid=None, bias=None, debug: bool = False,
-                     pre_norm: bool = False) -> dict:
+                     pre_norm: bool = False, adapter_ids=None) -> dict:
         """x (and resid) float32 [T, H] numpy; returns numpy outputs.  pre_norm: x is the
-        un-normalised hidden state (HYMOE_PRE_NORM); resid="x" passes x itself as residual."""
+        un-normalised hidden state (HYMOE_PRE_NORM); resid="x" passes x itself as residual.
+        adapter_ids int32 [T]: with the layer's adapters (set_adapters)."""
         import numpy as np
         x = np.ascontiguousarray(x, dtype=np.float32)
         T = x.shape[0]
@@ -382,21 +412,31 @@ class MoE:
         r = None if resid is None else x if isinstance(resid, str) and resid == "x" else \
             np.ascontiguousarray(resid, dtype=np.float32)
         b = None if bias is None else np.ascontiguousarray(bias, dtype=np.float32)
-        self._check(self.L.hymoe_forward(self.h, layer, x.ctypes.data,
-                                         None if r is None else r.ctypes.data, out.ctypes.data, T,
-                                         None if b is None else b.ctypes.data,
-                                         C.byref(dbg) if dbg else None,
-                                         HOST_PTRS | (PRE_NORM if pre_norm else 0)))
+        args = (self.h, layer, x.ctypes.data, None if r is None else r.ctypes.data, out.ctypes.data, T,
+                None if b is None else b.ctypes.data)
+        d, flags = C.byref(dbg) if dbg else None, HOST_PTRS | (PRE_NORM if pre_norm else 0)
+        if adapter_ids is None:
+            self._check(self.L.hymoe_forward(*args, d, flags))
+        else:
+            ids = np.ascontiguousarray(adapter_ids, dtype=np.int32)
+            if ids.shape != (T,):
+                raise ValueError(f"adapter_ids must be [{T}], got {ids.shape}")
+            self._check(self.L.hymoe_forward_adapted(*args, ids.ctypes.data, d, flags))
         return res
 
     def forward_device(self, layer: int, x_ptr: int, out_ptr: int, T: int, resid_ptr=None,
                        bias_ptr=None, dbg: Debug | None = None, host: bool = False,
-                       graph: bool = False, pre_norm: bool = False) -> None:
+                       graph: bool = False, pre_norm: bool = False, adapter_ids_ptr=None) -> None:
         """Raw pointers (device memory unless host=True); asynchronous on the set stream.
-        graph=True replays a captured CUDA graph for repeated (layer, T, pointers)."""
+        graph=True replays a captured CUDA graph for repeated (layer, T, pointers).
+        adapter_ids_ptr: with the layer's adapters (set_adapters)."""
         flags = (HOST_PTRS if host else 0) | (USE_GRAPH if graph else 0) | (PRE_NORM if pre_norm else 0)
-        self._check(self.L.hymoe_forward(self.h, layer, x_ptr, resid_ptr, out_ptr, T, bias_ptr,
-                                         C.byref(dbg) if dbg else None, flags))
+        d = C.byref(dbg) if dbg else None
+        if adapter_ids_ptr is None:
+            self._check(self.L.hymoe_forward(self.h, layer, x_ptr, resid_ptr, out_ptr, T, bias_ptr, d, flags))
+        else:
+            self._check(self.L.hymoe_forward_adapted(self.h, layer, x_ptr, resid_ptr, out_ptr, T, bias_ptr,
+                                                     adapter_ids_ptr, d, flags))
 
 
 # ---- Operators on the caller's device buffers: torch CUDA tensors in, torch CUDA tensors out,

@@ -124,7 +124,8 @@ void hymoe_destroy(hymoe_ctx* ctx);
 /* Message of the last failing call on this context ("" when none).  With ctx == NULL,
  * the last failure of hymoe_create on this thread. */
 const char* hymoe_last_error(const hymoe_ctx* ctx);
-/* (With ctx == NULL it also reports the last failure of hymoe_ffn_noalloc on this thread.) */
+/* (With ctx == NULL it also reports the last failure on this thread of hymoe_ffn_noalloc and of the
+ * other calls that take no context.) */
 
 /* Makes subsequent work run on `stream` (a cudaStream_t; NULL = the context's own). */
 hymoe_status hymoe_set_stream(hymoe_ctx* ctx, void* stream);
@@ -420,6 +421,37 @@ hymoe_status hymoe_adapt_backward(const hymoe_adapters* adapters, const hymoe_ma
                                   const int32_t* ids, uint32_t n_tokens, const hymoe_mat* base,
                                   const hymoe_mat* dx, float* da, float* db, void* workspace,
                                   size_t workspace_bytes, void* stream);
+
+/* ---- The same operators inside the block (one GPU; HYMOE_ERR_UNSUPPORTED with expert
+ * parallelism). */
+
+/* Routing of every later call of the context by a gate, n_experts and topk the context's; replaces
+ * hymoe_set_routing's variant (and is replaced by it).  NULL restores moe_forward_cpu's routing.
+ * The router's logits (+ router_bias) are the gate's; an expert whose logit is -inf takes no tokens,
+ * and entries of a token that has fewer than topk open experts add nothing (debug index -1, weight
+ * 0).  The debug probabilities are the gate's scores.  Every token count is supported; the
+ * one-kernel decode path is not used. */
+hymoe_status hymoe_set_gate(hymoe_ctx* ctx, const hymoe_gate* gate);
+
+/* The gate's selection bias of one layer: [E] F32 (host memory with HYMOE_HOST_PTRS, else device),
+ * copied; NULL removes it.  Used while a gate is set. */
+hymoe_status hymoe_set_balance_bias(hymoe_ctx* ctx, uint32_t layer, const float* bias, int flags);
+
+/* Adapters of one layer's shared expert for hymoe_forward_adapted, HYMOE_TYPE_F16: gate_up (H ->
+ * 2I: gate rows, then up rows) joins the projection before the SwiGLU, down (I -> H) its result;
+ * either may be NULL, both NULL remove them.  The weights are read where they are, in device memory
+ * of the context's device: keep them until they are replaced or the context is destroyed.  The first
+ * calls allocate the context's scratch for them. */
+hymoe_status hymoe_set_adapters(hymoe_ctx* ctx, uint32_t layer, const hymoe_adapters* gate_up,
+                                const hymoe_adapters* down);
+
+/* hymoe_forward with the layer's adapters: adapter_ids [n_tokens] (the same memory kind as x) names
+ * every token's adapter in both projections; a token whose id is outside an adapter set's range has
+ * none there.  NULL: adapter 0 for every token.  hymoe_forward itself leaves the adapters out.
+ * HYMOE_ERR_STATE where the layer has none. */
+hymoe_status hymoe_forward_adapted(hymoe_ctx* ctx, uint32_t layer, const float* x, const float* residual,
+                                   float* out, uint32_t n_tokens, const float* router_bias,
+                                   const int32_t* adapter_ids, hymoe_debug* dbg, int flags);
 
 /* ---- GGUF weight files (replaces HunyuanGGUFLoader, src/hunyuan_gguf_loader.h:20-71, for
  * the MoE tensors).  A file (GGUF version 2 or 3) is parsed by the library and mapped
