@@ -187,7 +187,7 @@ AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward) {
         l.bytes += (bytes + 255) / 256 * 256;
         return at;
     };
-    if (T == 0) return l;
+    if (T == 0 || (!backward && adapt_decodes(T, static_cast<int>(ad->rank)))) return l;
     const size_t long_pieces = T / kAdMinChunk < kAdMaxPieces ? T / kAdMinChunk : kAdMaxPieces;  // T / adapt_chunk at most
     l.max_tiles = static_cast<int>(T / kAdRows + (n + 1 < T ? n + 1 : T));
     l.max_items = static_cast<int>(n + long_pieces);
@@ -381,6 +381,31 @@ extern "C" hymoe_status hymoe_adapt(const hymoe_adapters* ad, const hymoe_mat* x
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int n = static_cast<int>(ad->n_adapters), R = static_cast<int>(ad->rank), t = static_cast<int>(T);
     const int n_sms = sm_count(dev);
+    if (adapt_decodes(T, R)) {
+        AdaptDecode d{};
+        d.x = x->data;
+        d.base = base ? base->data : nullptr;
+        d.out = out->data;
+        d.ids = ids;
+        d.a = ad->a;
+        d.b = ad->b;
+        d.scale = ad->scale;
+        d.ldx = static_cast<size_t>(x->ld);
+        d.ldb = base ? static_cast<size_t>(base->ld) : 0;
+        d.ldo = static_cast<size_t>(out->ld);
+        d.n = n;
+        d.R = R;
+        d.K = static_cast<int>(I);
+        d.N = static_cast<int>(O);
+        d.ctas = T <= 16 ? 16 : 8;
+        d.vec_x = rows_vec(x->data, 0, elem_bytes(x->type)) && (T == 1 || rows_vec(x->data, d.ldx, elem_bytes(x->type)));
+        d.vec_a = rows_vec(ad->a, I, 2);
+        d.vec_b = rows_vec(ad->b, R, 2);
+        d.in_place = base && base->data == out->data;
+        if (launch_adapt_decode(d, x->type, ad->type, out->type, t, st) != cudaSuccess)
+            return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt: kernel launch failed");
+        return HYMOE_OK;
+    }
     const AdaptLayout l = adapt_layout(ad, T, false);
     char* ws = static_cast<char*>(workspace);
     const AdaptPlan plan = plan_in(l, ws, false);

@@ -49,6 +49,10 @@ __host__ __device__ constexpr int adapt_splits(int tiles, int K, int slots) {
     return s < 1 ? 1 : s;
 }
 
+// Whether hymoe_adapt runs as clusters per token: the weights are read once per token, so up to 64
+// tokens and fewer where the rank is high.
+__host__ __device__ constexpr bool adapt_decodes(size_t T, int R) { return T <= 64 && T * adapt_rp(R) <= 4096; }
+
 // What the plan kernel writes: tokens in the order of their adapters (stable; those without one
 // last) and the work lists over that order.
 struct AdaptPlan {
@@ -93,6 +97,21 @@ struct AdaptGrad {     // G_a(m, j) = sum over a's rows of X[perm[row], m] low[r
     int M, R, gm, gj;
     int vec_x;
 };
+
+struct AdaptDecode {   // hymoe_adapt for a few tokens: clusters of `ctas` CTAs per token
+    const void* x;
+    const void* base;  // nullptr: zeros
+    void* out;
+    const int* ids;
+    const void* a;
+    const void* b;
+    const float* scale;
+    size_t ldx, ldb, ldo;
+    int n, R, K, N, ctas;
+    int vec_x, vec_a, vec_b;  // rows start on 16-byte boundaries
+    int in_place;
+};
+cudaError_t launch_adapt_decode(const AdaptDecode& d, int type_x, int type_w, int type_y, int T, cudaStream_t st);
 
 // type_x: HYMOE_TYPE_F32 or type_w; trans: the weight matrix has the rank as its fast dimension
 // (low) or the columns as its fast dimension (wide).
