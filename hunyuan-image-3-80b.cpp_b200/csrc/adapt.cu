@@ -10,8 +10,9 @@
 // adapt_grad.cu hold the three products.
 #include <initializer_list>
 
-#include "adapt.cuh"
-#include "kernels.h"
+#include <cudaTypedefs.h>
+
+#include "adapt_tc.cuh"
 
 namespace hymoe {
 namespace {
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
     };
     fetch(t_lo);
     for (int i = tid; i < W * nb; i += kPlanThreads) cnt[i] = 0;
-    for (int i = tid; i < p.max_tiles; i += kPlanThreads) p.counters[i] = 0u;
+    for (int i = tid; i < p.max_tiles * (p.tile_rows / kAdRows); i += kPlanThreads) p.counters[i] = 0u;
     __syncthreads();
     int* mine = cnt + (warp < W ? warp : 0) * nb;
     for (int t0 = t_lo; t0 < t_hi; t0 += 256) {
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
         if (lane == 31) {
             tot[a] = inc;
             off[a] = inc;
-            tpre[a] = (inc + kAdRows - 1) / kAdRows;
+            tpre[a] = (inc + p.tile_rows - 1) / p.tile_rows;
             const int pieces = a < n ? max(1, (inc + chunk - 1) / chunk) : 0;
             ipre[a] = pieces;
             spre[a] = pieces > 1 ? pieces : 0;
@@ -150,8 +151,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
     }
     const int n_tiles = tpre[nb];
     for (int i = tid; i < n_tiles; i += kPlanThreads) {
-        const int a = bucket_of(tpre, nb, i), r = (i - tpre[a]) * kAdRows;
-        p.tiles[i] = make_int4(a < n ? a : -1, off[a] + r, min(kAdRows, tot[a] - r), 0);
+        const int a = bucket_of(tpre, nb, i), r = (i - tpre[a]) * p.tile_rows;
+        p.tiles[i] = make_int4(a < n ? a : -1, off[a] + r, min(p.tile_rows, tot[a] - r), 0);
     }
     if (p.items != nullptr) {
         const int n_items = ipre[n];
@@ -161,9 +162,13 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
             p.items[i] = make_int4(a, off[a] + r, min(chunk, tot[a] - r), several ? spre[a] + q : -1);
         }
         for (int a = tid; a <= n; a += kPlanThreads) p.pieces[a] = ipre[a];
-        if (tid == 0) p.n_lists[1] = n_items;
+        if (tid == 0) p.n_lists[2] = n_items;
     }
-    if (tid == 0) p.n_lists[0] = n_tiles;
+    if (tid == 0) {
+        p.n_lists[0] = 0;
+        p.n_lists[1] = n_tiles;
+        p.n_lists[3] = tpre[n];
+    }
 }
 
 cudaError_t launch_plan_adapt(const int* ids, int T, int n, const AdaptPlan& p, cudaStream_t st) {
@@ -177,9 +182,10 @@ cudaError_t launch_plan_adapt(const int* ids, int T, int n, const AdaptPlan& p, 
 // The workspace: every part starts on 256 bytes.
 struct AdaptLayout {
     size_t perm, tiles, items, pieces, lists, counters, low, low2, low_part, part, bytes;
-    int max_tiles, max_items;
+    int tile_rows, max_tiles, max_items;
 };
-AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward) {
+// (the sizes do not depend on tile_rows)
+AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward, int tile_rows = kAdRows) {
     AdaptLayout l{};
     const size_t n = ad->n_adapters;
     auto take = [&](size_t bytes) {
@@ -189,14 +195,17 @@ AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward) {
     };
     if (T == 0 || (!backward && adapt_decodes(T, static_cast<int>(ad->rank)))) return l;
     const size_t long_pieces = T / kAdMinChunk < kAdMaxPieces ? T / kAdMinChunk : kAdMaxPieces;  // T / adapt_chunk at most
-    l.max_tiles = static_cast<int>(T / kAdRows + (n + 1 < T ? n + 1 : T));
+    const size_t buckets = n + 1 < T ? n + 1 : T;                   // adapters that have tokens, at most
+    const size_t tiles64 = T / kAdRows + buckets, half_tiles = tiles64 + buckets;  // also twice the tiles of 128
+    l.tile_rows = tile_rows;
+    l.max_tiles = static_cast<int>(T / tile_rows + buckets);
     l.max_items = static_cast<int>(n + long_pieces);
-    l.lists = take(2 * sizeof(int));
+    l.lists = take(4 * sizeof(int));
     l.perm = take(T * sizeof(int));
-    l.tiles = take(static_cast<size_t>(l.max_tiles) * sizeof(int4));
-    l.counters = take(static_cast<size_t>(l.max_tiles) * sizeof(unsigned));
+    l.tiles = take(tiles64 * sizeof(int4));
+    l.counters = take(half_tiles * sizeof(unsigned));
     l.low = take(T * adapt_rp(ad->rank) * sizeof(float));
-    const size_t shared_tiles = static_cast<size_t>(l.max_tiles) * kAdMaxSplits;
+    const size_t shared_tiles = half_tiles * kAdMaxSplits;
     l.low_part = take((shared_tiles < kAdMaxSlots ? shared_tiles : kAdMaxSlots) * kAdRows * adapt_rp(ad->rank) * sizeof(float));
     if (backward) {
         l.items = take(static_cast<size_t>(l.max_items) * sizeof(int4));
@@ -215,6 +224,7 @@ AdaptPlan plan_in(const AdaptLayout& l, char* ws, bool backward) {
     p.pieces = backward ? reinterpret_cast<int*>(ws + l.pieces) : nullptr;
     p.n_lists = reinterpret_cast<int*>(ws + l.lists);
     p.counters = reinterpret_cast<unsigned*>(ws + l.counters);
+    p.tile_rows = l.tile_rows;
     p.max_tiles = l.max_tiles;
     p.max_items = l.max_items;
     return p;
@@ -288,8 +298,62 @@ int sm_count(int dev) {
     return n < 1 ? 1 : n < kAdMaxSlots / 4 ? n : kAdMaxSlots / 4;
 }
 
+// ---- tensor maps of the tcgen05 kernels
+
+using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
+EncodeFn encode_fn() {
+    static const EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+bool encode(CUtensorMap* m, int type, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+            const cuuint32_t* box) {
+    const EncodeFn fn = encode_fn();
+    const cuuint32_t ones[3] = {1, 1, 1};
+    const CUtensorMapDataType t = type == HYMOE_TYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : type == HYMOE_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return fn && fn(m, t, rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Token rows [T, cols], boxes of 128 bytes of `rows` rows.
+bool encode_rows(AdaptMaps* m, const hymoe_mat& x, int T, int cols, int rows) {
+    const size_t es = elem_bytes(x.type);
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(T)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(T > 1 ? x.ld : cols) * es};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(rows)};
+    return encode(&m->rows, x.type, 2, x.data, dims, strides, box);
+}
+
+// Weights [n][rows][cols], boxes of 64 columns and `box_rows` rows of one adapter.
+bool encode_weights(AdaptMaps* m, const void* w, int type, int n, int rows, int cols, int box_rows) {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(n)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols) * 2, static_cast<cuuint64_t>(cols) * rows * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+    return encode(&m->w, type, 3, w, dims, strides, box);
+}
+
+// Rows that TMA can load in pieces of 128 bytes.
+bool rows_tma(const hymoe_mat* m, uint32_t cols) {
+    const size_t es = elem_bytes(m->type);
+    return rows_vec(m->data, static_cast<size_t>(m->ld), es) && static_cast<size_t>(m->ld) * es < (size_t(1) << 40) &&
+           cols * es % 16 == 0 && cols >= 64;
+}
+bool weights_tma(const hymoe_adapters* ad) {
+    return ad->rank % 8 == 0 && ad->in_features % 8 == 0 && ad->out_features % 8 == 0 && entry_aligned(ad->a, 16) &&
+           entry_aligned(ad->b, 16);
+}
+
 cudaError_t run_low(const AdaptPlan& plan, const hymoe_mat& x, const void* w, int type_w, bool trans, const float* scale,
-                    float* low, float* part, int R, int K, int n_sms, cudaStream_t st) {
+                    float* low, float* part, int R, int K, int T, int n, bool tc, int n_sms, cudaStream_t st) {
     AdaptLow a{};
     a.plan = plan;
     a.x = x.data;
@@ -300,13 +364,20 @@ cudaError_t run_low(const AdaptPlan& plan, const hymoe_mat& x, const void* w, in
     a.part = part;
     a.K = K;
     a.R = R;
+    if (tc) {
+        AdaptMaps m;
+        if (!encode_rows(&m, x, T, K, kTcRows) ||
+            !(trans ? encode_weights(&m, w, type_w, n, K, R, 64) : encode_weights(&m, w, type_w, n, R, K, adapt_rp(R))))
+            return cudaErrorInvalidValue;
+        return launch_adapt_low_tc(m, a, type_w, trans, n_sms, st);
+    }
     a.vec_x = rows_vec(x.data, a.ldx, elem_bytes(x.type));
     a.vec_w = rows_vec(w, trans ? R : K, 2);
     return launch_adapt_low(a, x.type, type_w, trans, n_sms, st);
 }
 
 cudaError_t run_wide(const AdaptPlan& plan, const float* low, const void* w, int type_w, bool trans, const hymoe_mat* base,
-                     const hymoe_mat& out, int R, int N, int n_sms, cudaStream_t st) {
+                     const hymoe_mat& out, int R, int N, int T, int n, bool tc, int n_sms, cudaStream_t st) {
     const size_t es = elem_bytes(out.type);
     AdaptWide a{};
     a.plan = plan;
@@ -318,10 +389,18 @@ cudaError_t run_wide(const AdaptPlan& plan, const float* low, const void* w, int
     a.ldo = static_cast<size_t>(out.ld);
     a.N = N;
     a.R = R;
+    a.in_place = base && base->data == out.data;
+    if (tc) {
+        AdaptMaps m;
+        if (!encode_rows(&m, base ? *base : out, T, N, kTcRows) ||
+            !(trans ? encode_weights(&m, w, type_w, n, R, N, adapt_rp(R))
+                    : encode_weights(&m, w, type_w, n, N, R, out.type == HYMOE_TYPE_F32 ? 64 : 128)))
+            return cudaErrorInvalidValue;
+        return launch_adapt_wide_tc(m, a, out.type, type_w, trans, n_sms, st);
+    }
     a.vec_w = rows_vec(w, trans ? N : R, 2);
     a.vec_b = base ? rows_vec(base->data, a.ldb, es) : 0;
     a.vec_o = rows_vec(out.data, a.ldo, es);
-    a.in_place = base && base->data == out.data;
     return launch_adapt_wide(a, out.type, type_w, trans, n_sms, st);
 }
 
@@ -406,14 +485,18 @@ extern "C" hymoe_status hymoe_adapt(const hymoe_adapters* ad, const hymoe_mat* x
             return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt: kernel launch failed");
         return HYMOE_OK;
     }
-    const AdaptLayout l = adapt_layout(ad, T, false);
+    // The tensor cores' kernels need TMA's alignment; mma.sync takes any rows, and fp32 ones of x.
+    const bool aligned = T > kTcRows && weights_tma(ad);
+    const bool tc_low = aligned && x->type == ad->type && rows_tma(x, I);
+    const bool tc_wide = aligned && rows_tma(out, O) && (!base || rows_tma(base, O));
+    const AdaptLayout l = adapt_layout(ad, T, false, tc_low || tc_wide ? kTcRows : kAdRows);
     char* ws = static_cast<char*>(workspace);
     const AdaptPlan plan = plan_in(l, ws, false);
     float* low = reinterpret_cast<float*>(ws + l.low);
     float* low_part = reinterpret_cast<float*>(ws + l.low_part);
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
-    if (e == cudaSuccess) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low, low_part, R, static_cast<int>(I), n_sms, st);
-    if (e == cudaSuccess) e = run_wide(plan, low, ad->b, ad->type, false, base, *out, R, static_cast<int>(O), n_sms, st);
+    if (e == cudaSuccess) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low, low_part, R, static_cast<int>(I), t, n, tc_low, n_sms, st);
+    if (e == cudaSuccess) e = run_wide(plan, low, ad->b, ad->type, false, base, *out, R, static_cast<int>(O), t, n, tc_wide, n_sms, st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt: kernel launch failed");
     return HYMOE_OK;
 }
@@ -470,7 +553,10 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
         return HYMOE_OK;
     }
     const int n_sms = sm_count(dev);
-    const AdaptLayout l = adapt_layout(ad, T, true);
+    const bool aligned = T > kTcRows && weights_tma(ad);
+    const bool tc_x = aligned && x->type == ad->type && rows_tma(x, I), tc_dy = aligned && dy->type == ad->type && rows_tma(dy, O);
+    const bool tc_dx = aligned && dx && rows_tma(dx, I) && (!base || rows_tma(base, I));
+    const AdaptLayout l = adapt_layout(ad, T, true, tc_x || tc_dy || tc_dx ? kTcRows : kAdRows);
     char* ws = static_cast<char*>(workspace);
     const AdaptPlan plan = plan_in(l, ws, true);
     float* low_dy = reinterpret_cast<float*>(ws + l.low);
@@ -479,9 +565,9 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
     float* part = reinterpret_cast<float*>(ws + l.part);
     const int i = static_cast<int>(I), o = static_cast<int>(O);
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
-    if (e == cudaSuccess && (dx || da)) e = run_low(plan, *dy, ad->b, ad->type, true, ad->scale, low_dy, low_part, R, o, n_sms, st);
-    if (e == cudaSuccess && dx) e = run_wide(plan, low_dy, ad->a, ad->type, true, base, *dx, R, i, n_sms, st);
-    if (e == cudaSuccess && db) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low_x, low_part, R, i, n_sms, st);
+    if (e == cudaSuccess && (dx || da)) e = run_low(plan, *dy, ad->b, ad->type, true, ad->scale, low_dy, low_part, R, o, t, n, tc_dy, n_sms, st);
+    if (e == cudaSuccess && dx) e = run_wide(plan, low_dy, ad->a, ad->type, true, base, *dx, R, i, t, n, tc_dx, n_sms, st);
+    if (e == cudaSuccess && db) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low_x, low_part, R, i, t, n, tc_x, n_sms, st);
     if (e == cudaSuccess && da) e = run_grad(plan, low_dy, *x, da, part, t, n, R, i, 1, i, st);
     if (e == cudaSuccess && db) e = run_grad(plan, low_x, *dy, db, part, t, n, R, o, R, 1, st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt_backward: kernel launch failed");

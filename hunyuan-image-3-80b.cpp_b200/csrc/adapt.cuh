@@ -57,10 +57,12 @@ __host__ __device__ constexpr bool adapt_decodes(size_t T, int R) { return T <= 
 // last) and the work lists over that order.
 struct AdaptPlan {
     int* perm;       // [T] token of each sorted row
-    int4* tiles;     // {adapter or -1, first row, rows, 0} of at most kAdRows rows
+    int4* tiles;     // {adapter or -1, first row, rows, 0} of at most tile_rows rows
     int4* items;     // gradients: {adapter, first row, rows, partial slot or -1}; every adapter has one
     int* pieces;     // gradients: [n + 1] first item of each adapter (items are adapter-major)
-    int* n_lists;    // [0] tiles, [1] items
+    int* n_lists;    // [0] status (0, or DevErr bits of a wait that expired), [1] tiles, [2] items,
+                     // [3] tiles that have an adapter (the first ones)
+    int tile_rows;   // 64 or 128
     unsigned* counters;  // [max_tiles] CTAs of a tile that have left their partial sums (0 between launches)
     int max_tiles, max_items;
 };
@@ -120,6 +122,17 @@ cudaError_t launch_adapt_wide(const AdaptWide& a, int type_y, int type_w, bool t
 cudaError_t launch_adapt_grad(const AdaptGrad& a, int type_x, int T, int n, cudaStream_t st);
 
 #ifdef __CUDACC__
+
+// The 64 rows that a CTA of the mma.sync kernels takes: part of a tile; rows 0: none.
+__device__ __forceinline__ int4 ad_part_tile(const AdaptPlan& p, int id) {
+    const int sub = p.tile_rows / kAdRows;
+    if (id / sub >= p.n_lists[1]) return make_int4(-1, 0, 0, 0);
+    int4 t = p.tiles[id / sub];
+    const int off = id % sub * kAdRows;
+    t.y += off;
+    t.z = min(kAdRows, t.z - off);
+    return t.z > 0 ? t : make_int4(-1, 0, 0, 0);
+}
 
 constexpr int ad_pad16(int bytes) { return (bytes / 16 % 2 == 0) ? bytes + 16 : bytes; }  // odd number of pieces
 

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant_
     extern __shared__ __align__(128) char smem[];
     griddep_wait();
     griddep_launch_dependents();
-    if (static_cast<int>(blockIdx.x) >= a.plan.n_lists[1]) return;
+    if (static_cast<int>(blockIdx.x) >= a.plan.n_lists[2]) return;
     const int4 item = a.plan.items[blockIdx.x];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int m0 = blockIdx.y * kAdGradCols;

@@ -34,9 +34,8 @@ __global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void 
     griddep_wait();
     griddep_launch_dependents();
     const int tile_id = blockIdx.x / S, rank = blockIdx.x % S;
-    if (tile_id >= a.plan.n_lists[0]) return;
-    const int4 tile = a.plan.tiles[tile_id];
-    if (tile.x < 0) return;  // rows without an adapter
+    const int4 tile = ad_part_tile(a.plan, tile_id);
+    if (tile.x < 0) return;  // none, or rows without an adapter
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nk = (a.K + kLowK - 1) / kLowK;
     const int k_lo = static_cast<int>(static_cast<int64_t>(nk) * rank / S);
@@ -214,8 +213,9 @@ cudaError_t launch_t(const AdaptLow& a, int n_sms, cudaStream_t st) {
     auto kern = low_kernel<X, W, RP, TRANS>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
-    const int S = adapt_splits(a.plan.max_tiles, a.K, L::kPerSm * n_sms);
-    return launch_kernel(true, kern, dim3(static_cast<unsigned>(a.plan.max_tiles) * S), dim3(kAdThreads), L::kSmem, st, a, S);
+    const int tiles = a.plan.max_tiles * (a.plan.tile_rows / kAdRows);
+    const int S = adapt_splits(tiles, a.K, L::kPerSm * n_sms);
+    return launch_kernel(true, kern, dim3(static_cast<unsigned>(tiles) * S), dim3(kAdThreads), L::kSmem, st, a, S);
 }
 
 template <typename X, typename W>

@@ -1,0 +1,236 @@
+// adapt_low_tc.cu — the adapters' narrow product on the 5th-generation tensor cores, for rows of the
+// weights' 16-bit type on 16-byte boundaries: low[row] = scale[a] * W_a x[token of row].
+//
+// A tile of 128 sorted rows of one adapter is a cluster of S CTAs (1, 2, 4 or 8), each over a part
+// of the long dimension.  64 columns of the rows and of the weights make a stage: one thread brings
+// the weights in by TMA, and the rows too where their tokens are consecutive; rows in any order are
+// copied by the four later epilogue warps, eight lanes to a row (gather4 loads of four rows were
+// tried: they top out at 2.5 TB/s).  One thread issues the products (M = 128 rows, N = RP) into
+// tensor memory.  The parts are added in distributed shared memory, every CTA taking its share of
+// the rows, in the order of the parts.  Bound by reading x.
+#include "adapt_tc.cuh"
+
+namespace hymoe {
+namespace {
+
+constexpr int kLtcRows = kTcRows;
+constexpr int kLtcThreads = 192;  // TMA, MMA, four copying and epilogue warps
+
+// N: columns of the product; an MN-major weight tile has whole blocks of 64.
+template <int RP, bool TRANS>
+struct LtcTile {
+    static constexpr int kN = TRANS && RP < 64 ? 64 : RP;
+    static constexpr int kA = kLtcRows * 128, kB = kN * 128;
+    static constexpr int kStages = kN == 128 ? 3 : 4;
+    static constexpr int kSmem = 1024 + kStages * (kA + kB);
+    static_assert(kStages * (kA + kB) >= kLtcRows * (RP + 4) * 4, "the stages hold the partial sums");
+    static constexpr int kCols = kN < 32 ? 32 : kN;
+};
+
+template <typename W, int RP, bool TRANS>
+__global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_constant__ AdaptMaps maps,
+                                                                const __grid_constant__ AdaptLow a, int S) {
+    using L = LtcTile<RP, TRANS>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    __shared__ uint64_t full[L::kStages], empty[L::kStages], done;
+    __shared__ uint32_t tmem_s;
+    __shared__ int tok[kLtcRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    griddep_wait();
+    griddep_launch_dependents();
+    const int tile_id = blockIdx.x / S, rank = blockIdx.x % S;
+    int4 tile = make_int4(-1, 0, 0, 0);
+    if (tile_id < a.plan.n_lists[1]) tile = a.plan.tiles[tile_id];
+    if (tile.x < 0) return;  // the whole cluster: no such tile, or rows without an adapter
+    int first;
+    const bool run = tile_run(a.plan, tile, &first);
+    if (tid < kLtcRows) tok[tid] = __ldg(a.plan.perm + tile.y + min(tid, tile.z - 1));
+    if (tid == 0) {
+        for (int s = 0; s < L::kStages; ++s) {
+            mbar_init(&full[s], run ? 1 : 129);  // TMA, and the copying threads
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&done, 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&tmem_s, L::kCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_s;
+    const int nk = (a.K + 63) / 64;
+    const int k_lo = static_cast<int>(static_cast<int64_t>(nk) * rank / S);
+    const int k_hi = static_cast<int>(static_cast<int64_t>(nk) * (rank + 1) / S);
+    int* err = a.plan.n_lists;  // the status word
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
+                const int s = it % L::kStages;
+                if (!mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER)) break;
+                uint8_t* sa = smem + s * (L::kA + L::kB);
+                mbar_arrive_expect_tx(&full[s], L::kB + (run ? L::kA : 0));
+                if (run) tma_load_2d(sa, &maps.rows, &full[s], kb * 64, first);
+                if (TRANS) {
+                    // weights [K][R]: 64 K rows, in blocks of 64 along the rank
+#pragma unroll
+                    for (int n = 0; n < L::kN / 64; ++n)
+                        tma_load_3d(sa + L::kA + n * 8192, &maps.w, &full[s], n * 64, kb * 64, tile.x);
+                } else {
+                    tma_load_3d(sa + L::kA, &maps.w, &full[s], kb * 64, 0, tile.x);
+                }
+            }
+            // (a stage whose rows are copied completes only if the copying warps went on as well)
+            for (int j = it > L::kStages ? it - L::kStages : 0; j < it; ++j) mbar_drain(&full[j % L::kStages], (j / L::kStages) & 1);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = ad_idesc<W>(L::kN, false, TRANS);
+            int it = 0;
+            for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
+                const int s = it % L::kStages;
+                if (!mbar_wait(&full[s], (it / L::kStages) & 1, err, DEVERR_TIMEOUT_MMA)) break;
+                if (!run) fence_proxy_async_smem();  // the copied rows, before the tensor core reads them
+                tc_fence_after();
+                const uint32_t sa = smem_u32(smem + s * (L::kA + L::kB)), sb = sa + L::kA;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    mma_f16_ss(tmem, sw128_kmajor_desc(sa + kk * 32),
+                               TRANS ? sw128_mnmajor_desc(sb + kk * 2048, 8192) : sw128_kmajor_desc(sb + kk * 32), idesc,
+                               (it | kk) != 0 ? 1u : 0u);
+                mma_commit(&empty[s]);
+            }
+            mma_commit(&done);
+            mbar_drain(&done, 0);  // every product has ended before tensor memory is freed
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3, et = tid - 64;
+        if (!run) {
+            // this thread's piece of rows et / 8 + 16 i
+            const int piece = et & 7;
+            const char* src[8];
+            uint32_t dst[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = (et >> 3) + 16 * i;
+                src[i] = static_cast<const char*>(a.x) + (static_cast<size_t>(tok[r]) * a.ldx + piece * 8) * 2;
+                dst[i] = sw128_offset(r, piece);
+            }
+            int it = 0;
+            for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
+                const int s = it % L::kStages;
+                if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER))) break;
+                uint8_t* sa = smem + s * (L::kA + L::kB);
+                const int left = a.K - kb * 64 - piece * 8;
+                const int bytes = left >= 8 ? 16 : 0;  // K is a multiple of 8
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    cp_async16_part(sa + dst[i], bytes ? src[i] + static_cast<size_t>(kb) * 128 : static_cast<const char*>(a.x), bytes);
+                cp_async_arrive(&full[s]);
+            }
+            cp_async_wait_all();
+        }
+        // on an expired wait the status word says that the results are not valid
+        mbar_wait(&done, 0, err, DEVERR_TIMEOUT_EPILOGUE);
+        tc_fence_after();
+        const int r = q * 32 + lane;
+        const float f = a.scale != nullptr ? __ldg(a.scale + tile.x) : 1.f;
+        // the sums through shared memory (the stages are free): rows padded by four floats
+        float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int c = 0; c < RP; c += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < (RP < 32 ? RP : 32); j += 4)
+                *reinterpret_cast<uint4*>(red + r * (RP + 4) + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        }
+        tc_fence_before();
+        if (S == 1) {
+            named_bar_sync(1, 128);
+        } else {
+            cluster_arrive();
+            cluster_wait();
+        }
+        const int rows = kLtcRows / S;
+        for (int p = et; p < rows * (RP / 4); p += 128) {
+            const int row = rank * rows + p / (RP / 4), c = p % (RP / 4) * 4;
+            if (row >= tile.z) break;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < S; ++i) {
+                const float4 v = ld_cluster4(mapa_shared(red + row * (RP + 4) + c, i));
+                s.x += v.x;
+                s.y += v.y;
+                s.z += v.z;
+                s.w += v.w;
+            }
+            *reinterpret_cast<float4*>(a.low + static_cast<size_t>(tile.y + row) * RP + c) =
+                make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+        }
+    }
+    if (S > 1) {  // every thread arrives once before the sums are read and once after
+        if (warp < 2) {
+            cluster_arrive();
+            cluster_wait();
+        }
+        cluster_arrive();
+        cluster_wait();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, L::kCols);
+    }
+}
+
+template <typename W, int RP, bool TRANS>
+cudaError_t launch_t(const AdaptMaps& maps, const AdaptLow& a, int n_sms, cudaStream_t st) {
+    using L = LtcTile<RP, TRANS>;
+    auto kern = low_tc_kernel<W, RP, TRANS>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    if (e != cudaSuccess) return e;
+    // as many CTAs as two to an SM allow, each with two stages of columns at least
+    const int nk = (a.K + 63) / 64;
+    int S = 1;
+    while (S < 8 && a.plan.max_tiles * 2 * S <= 2 * n_sms && nk >= 4 * S) S *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.plan.max_tiles) * S);
+    cfg.blockDim = dim3(kLtcThreads);
+    cfg.dynamicSmemBytes = L::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, maps, a, S);
+}
+
+template <typename W>
+cudaError_t launch_w(const AdaptMaps& maps, const AdaptLow& a, bool trans, int n_sms, cudaStream_t st) {
+    switch (adapt_rp(a.R)) {
+        case 16: return trans ? launch_t<W, 16, true>(maps, a, n_sms, st) : launch_t<W, 16, false>(maps, a, n_sms, st);
+        case 32: return trans ? launch_t<W, 32, true>(maps, a, n_sms, st) : launch_t<W, 32, false>(maps, a, n_sms, st);
+        case 64: return trans ? launch_t<W, 64, true>(maps, a, n_sms, st) : launch_t<W, 64, false>(maps, a, n_sms, st);
+        default: return trans ? launch_t<W, 128, true>(maps, a, n_sms, st) : launch_t<W, 128, false>(maps, a, n_sms, st);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_adapt_low_tc(const AdaptMaps& maps, const AdaptLow& a, int type_w, bool trans, int n_sms, cudaStream_t st) {
+    return type_w == HYMOE_TYPE_F16 ? launch_w<__half>(maps, a, trans, n_sms, st) : launch_w<__nv_bfloat16>(maps, a, trans, n_sms, st);
+}
+
+}  // namespace hymoe

@@ -49,8 +49,8 @@ __global__ __launch_bounds__(kAdThreads, WideTile<Y, RP, TRANS>::kPerSm) void wi
     extern __shared__ __align__(128) char smem[];
     griddep_wait();
     griddep_launch_dependents();
-    if (static_cast<int>(blockIdx.x) >= a.plan.n_lists[0]) return;
-    const int4 tile = a.plan.tiles[blockIdx.x];
+    const int4 tile = ad_part_tile(a.plan, blockIdx.x);
+    if (tile.z == 0) return;
     const bool mul = tile.x >= 0;
     if (!mul && a.in_place) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -268,10 +268,11 @@ cudaError_t launch_t(const AdaptWide& a, int n_sms, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
     // runs of columns: as many as fill the GPU once
-    const int blks = (a.N + kWideCols - 1) / kWideCols, fit = L::kPerSm * n_sms / a.plan.max_tiles;
+    const int blks = (a.N + kWideCols - 1) / kWideCols, tiles = a.plan.max_tiles * (a.plan.tile_rows / kAdRows);
+    const int fit = L::kPerSm * n_sms / tiles;
     const int parts = fit < 1 ? 1 : fit < blks ? fit : blks;
     const int cols = (blks + parts - 1) / parts * kWideCols;
-    return launch_kernel(true, kern, dim3(a.plan.max_tiles, (a.N + cols - 1) / cols), dim3(kAdThreads), L::kSmem, st, a, cols);
+    return launch_kernel(true, kern, dim3(tiles, (a.N + cols - 1) / cols), dim3(kAdThreads), L::kSmem, st, a, cols);
 }
 
 template <typename Y, typename W>

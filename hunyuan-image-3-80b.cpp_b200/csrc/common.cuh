@@ -67,6 +67,8 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Programmatic dependent launch.  A kernel launched with the programmatic-serialisation
 // attribute (launch_kernel(pdl = true)) may be scheduled while its predecessor in the stream is
 // still running: griddep_wait blocks until that predecessor has completed and its writes are
