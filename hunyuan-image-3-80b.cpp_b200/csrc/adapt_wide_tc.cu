@@ -43,6 +43,22 @@ struct WtcTile {
     static_assert(kStages >= 2, "a ring");
 };
 
+// Bounded wait of a whole warp until a counter in shared memory reaches n.
+__device__ __forceinline__ bool count_wait(const uint32_t* count, int n, int* err) {
+    int ok = 1;
+    if (n > 0 && (threadIdx.x & 31) == 0) {
+        const uint64_t t0 = globaltimer_ns();
+        while (ok && static_cast<int>(ld_acquire_cta_u32(count)) < n) {
+            __nanosleep(40);
+            if (globaltimer_ns() - t0 > kWaitBudgetNs || *(volatile int*)err != 0) {
+                atomicOr(err, DEVERR_TIMEOUT_PRODUCER);
+                ok = 0;
+            }
+        }
+    }
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
 template <typename Y, typename W, int RP, bool TRANS>
 __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_constant__ AdaptMaps maps,
                                                                  const __grid_constant__ AdaptWide a) {
@@ -51,7 +67,7 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
     uint8_t* sA = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* ring = sA + L::kA;
     __shared__ uint64_t full[L::kStages], copied[L::kStages], empty[L::kStages], acc_full[kWtcAccs], acc_empty[kWtcAccs], a_full, mma_end;
-    __shared__ uint32_t tmem_s;
+    __shared__ uint32_t tmem_s, armed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < L::kStages; ++s) {
@@ -65,6 +81,7 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
         }
         mbar_init(&a_full, 8);
         mbar_init(&mma_end, 1);
+        armed = 0u;
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -107,6 +124,7 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
                 const int s = it % L::kStages;
                 uint8_t* sb = ring + s * L::kStage;
                 if (!mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER)) break;
+                red_release_cta_add(&armed, 1u);
                 mbar_arrive_expect_tx(&full[s], (tile.x >= 0 ? L::kW : 0) + (run ? kWtcBase : 0));
                 if (tile.x >= 0) {
                     uint8_t* sw = sb + kWtcBase;
@@ -134,7 +152,7 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
         constexpr int kPer = 16 / static_cast<int>(sizeof(Y));
         const int ct = tid - 320, piece = ct & 15, row0 = ct >> 4;  // rows row0 + 8 i of the tile
         const char* src[16];
-        int it = 0, at = -1;
+        int it = 0, at = -1, n_copied = 0;
         bool copy = false;
         for (int ti = ti0, blk = blk0; it < n_units; ++it, ++blk) {
             if (blk == n_blk) {
@@ -154,21 +172,20 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
                                  (static_cast<size_t>(__ldg(a.plan.perm + tile.y + min(row0 + 8 * i, tile.z - 1))) * a.ldb + piece * kPer) * sizeof(Y);
                 }
             }
-            // These warps take part in every unit, copied or not: a parity wait tells phases apart only
-            // for a warp that the ring cannot leave behind.
+            if (!copy) continue;
+            // Units between copied ones pass without these warps, so they follow the producer's count of
+            // slots that it found free (a barrier's parity tells phases apart only for a warp that
+            // takes part in each).  The barriers `copied` are taken in turn.
             const int s = it % L::kStages;
-            if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER))) break;
-            if (!copy) {
-                mbar_arrive(&copied[s]);
-                continue;
-            }
+            if (!count_wait(&armed, it + 1, err)) break;
             uint8_t* dst = ring + s * L::kStage + piece / 8 * kWtcPanel;
             const int bytes = c0 + piece * kPer < a.N ? 16 : 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 cp_async16_part(dst + sw128_offset(row0 + 8 * i, piece % 8),
                                 bytes ? src[i] + static_cast<size_t>(c0) * sizeof(Y) : static_cast<const char*>(a.base), bytes);
-            cp_async_arrive(&copied[s]);
+            cp_async_arrive(&copied[n_copied % L::kStages]);
+            ++n_copied;
         }
         cp_async_wait_all();
     } else if (warp == 1) {
@@ -224,8 +241,9 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
     } else {
         // ------------------------------------------------------------ epilogue
         const int q = warp & 3, half = (warp - 2) >> 2, r = q * 32 + lane;
-        int it = 0, at = -1, accs = 0;
+        int it = 0, at = -1, accs = 0, n_copied = 0;
         int4 tile = make_int4(-1, 0, 0, 0);
+        bool copy = false;
         char* op[8];       // rows 4 i + lane / 8 of the quarter, at this lane's piece; nullptr: no such row
         float back = 1.f;
         constexpr int kPer = 16 / static_cast<int>(sizeof(Y));  // values of a piece
@@ -243,6 +261,8 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
                 // the previous tile's products have ended: their sums were waited for
                 at = ti;
                 tile = a.plan.tiles[ti];
+                int first;
+                copy = a.base != nullptr && !tile_run(a.plan, tile, &first);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int row = q * 32 + 4 * i + (lane >> 3);
@@ -294,46 +314,49 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
             uint8_t* sb = ring + s * L::kStage;
             const int b = accs % kWtcAccs;
             if (mul) ok = mbar_wait(&acc_full[b], (accs / kWtcAccs) & 1, err, DEVERR_TIMEOUT_EPILOGUE);
-            // the base rows, however they came
-            ok = ok && mbar_wait(&full[s], (it / L::kStages) & 1, err, DEVERR_TIMEOUT_EPILOGUE) &&
-                 mbar_wait(&copied[s], (it / L::kStages) & 1, err, DEVERR_TIMEOUT_EPILOGUE);
+            // the base rows, however they came (`full` in any case: see the copying warps)
+            ok = ok && mbar_wait(&full[s], (it / L::kStages) & 1, err, DEVERR_TIMEOUT_EPILOGUE);
+            if (ok && copy) ok = mbar_wait(&copied[n_copied % L::kStages], (n_copied / L::kStages) & 1, err, DEVERR_TIMEOUT_EPILOGUE);
             ok = __all_sync(0xffffffffu, ok);
+            n_copied += copy;
             if (!ok) break;
             if (mul || a.base == nullptr) {
                 tc_fence_after();
                 uint8_t* panel = sb + half * kWtcPanel + r * 128;
                 const uint32_t flip = static_cast<uint32_t>(r & 7) << 4;
+                uint4 o[8];  // the row's 128 bytes of this panel, all loaded before any is stored
 #pragma unroll
-                for (int h = 0; h < kHalf; h += 32) {
-                    uint32_t v[32];
-                    if (mul) {
-                        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 128 + half * kHalf + h, v);
+                for (int j = 0; j < 8; ++j)
+                    o[j] = a.base != nullptr ? *reinterpret_cast<const uint4*>(panel + ((static_cast<uint32_t>(j) << 4) ^ flip))
+                                             : make_uint4(0u, 0u, 0u, 0u);
+                if (mul) {
+                    constexpr int kPieces = 32 / kPer;  // pieces of 32 columns
+#pragma unroll
+                    for (int h = 0; h < kHalf / 32; ++h) {
+                        uint32_t v[32];
+                        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 128 + half * kHalf + h * 32, v);
                         tmem_ld_wait();
-                    } else {
+                        if (AdType<W>::kScaled) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0u;
-                    }
-                    if (AdType<W>::kScaled) {
+                            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * back);
+                        }
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * back);
-                    }
+                        for (int j = 0; j < kPieces; ++j) {
+                            uint32_t* ow = reinterpret_cast<uint32_t*>(&o[h * kPieces + j]);
 #pragma unroll
-                    for (int j = 0; j < 32 / kPer; ++j) {
-                        uint4* at16 = reinterpret_cast<uint4*>(panel + ((static_cast<uint32_t>(h / kPer + j) << 4) ^ flip));
-                        uint4 o = a.base != nullptr ? *at16 : make_uint4(0u, 0u, 0u, 0u);
-                        uint32_t* ow = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if constexpr (L::kF32) {
-                                ow[i] = __float_as_uint(__uint_as_float(ow[i]) + __uint_as_float(v[4 * j + i]));
-                            } else {
-                                const float2 f2 = AdType<W>::unpack(ow[i]);
-                                ow[i] = AdType<W>::pack(f2.x + __uint_as_float(v[8 * j + 2 * i]), f2.y + __uint_as_float(v[8 * j + 2 * i + 1]));
+                            for (int i = 0; i < 4; ++i) {
+                                if constexpr (L::kF32) {
+                                    ow[i] = __float_as_uint(__uint_as_float(ow[i]) + __uint_as_float(v[4 * j + i]));
+                                } else {
+                                    const float2 f2 = AdType<W>::unpack(ow[i]);
+                                    ow[i] = AdType<W>::pack(f2.x + __uint_as_float(v[8 * j + 2 * i]), f2.y + __uint_as_float(v[8 * j + 2 * i + 1]));
+                                }
                             }
                         }
-                        *at16 = o;
                     }
                 }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(panel + ((static_cast<uint32_t>(j) << 4) ^ flip)) = o[j];
                 if (mul) {
                     tc_fence_before();
                     __syncwarp();
@@ -343,13 +366,17 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
                 __syncwarp();
             }
             // the warp's 32 rows of 128 bytes, four rows per store
-            if (c0 + col_off < a.N) {
+            {
                 const uint8_t* from = sb + half * kWtcPanel + (q * 32 + (lane >> 3)) * 128;
+                uint4 o[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (op[i] != nullptr)
-                        *reinterpret_cast<uint4*>(op[i] + static_cast<size_t>(c0) * sizeof(Y)) = *reinterpret_cast<const uint4*>(
-                            from + i * 512 + (((lane & 7) ^ ((4 * i + (lane >> 3)) & 7)) << 4));
+                    o[i] = *reinterpret_cast<const uint4*>(from + i * 512 + (((lane & 7) ^ ((4 * i + (lane >> 3)) & 7)) << 4));
+                if (c0 + col_off < a.N) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (op[i] != nullptr) *reinterpret_cast<uint4*>(op[i] + static_cast<size_t>(c0) * sizeof(Y)) = o[i];
+                }
             }
             fence_proxy_async_smem();  // the slot was written here and is TMA's next
             __syncwarp();
