@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
     const int64_t lo64 = static_cast<int64_t>(warp) * per;
     const int t_lo = lo64 < T ? static_cast<int>(lo64) : T, t_hi = warp < W ? min(T, t_lo + per) : t_lo;
     const int bits = 32 - __clz(n);
-    int b[8];
+    int b[8], rank[8], peers[8];  // adapter, place among the step's tokens of that adapter, their number
     auto fetch = [&](int t0) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -97,13 +97,18 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
     for (int i = tid; i < p.max_tiles * (p.tile_rows / kAdRows); i += kPlanThreads) p.counters[i] = 0u;
     __syncthreads();
     int* mine = cnt + (warp < W ? warp : 0) * nb;
+    auto rate = [&](int i) {
+        const unsigned same = equals(b[i]);
+        rank[i] = __popc(same & ((1u << lane) - 1u));
+        peers[i] = __popc(same);
+    };
     for (int t0 = t_lo; t0 < t_hi; t0 += 256) {
         if (t0 > t_lo) fetch(t0);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (t0 + 32 * i >= t_hi) break;
-            const unsigned same = equals(b[i]);
-            if (b[i] >= 0 && (same & ((1u << lane) - 1u)) == 0) mine[b[i]] += __popc(same);
+            rate(i);
+            if (b[i] >= 0 && rank[i] == 0) mine[b[i]] += peers[i];
             __syncwarp();
         }
     }
@@ -132,19 +137,18 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
     if (warp == 2) warp_scan(ipre, n);
     if (warp == 3) warp_scan(spre, n);
     __syncthreads();
-    if (t_hi - t_lo > 256) fetch(t_lo);
+    const bool again = t_hi - t_lo > 256;  // more tokens than the registers held
     for (int t0 = t_lo; t0 < t_hi; t0 += 256) {
-        if (t0 > t_lo) fetch(t0);
+        if (again) fetch(t0);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (t0 + 32 * i >= t_hi) break;
-            const unsigned same = equals(b[i]);
-            const int before = __popc(same & ((1u << lane) - 1u));
+            if (again) rate(i);
             const int at = b[i] >= 0 ? mine[b[i]] : 0;
             __syncwarp();
             if (b[i] >= 0) {
-                p.perm[off[b[i]] + at + before] = t0 + 32 * i + lane;
-                if (before == 0) mine[b[i]] = at + __popc(same);
+                p.perm[off[b[i]] + at + rank[i]] = t0 + 32 * i + lane;
+                if (rank[i] == 0) mine[b[i]] = at + peers[i];
             }
             __syncwarp();
         }
@@ -182,7 +186,7 @@ cudaError_t launch_plan_adapt(const int* ids, int T, int n, const AdaptPlan& p, 
 // The workspace: every part starts on 256 bytes.
 struct AdaptLayout {
     size_t perm, tiles, items, pieces, lists, counters, low, low2, low_part, part, bytes;
-    int tile_rows, max_tiles, max_items;
+    int tile_rows, max_tiles, spare_tiles, max_items;
 };
 // (the sizes do not depend on tile_rows)
 AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward, int tile_rows = kAdRows) {
@@ -199,6 +203,7 @@ AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward, int 
     const size_t tiles64 = T / kAdRows + buckets, half_tiles = tiles64 + buckets;  // also twice the tiles of 128
     l.tile_rows = tile_rows;
     l.max_tiles = static_cast<int>(T / tile_rows + buckets);
+    l.spare_tiles = static_cast<int>(buckets);
     l.max_items = static_cast<int>(n + long_pieces);
     l.lists = take(4 * sizeof(int));
     l.perm = take(T * sizeof(int));
@@ -226,6 +231,7 @@ AdaptPlan plan_in(const AdaptLayout& l, char* ws, bool backward) {
     p.counters = reinterpret_cast<unsigned*>(ws + l.counters);
     p.tile_rows = l.tile_rows;
     p.max_tiles = l.max_tiles;
+    p.spare_tiles = l.spare_tiles;
     p.max_items = l.max_items;
     return p;
 }

@@ -65,6 +65,7 @@ struct AdaptPlan {
     int tile_rows;   // 64 or 128
     unsigned* counters;  // [max_tiles] CTAs of a tile that have left their partial sums (0 between launches)
     int max_tiles, max_items;
+    int spare_tiles; // of max_tiles, those for adapters' last, part-filled tiles
 };
 
 struct AdaptLow {      // low[row, j] = scale[a] * sum_k X[perm[row], k] W_a(j, k), rows in sorted order

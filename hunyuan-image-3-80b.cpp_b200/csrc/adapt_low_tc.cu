@@ -197,10 +197,11 @@ cudaError_t launch_t(const AdaptMaps& maps, const AdaptLow& a, int n_sms, cudaSt
     auto kern = low_tc_kernel<W, RP, TRANS>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
-    // as many CTAs as two to an SM allow, each with two stages of columns at least
-    const int nk = (a.K + 63) / 64;
+    // as many CTAs as two to an SM allow (for the tiles that are likely: half of the adapters' last
+    // ones are short of the bound), each with two stages of columns at least
+    const int nk = (a.K + 63) / 64, tiles = a.plan.max_tiles - a.plan.spare_tiles / 2;
     int S = 1;
-    while (S < 8 && a.plan.max_tiles * 2 * S <= 2 * n_sms && nk >= 4 * S) S *= 2;
+    while (S < 8 && tiles * 2 * S <= 2 * n_sms && nk >= 4 * S) S *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(a.plan.max_tiles) * S);
     cfg.blockDim = dim3(kLtcThreads);

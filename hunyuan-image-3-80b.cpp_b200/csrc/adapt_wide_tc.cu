@@ -92,7 +92,10 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_s;
-    griddep_wait();
+    // The plan was complete before the narrow product began (which let this grid be scheduled), and
+    // whatever wrote the base and the weights before the plan began: their loads need not wait for the
+    // narrow product, only its readers do.
+    if (warp >= 2 && warp < 10) griddep_wait();
     griddep_launch_dependents();
     int* err = a.plan.n_lists;
     const int n_blk = (a.N + L::kCols - 1) / L::kCols;
