@@ -166,6 +166,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
             p.items[i] = make_int4(a, off[a] + r, min(chunk, tot[a] - r), several ? spre[a] + q : -1);
         }
         for (int a = tid; a <= n; a += kPlanThreads) p.pieces[a] = ipre[a];
+        for (int a = tid; a < 2 * n; a += kPlanThreads) p.amax[a] = 0u;
         if (tid == 0) p.n_lists[2] = n_items;
     }
     if (tid == 0) {
@@ -185,7 +186,7 @@ cudaError_t launch_plan_adapt(const int* ids, int T, int n, const AdaptPlan& p, 
 
 // The workspace: every part starts on 256 bytes.
 struct AdaptLayout {
-    size_t perm, tiles, items, pieces, lists, counters, low, low2, low_part, part, bytes;
+    size_t perm, tiles, items, pieces, amax, lists, counters, low, low2, low_part, part, slots, bytes;
     int tile_rows, max_tiles, spare_tiles, max_items;
 };
 // (the sizes do not depend on tile_rows)
@@ -215,9 +216,10 @@ AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward, int 
     if (backward) {
         l.items = take(static_cast<size_t>(l.max_items) * sizeof(int4));
         l.pieces = take((n + 1) * sizeof(int));
+        l.amax = take(2 * n * sizeof(unsigned));
         l.low2 = take(T * adapt_rp(ad->rank) * sizeof(float));
-        // an adapter of c tokens in p > 1 pieces: p < 2 c / chunk
-        l.part = take(2 * long_pieces * ad->rank * (static_cast<size_t>(ad->in_features) + ad->out_features) * sizeof(float));
+        l.slots = 2 * long_pieces;  // an adapter of c tokens in p > 1 pieces: p < 2 c / chunk
+        l.part = take(l.slots * ad->rank * (static_cast<size_t>(ad->in_features) + ad->out_features) * sizeof(float));
     }
     return l;
 }
@@ -227,6 +229,7 @@ AdaptPlan plan_in(const AdaptLayout& l, char* ws, bool backward) {
     p.tiles = reinterpret_cast<int4*>(ws + l.tiles);
     p.items = backward ? reinterpret_cast<int4*>(ws + l.items) : nullptr;
     p.pieces = backward ? reinterpret_cast<int*>(ws + l.pieces) : nullptr;
+    p.amax = backward ? reinterpret_cast<unsigned*>(ws + l.amax) : nullptr;
     p.n_lists = reinterpret_cast<int*>(ws + l.lists);
     p.counters = reinterpret_cast<unsigned*>(ws + l.counters);
     p.tile_rows = l.tile_rows;
@@ -331,12 +334,12 @@ bool encode(CUtensorMap* m, int type, int rank, const void* base, const cuuint64
 }
 
 // Token rows [T, cols], boxes of 128 bytes of `rows` rows.
-bool encode_rows(AdaptMaps* m, const hymoe_mat& x, int T, int cols, int rows) {
+bool encode_rows(CUtensorMap* m, const hymoe_mat& x, int T, int cols, int rows) {
     const size_t es = elem_bytes(x.type);
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(T)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(T > 1 ? x.ld : cols) * es};
     const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(rows)};
-    return encode(&m->rows, x.type, 2, x.data, dims, strides, box);
+    return encode(m, x.type, 2, x.data, dims, strides, box);
 }
 
 // Weights [n][rows][cols], boxes of 64 columns and `box_rows` rows of one adapter.
@@ -359,7 +362,7 @@ bool weights_tma(const hymoe_adapters* ad) {
 }
 
 cudaError_t run_low(const AdaptPlan& plan, const hymoe_mat& x, const void* w, int type_w, bool trans, const float* scale,
-                    float* low, float* part, int R, int K, int T, int n, bool tc, int n_sms, cudaStream_t st) {
+                    float* low, float* part, unsigned* amax, int R, int K, int T, int n, bool tc, int n_sms, cudaStream_t st) {
     AdaptLow a{};
     a.plan = plan;
     a.x = x.data;
@@ -368,11 +371,12 @@ cudaError_t run_low(const AdaptPlan& plan, const hymoe_mat& x, const void* w, in
     a.scale = scale;
     a.low = low;
     a.part = part;
+    a.amax = amax;
     a.K = K;
     a.R = R;
     if (tc) {
         AdaptMaps m;
-        if (!encode_rows(&m, x, T, K, kTcRows) ||
+        if (!encode_rows(&m.rows, x, T, K, kTcRows) ||
             !(trans ? encode_weights(&m, w, type_w, n, K, R, 64) : encode_weights(&m, w, type_w, n, R, K, adapt_rp(R))))
             return cudaErrorInvalidValue;
         return launch_adapt_low_tc(m, a, type_w, trans, n_sms, st);
@@ -398,7 +402,7 @@ cudaError_t run_wide(const AdaptPlan& plan, const float* low, const void* w, int
     a.in_place = base && base->data == out.data;
     if (tc) {
         AdaptMaps m;
-        if (!encode_rows(&m, base ? *base : out, T, N, kTcRows) ||
+        if (!encode_rows(&m.rows, base ? *base : out, T, N, kTcRows) ||
             !(trans ? encode_weights(&m, w, type_w, n, R, N, adapt_rp(R))
                     : encode_weights(&m, w, type_w, n, N, R, out.type == HYMOE_TYPE_F32 ? 64 : 128)))
             return cudaErrorInvalidValue;
@@ -410,8 +414,8 @@ cudaError_t run_wide(const AdaptPlan& plan, const float* low, const void* w, int
     return launch_adapt_wide(a, out.type, type_w, trans, n_sms, st);
 }
 
-cudaError_t run_grad(const AdaptPlan& plan, const float* low, const hymoe_mat& x, float* g, float* part, int T, int n,
-                     int R, int M, int gm, int gj, cudaStream_t st) {
+AdaptGrad grad_args(const AdaptPlan& plan, const float* low, const hymoe_mat& x, float* g, float* part, int n, int R, int M,
+                    int gm, int gj) {
     AdaptGrad a{};
     a.plan = plan;
     a.low = low;
@@ -423,8 +427,9 @@ cudaError_t run_grad(const AdaptPlan& plan, const float* low, const hymoe_mat& x
     a.R = R;
     a.gm = gm;
     a.gj = gj;
+    a.n = n;
     a.vec_x = rows_vec(x.data, a.ldx, elem_bytes(x.type));
-    return launch_adapt_grad(a, x.type, T, n, st);
+    return a;
 }
 
 bool all_on(int dev, std::initializer_list<const void*> ps) {
@@ -501,7 +506,7 @@ extern "C" hymoe_status hymoe_adapt(const hymoe_adapters* ad, const hymoe_mat* x
     float* low = reinterpret_cast<float*>(ws + l.low);
     float* low_part = reinterpret_cast<float*>(ws + l.low_part);
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
-    if (e == cudaSuccess) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low, low_part, R, static_cast<int>(I), t, n, tc_low, n_sms, st);
+    if (e == cudaSuccess) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low, low_part, nullptr, R, static_cast<int>(I), t, n, tc_low, n_sms, st);
     if (e == cudaSuccess) e = run_wide(plan, low, ad->b, ad->type, false, base, *out, R, static_cast<int>(O), t, n, tc_wide, n_sms, st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt: kernel launch failed");
     return HYMOE_OK;
@@ -561,6 +566,7 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
     const int n_sms = sm_count(dev);
     const bool aligned = T > kTcRows && weights_tma(ad);
     const bool tc_x = aligned && x->type == ad->type && rows_tma(x, I), tc_dy = aligned && dy->type == ad->type && rows_tma(dy, O);
+    const bool tc_grad = (!da || tc_x) && (!db || (tc_dy && entry_aligned(db, 16)));
     const bool tc_dx = aligned && dx && rows_tma(dx, I) && (!base || rows_tma(base, I));
     const AdaptLayout l = adapt_layout(ad, T, true, tc_x || tc_dy || tc_dx ? kTcRows : kAdRows);
     char* ws = static_cast<char*>(workspace);
@@ -570,12 +576,24 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
     float* low_part = reinterpret_cast<float*>(ws + l.low_part);
     float* part = reinterpret_cast<float*>(ws + l.part);
     const int i = static_cast<int>(I), o = static_cast<int>(O);
+    unsigned* amax = tc_grad && ad->type == HYMOE_TYPE_F16 ? plan.amax : nullptr;
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
-    if (e == cudaSuccess && (dx || da)) e = run_low(plan, *dy, ad->b, ad->type, true, ad->scale, low_dy, low_part, R, o, t, n, tc_dy, n_sms, st);
+    if (e == cudaSuccess && (dx || da)) e = run_low(plan, *dy, ad->b, ad->type, true, ad->scale, low_dy, low_part, amax, R, o, t, n, tc_dy, n_sms, st);
     if (e == cudaSuccess && dx) e = run_wide(plan, low_dy, ad->a, ad->type, true, base, *dx, R, i, t, n, tc_dx, n_sms, st);
-    if (e == cudaSuccess && db) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low_x, low_part, R, i, t, n, tc_x, n_sms, st);
-    if (e == cudaSuccess && da) e = run_grad(plan, low_dy, *x, da, part, t, n, R, i, 1, i, st);
-    if (e == cudaSuccess && db) e = run_grad(plan, low_x, *dy, db, part, t, n, R, o, R, 1, st);
+    if (e == cudaSuccess && db) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low_x, low_part, amax ? amax + n : nullptr, R, i, t, n, tc_x, n_sms, st);
+    // dA from x and dy's narrow rows, dB from dy and x's; long adapters in pieces
+    AdaptGradPair grads;
+    grads.g[0] = grad_args(plan, low_dy, *x, da, part, n, R, i, 1, i);
+    grads.g[1] = grad_args(plan, low_x, *dy, db, part + l.slots * R * I, n, R, o, R, 1);
+    if (tc_grad) {
+        if (e == cudaSuccess && da && !encode_rows(&grads.rows[0], *x, t, i, 64)) e = cudaErrorInvalidValue;
+        if (e == cudaSuccess && db && !encode_rows(&grads.rows[1], *dy, t, o, 64)) e = cudaErrorInvalidValue;
+        if (e == cudaSuccess && (da || db)) e = launch_adapt_grad_tc(grads, ad->type, st);
+    } else {
+        if (e == cudaSuccess && da) e = launch_adapt_grad(grads.g[0], x->type, st);
+        if (e == cudaSuccess && db) e = launch_adapt_grad(grads.g[1], dy->type, st);
+    }
+    if (e == cudaSuccess && (da || db) && t > adapt_chunk(t, n)) e = launch_adapt_join(grads.g[0], grads.g[1], st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt_backward: kernel launch failed");
     return HYMOE_OK;
 }

@@ -25,12 +25,12 @@ constexpr int kAdGradCols = 128;    // columns of a gradient tile
 // Rank padded to the kernels' sizes.
 __host__ __device__ constexpr int adapt_rp(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
-// Tokens of one gradient item.  An adapter of average length stays whole; a long one is cut into
+// Tokens of one gradient item.  An adapter of up to twice the average length stays whole; a long one is cut into
 // pieces that run side by side (their sums are added in order by a second kernel), five where it
 // has all the tokens, at most eight.
 constexpr int kAdMinChunk = 512, kAdMaxPieces = 8;
 __host__ __device__ constexpr int adapt_chunk(int T, int n) {
-    const int avg = static_cast<int>(static_cast<int64_t>(T) * 3 / (2 * static_cast<int64_t>(n))), fifth = T / 5;
+    const int avg = static_cast<int>(static_cast<int64_t>(T) * 2 / n), fifth = T / 5;
     int c = avg < fifth ? avg : fifth;
     const int least = (T + kAdMaxPieces - 1) / kAdMaxPieces;
     c = c < least ? least : c;
@@ -63,6 +63,7 @@ struct AdaptPlan {
     int* n_lists;    // [0] status (0, or DevErr bits of a wait that expired), [1] tiles, [2] items,
                      // [3] tiles that have an adapter (the first ones)
     int tile_rows;   // 64 or 128
+    unsigned* amax;  // gradients of fp16 rows: [2 n] largest |low| of every adapter (bits), of dy's then of x's
     unsigned* counters;  // [max_tiles] CTAs of a tile that have left their partial sums (0 between launches)
     int max_tiles, max_items;
     int spare_tiles; // of max_tiles, those for adapters' last, part-filled tiles
@@ -76,6 +77,7 @@ struct AdaptLow {      // low[row, j] = scale[a] * sum_k X[perm[row], k] W_a(j, 
     const float* scale;
     float* low;        // [T, RP]
     float* part;       // [max_tiles * S] partial sums of 64 x RP
+    unsigned* amax;    // [n] largest |low| of every adapter, or nullptr
     int K, R;
     int vec_x, vec_w;  // rows start on 16-byte boundaries
 };
@@ -97,7 +99,7 @@ struct AdaptGrad {     // G_a(m, j) = sum over a's rows of X[perm[row], m] low[r
     size_t ldx;
     float* g;          // [n] matrices: element (m, j) at m * gm + j * gj
     float* part;       // partial slots of M * R
-    int M, R, gm, gj;
+    int M, R, gm, gj, n;
     int vec_x;
 };
 
@@ -120,7 +122,9 @@ cudaError_t launch_adapt_decode(const AdaptDecode& d, int type_x, int type_w, in
 // (low) or the columns as its fast dimension (wide).
 cudaError_t launch_adapt_low(const AdaptLow& a, int type_x, int type_w, bool trans, int n_sms, cudaStream_t st);
 cudaError_t launch_adapt_wide(const AdaptWide& a, int type_y, int type_w, bool trans, int n_sms, cudaStream_t st);
-cudaError_t launch_adapt_grad(const AdaptGrad& a, int type_x, int T, int n, cudaStream_t st);
+cudaError_t launch_adapt_grad(const AdaptGrad& a, int type_x, cudaStream_t st);
+// Adds the pieces of long adapters in one or two gradients (g == nullptr: none).
+cudaError_t launch_adapt_join(const AdaptGrad& a, const AdaptGrad& b, cudaStream_t st);
 
 #ifdef __CUDACC__
 
@@ -133,6 +137,13 @@ __device__ __forceinline__ int4 ad_part_tile(const AdaptPlan& p, int id) {
     t.y += off;
     t.z = min(kAdRows, t.z - off);
     return t.z > 0 ? t : make_int4(-1, 0, 0, 0);
+}
+
+// The warp's largest |value| (never negative) into an adapter's entry: maxima commute, so any order
+// gives the same.
+__device__ __forceinline__ void ad_amax(unsigned* amax, float v) {
+    const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+    if ((threadIdx.x & 31) == 0) atomicMax(amax, m);
 }
 
 constexpr int ad_pad16(int bytes) { return (bytes / 16 % 2 == 0) ? bytes + 16 : bytes; }  // odd number of pieces

@@ -204,10 +204,12 @@ __global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant_
             }
 }
 
-// The pieces of adapters that have several, added in order.  Grid (columns, adapters).
-__global__ __launch_bounds__(256) void grad_join_kernel(const __grid_constant__ AdaptGrad a) {
+// The pieces of adapters that have several, added in order.  Grid (elements, adapters, gradients).
+__global__ __launch_bounds__(256) void grad_join_kernel(const __grid_constant__ AdaptGrad a0, const __grid_constant__ AdaptGrad a1) {
     griddep_wait();
     griddep_launch_dependents();
+    const AdaptGrad& a = blockIdx.z == 0 ? a0 : a1;
+    if (a.g == nullptr) return;
     const int ad = blockIdx.y, lo = a.plan.pieces[ad], hi = a.plan.pieces[ad + 1];
     if (hi - lo < 2) return;
     const size_t size = static_cast<size_t>(a.M) * a.R;
@@ -219,33 +221,36 @@ __global__ __launch_bounds__(256) void grad_join_kernel(const __grid_constant__ 
 }
 
 template <typename X, int RP>
-cudaError_t launch_t(const AdaptGrad& a, int T, int n, cudaStream_t st) {
+cudaError_t launch_t(const AdaptGrad& a, cudaStream_t st) {
     using L = GradTile<X, RP>;
     auto kern = grad_kernel<X, RP>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
-    e = launch_kernel(true, kern, dim3(a.plan.max_items, (a.M + kAdGradCols - 1) / kAdGradCols), dim3(kAdThreads), L::kSmem, st, a);
-    if (e != cudaSuccess || T <= adapt_chunk(T, n)) return e;  // no adapter can have two pieces
-    const size_t size = static_cast<size_t>(a.M) * a.R, blk = (size + 255) / 256;
-    return launch_kernel(true, grad_join_kernel, dim3(static_cast<unsigned>(blk < 1024 ? blk : 1024), n), dim3(256), 0, st, a);
+    return launch_kernel(true, kern, dim3(a.plan.max_items, (a.M + kAdGradCols - 1) / kAdGradCols), dim3(kAdThreads), L::kSmem, st, a);
 }
 
 template <typename X>
-cudaError_t launch_x(const AdaptGrad& a, int T, int n, cudaStream_t st) {
+cudaError_t launch_x(const AdaptGrad& a, cudaStream_t st) {
     switch (adapt_rp(a.R)) {
-        case 16: return launch_t<X, 16>(a, T, n, st);
-        case 32: return launch_t<X, 32>(a, T, n, st);
-        case 64: return launch_t<X, 64>(a, T, n, st);
-        default: return launch_t<X, 128>(a, T, n, st);
+        case 16: return launch_t<X, 16>(a, st);
+        case 32: return launch_t<X, 32>(a, st);
+        case 64: return launch_t<X, 64>(a, st);
+        default: return launch_t<X, 128>(a, st);
     }
 }
 
 }  // namespace
 
-cudaError_t launch_adapt_grad(const AdaptGrad& a, int type_x, int T, int n, cudaStream_t st) {
-    if (type_x == HYMOE_TYPE_F32) return launch_x<float>(a, T, n, st);
-    if (type_x == HYMOE_TYPE_F16) return launch_x<__half>(a, T, n, st);
-    return launch_x<__nv_bfloat16>(a, T, n, st);
+cudaError_t launch_adapt_join(const AdaptGrad& a, const AdaptGrad& b, cudaStream_t st) {
+    const size_t ma = a.g ? static_cast<size_t>(a.M) * a.R : 0, mb = b.g ? static_cast<size_t>(b.M) * b.R : 0;
+    const size_t blk = ((ma > mb ? ma : mb) + 255) / 256;
+    return launch_kernel(true, grad_join_kernel, dim3(static_cast<unsigned>(blk < 512 ? blk : 512), a.n, 2), dim3(256), 0, st, a, b);
+}
+
+cudaError_t launch_adapt_grad(const AdaptGrad& a, int type_x, cudaStream_t st) {
+    if (type_x == HYMOE_TYPE_F32) return launch_x<float>(a, st);
+    if (type_x == HYMOE_TYPE_F16) return launch_x<__half>(a, st);
+    return launch_x<__nv_bfloat16>(a, st);
 }
 
 }  // namespace hymoe

@@ -174,16 +174,23 @@ __global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void 
     float* dst = S == 1 ? a.low + static_cast<size_t>(tile.y) * RP
                         : a.part + (static_cast<size_t>(tile_id) * S + rank) * (kAdRows * RP);
     const float f1 = S == 1 ? f : 1.f;
+    float top = 0.f;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int r = warp * 16 + g + 8 * q;
         if (r >= tile.z) continue;
 #pragma unroll
-        for (int j = 0; j < RP / 8; ++j)
-            *reinterpret_cast<float2*>(dst + static_cast<size_t>(r) * RP + j * 8 + 2 * t) =
-                make_float2(acc[j][2 * q] * f1, acc[j][2 * q + 1] * f1);
+        for (int j = 0; j < RP / 8; ++j) {
+            const float2 v = make_float2(acc[j][2 * q] * f1, acc[j][2 * q + 1] * f1);
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+            *reinterpret_cast<float2*>(dst + static_cast<size_t>(r) * RP + j * 8 + 2 * t) = v;
+        }
     }
-    if (S == 1) return;
+    __syncwarp();
+    if (S == 1) {
+        if (a.amax != nullptr) ad_amax(a.amax + tile.x, top);
+        return;
+    }
     // The tile's last CTA adds the parts.  Its counter wraps back to 0 for the next call.
     __shared__ int last;
     __threadfence();
@@ -193,6 +200,7 @@ __global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void 
     if (!last) return;
     __threadfence();
     const float* part = a.part + static_cast<size_t>(tile_id) * S * (kAdRows * RP);
+    top = 0.f;
     for (int p = tid; p < tile.z * (RP / 4); p += kAdThreads) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -203,8 +211,12 @@ __global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void 
             s.z += v.z;
             s.w += v.w;
         }
-        reinterpret_cast<float4*>(a.low + static_cast<size_t>(tile.y) * RP)[p] = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+        s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w))));
+        reinterpret_cast<float4*>(a.low + static_cast<size_t>(tile.y) * RP)[p] = s;
     }
+    __syncwarp();
+    if (a.amax != nullptr) ad_amax(a.amax + tile.x, top);
 }
 
 template <typename X, typename W, int RP, bool TRANS>

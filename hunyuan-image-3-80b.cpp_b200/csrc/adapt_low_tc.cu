@@ -161,6 +161,7 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
             cluster_wait();
         }
         const int rows = kLtcRows / S;
+        float top = 0.f;
         for (int p = et; p < rows * (RP / 4); p += 128) {
             const int row = rank * rows + p / (RP / 4), c = p % (RP / 4) * 4;
             if (row >= tile.z) break;
@@ -172,9 +173,12 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
                 s.z += v.z;
                 s.w += v.w;
             }
-            *reinterpret_cast<float4*>(a.low + static_cast<size_t>(tile.y + row) * RP + c) =
-                make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+            s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w))));
+            *reinterpret_cast<float4*>(a.low + static_cast<size_t>(tile.y + row) * RP + c) = s;
         }
+        __syncwarp();
+        if (a.amax != nullptr) ad_amax(a.amax + tile.x, top);
     }
     if (S > 1) {  // every thread arrives once before the sums are read and once after
         if (warp < 2) {

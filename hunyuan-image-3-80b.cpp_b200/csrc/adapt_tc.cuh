@@ -27,6 +27,14 @@ cudaError_t launch_adapt_low_tc(const AdaptMaps& maps, const AdaptLow& a, int ty
 cudaError_t launch_adapt_wide_tc(const AdaptMaps& maps, const AdaptWide& a, int type_y, int type_w, bool trans, int n_sms,
                                  cudaStream_t st);
 
+// Both gradients of a call (either may be absent: g[i].g == nullptr; plan, R and n are always set).
+struct AdaptGradPair {
+    AdaptGrad g[2];
+    CUtensorMap rows[2];  // their long rows, box {64 values, 64 rows}
+    int groups0;          // column groups of the first (set by the launcher)
+};
+cudaError_t launch_adapt_grad_tc(AdaptGradPair p, int type_w, cudaStream_t st);
+
 #ifdef __CUDACC__
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
@@ -58,6 +66,16 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
                  : "r"(addr)
                  : "memory");
     return v;
+}
+
+// 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
 }
 
 // MN-major operand in the 128B swizzle (see above).
