@@ -161,9 +161,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
     if (p.items != nullptr) {
         const int n_items = ipre[n];
         for (int i = tid; i < n_items; i += kPlanThreads) {
-            const int a = bucket_of(ipre, n, i), q = i - ipre[a], r = q * chunk;
-            const bool several = ipre[a + 1] - ipre[a] > 1;
-            p.items[i] = make_int4(a, off[a] + r, min(chunk, tot[a] - r), several ? spre[a] + q : -1);
+            // equal pieces of whole 64s: none is empty, as chunk >= 512 makes tot > 512 (pieces - 1)
+            // and pieces <= 8
+            const int a = bucket_of(ipre, n, i), q = i - ipre[a], pieces = ipre[a + 1] - ipre[a];
+            const int len = ((tot[a] + pieces - 1) / pieces + 63) / 64 * 64, r = q * len;
+            p.items[i] = make_int4(a, off[a] + r, min(len, tot[a] - r), pieces > 1 ? spre[a] + q : -1);
         }
         for (int a = tid; a <= n; a += kPlanThreads) p.pieces[a] = ipre[a];
         for (int a = tid; a < 2 * n; a += kPlanThreads) p.amax[a] = 0u;

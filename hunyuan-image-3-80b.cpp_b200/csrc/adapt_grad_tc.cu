@@ -6,7 +6,7 @@
 // gradients' CTAs are one grid.  The tensor core sums over the tokens: D[128 columns, RP] +=
 // X^T low, twice.
 //   A  the rows as they lie in memory, [64 tokens][64 columns] panels: an MN-major operand; by TMA
-//      where the item's tokens are consecutive, else copied
+//      where a stage's tokens are consecutive, else copied
 //   B  low, split into three 16-bit parts and turned to [RP][64 tokens] on the way: K-major
 // bf16 parts hold fp32 whole; fp16 ones hold 33 bits below the adapter's largest value, by a power of
 // two that the narrow product left behind.  The sums go to several accumulators in turn (the pipe
@@ -20,7 +20,8 @@ namespace {
 
 constexpr int kGtcTok = 64;
 constexpr int kGtcCols = 256;                     // columns per CTA: two products of 128
-constexpr int kGtcThreads = 320;                  // TMA, MMA, four converting and four copying warps
+constexpr int kGtcConv = 2;                       // groups of four converting warps, in turn
+constexpr int kGtcThreads = 64 + (kGtcConv + 1) * 128;  // TMA, MMA, converting and copying warps
 constexpr int kGtcPanel = kGtcTok * 128;          // 64 columns of the stage's rows
 constexpr int kGtcX = kGtcCols / 64 * kGtcPanel;
 constexpr int kGtcParts = 3;
@@ -30,6 +31,7 @@ struct GtcTile {
     static constexpr int kPart = RP * 128;
     static constexpr int kStage = kGtcX + kGtcParts * kPart;
     static constexpr int kStages = 224 * 1024 / kStage < 4 ? 224 * 1024 / kStage : 4;
+    static_assert(kStages % kGtcConv == 0, "a group of converting warps always meets the same stages");
     static constexpr int kSmem = 1024 + kStages * kStage;
     static constexpr int kSet = kGtcCols / 128 * RP;           // accumulator columns of a set
     static constexpr int kSets = 512 / kSet < 4 ? 512 / kSet : 4;
@@ -54,12 +56,17 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
     const int4 item = a.plan.items[blockIdx.x];
     const int n_st = (item.z + kGtcTok - 1) / kGtcTok;
     const int* perm = a.plan.perm + item.y;
-    const int first = n_st > 0 ? __ldg(perm) : 0;
-    const bool run = n_st > 0 && __ldg(perm + item.z - 1) - first == item.z - 1;
-    const int n_tma = run ? item.z / kGtcTok : 0;  // the first stages by TMA, the others copied
+    // Of stages it .. it + 31, one per lane: the first token, and those that TMA takes (whole, of
+    // consecutive tokens); the others are copied.
+    const auto look = [&](int it, int* first) {
+        const int t = (it + lane) * kGtcTok;
+        const bool whole = t + kGtcTok <= item.z;
+        *first = whole ? __ldg(perm + t) : 0;
+        return __ballot_sync(0xffffffffu, whole && __ldg(perm + min(t, item.z - kGtcTok) + kGtcTok - 1) - *first == kGtcTok - 1);
+    };
     if (tid == 0) {
         for (int s = 0; s < L::kStages; ++s) {
-            mbar_init(&full[s], 9);  // TMA's thread, four converting and four copying warps
+            mbar_init(&full[s], 9);  // TMA's thread, a group of converting warps, four copying warps
             mbar_init(&empty[s], 1);
         }
         mbar_init(&done, 1);
@@ -83,21 +90,25 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
     }
 
     if (warp == 0) {
-        if (lane == 0) {
-            int it = 0;
-            for (; it < n_st; ++it) {
-                const int s = it % L::kStages;
-                if (!mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER)) break;
+        int it = 0, firsts = 0;
+        uint32_t tma = 0;
+        for (; it < n_st; ++it) {
+            const int s = it % L::kStages;
+            if (it % 32 == 0) tma = look(it, &firsts);
+            const int first = __shfl_sync(0xffffffffu, firsts, it % 32);
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER))) break;
+            if (lane == 0) {
                 uint8_t* sx = smem + s * L::kStage;
-                if (it < n_tma) {
+                if (tma >> (it % 32) & 1) {
                     mbar_arrive_expect_tx(&full[s], kGtcX);
 #pragma unroll
-                    for (int p = 0; p < kGtcCols / 64; ++p)
-                        tma_load_2d(sx + p * kGtcPanel, map, &full[s], m0 + p * 64, first + it * kGtcTok);
+                    for (int p = 0; p < kGtcCols / 64; ++p) tma_load_2d(sx + p * kGtcPanel, map, &full[s], m0 + p * 64, first);
                 } else {
                     mbar_arrive(&full[s]);
                 }
             }
+        }
+        if (lane == 0) {
             for (int j = it > L::kStages ? it - L::kStages : 0; j < it; ++j) mbar_drain(&full[j % L::kStages], (j / L::kStages) & 1);
         }
         __syncwarp();
@@ -128,13 +139,13 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
             mbar_drain(&done, 0);
         }
         __syncwarp();
-    } else if (warp < 6) {
+    } else if (warp < 2 + kGtcConv * 4) {
         // ------------------------------------------------------------ low's parts, then the results
-        const int ct = tid - 64;
+        const int ct = (tid - 64) & 127, group = (tid - 64) >> 7;
         constexpr int kJ = RP < 128 ? RP : 128;             // rank columns side by side over the threads
         constexpr int kOct = kGtcTok / 8;                   // groups of eight tokens
         constexpr int kPer = RP * kOct / 128;               // (column, octet) pairs of a thread
-        for (int it = 0; it < n_st; ++it) {
+        for (int it = group; it < n_st; it += kGtcConv) {
             const int s = it % L::kStages;
             bool ok = true;
 #pragma unroll
@@ -182,7 +193,7 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
         float* out = item.w >= 0 ? a.part + static_cast<size_t>(item.w) * a.M * a.R : a.g + static_cast<size_t>(item.x) * a.M * a.R;
         const int sets = n_st < L::kSets ? n_st : L::kSets;
 #pragma unroll 1
-        for (int h = 0; h < kGtcCols / 128; ++h) {
+        for (int h = group; h < kGtcCols / 128; h += kGtcConv) {
             const int m = m0 + h * 128 + q * 32 + lane;
 #pragma unroll 1
             for (int c = 0; c < RP; c += 16) {
@@ -214,13 +225,15 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
         tc_fence_before();
     } else {
         // ------------------------------------------------------------ rows in any order, and short stages
-        const int ct = tid - 192, piece = ct & 31, row0 = ct >> 5;  // pieces of 16 bytes of rows row0 + 4 i
+        const int ct = tid - 64 - kGtcConv * 128, piece = ct & 31, row0 = ct >> 5;  // pieces of 16 bytes of rows row0 + 4 i
         const bool in = m0 + piece * 8 < a.M;                       // M is a multiple of 8
-        int it = 0;
+        int it = 0, firsts;
+        uint32_t tma = 0;
         for (; it < n_st; ++it) {
             const int s = it % L::kStages;
+            if (it % 32 == 0) tma = look(it, &firsts);
             if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER))) break;
-            if (it >= n_tma) {
+            if (!(tma >> (it % 32) & 1)) {
                 uint8_t* dst = smem + s * L::kStage + piece / 8 * kGtcPanel;
 #pragma unroll
                 for (int i = 0; i < kGtcTok / 4; ++i) {

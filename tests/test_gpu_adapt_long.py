@@ -150,5 +150,4 @@ def test_other_types_beside_the_weights():
     """fp32 rows on one side only: each product takes its own path over one plan."""
     for x, y in (("f32", "bf16"), ("bf16", "f32")):
         p = with_ids(runs(*MIXES["both"]), 256, 264, 16, 4, x=x, y=y)
-        assert p.x.dtype == T16[x] and p.dy.dtype == T16[y]
         check(p)
