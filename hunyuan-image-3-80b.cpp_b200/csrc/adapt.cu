@@ -188,7 +188,7 @@ cudaError_t launch_plan_adapt(const int* ids, int T, int n, const AdaptPlan& p, 
 
 // The workspace: every part starts on 256 bytes.
 struct AdaptLayout {
-    size_t perm, tiles, items, pieces, amax, lists, counters, low, low2, low_part, part, slots, bytes;
+    size_t perm, tiles, items, pieces, amax, lists, counters, low, low2, low_part, part, slots, low16[2], bytes;
     int tile_rows, max_tiles, spare_tiles, max_items;
 };
 // (the sizes do not depend on tile_rows)
@@ -220,6 +220,7 @@ AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward, int 
         l.pieces = take((n + 1) * sizeof(int));
         l.amax = take(2 * n * sizeof(unsigned));
         l.low2 = take(T * adapt_rp(ad->rank) * sizeof(float));
+        for (size_t& at : l.low16) at = take(T > kTcRows ? T * adapt_parts(adapt_rp(ad->rank)) * 2 : 0);
         l.slots = 2 * long_pieces;  // an adapter of c tokens in p > 1 pieces: p < 2 c / chunk
         l.part = take(l.slots * ad->rank * (static_cast<size_t>(ad->in_features) + ad->out_features) * sizeof(float));
     }
@@ -588,8 +589,13 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
     grads.g[0] = grad_args(plan, low_dy, *x, da, part, n, R, i, 1, i);
     grads.g[1] = grad_args(plan, low_x, *dy, db, part + l.slots * R * I, n, R, o, R, 1);
     if (tc_grad) {
-        if (e == cudaSuccess && da && !encode_rows(&grads.rows[0], *x, t, i, 64)) e = cudaErrorInvalidValue;
-        if (e == cudaSuccess && db && !encode_rows(&grads.rows[1], *dy, t, o, 64)) e = cudaErrorInvalidValue;
+        const int wide = adapt_parts(adapt_rp(R));
+        for (int k = 0; k < 2; ++k) {
+            const hymoe_mat rows = k == 0 ? *x : *dy, low = {ws + l.low16[k], ad->type, wide};
+            grads.parts[k] = low.data;
+            if (grads.g[k].g && (!encode_rows(&grads.rows[k], rows, t, k == 0 ? i : o, 64) || !encode_rows(&grads.lows[k], low, t, wide, 64)))
+                e = cudaErrorInvalidValue;
+        }
         if (e == cudaSuccess && (da || db)) e = launch_adapt_grad_tc(grads, ad->type, st);
     } else {
         if (e == cudaSuccess && da) e = launch_adapt_grad(grads.g[0], x->type, st);

@@ -212,8 +212,20 @@ __global__ __launch_bounds__(256) void grad_join_kernel(const __grid_constant__ 
     if (a.g == nullptr) return;
     const int ad = blockIdx.y, lo = a.plan.pieces[ad], hi = a.plan.pieces[ad + 1];
     if (hi - lo < 2) return;
-    const size_t size = static_cast<size_t>(a.M) * a.R;
-    for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < size; i += static_cast<size_t>(gridDim.x) * 256) {
+    const size_t size = static_cast<size_t>(a.M) * a.R, at = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+    const size_t step = static_cast<size_t>(gridDim.x) * 256;
+    if (size % 4 == 0 && (reinterpret_cast<uintptr_t>(a.g) & 15) == 0) {
+        for (size_t i = at; i < size / 4; i += step) {
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int p = lo; p < hi; ++p) {
+                const float4 v = reinterpret_cast<const float4*>(a.part + static_cast<size_t>(a.plan.items[p].w) * size)[i];
+                s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+            }
+            reinterpret_cast<float4*>(a.g + ad * size)[i] = s;
+        }
+        return;
+    }
+    for (size_t i = at; i < size; i += step) {
         float s = 0.f;
         for (int p = lo; p < hi; ++p) s += a.part[static_cast<size_t>(a.plan.items[p].w) * size + i];
         a.g[ad * size + i] = s;
@@ -243,7 +255,7 @@ cudaError_t launch_x(const AdaptGrad& a, cudaStream_t st) {
 
 cudaError_t launch_adapt_join(const AdaptGrad& a, const AdaptGrad& b, cudaStream_t st) {
     const size_t ma = a.g ? static_cast<size_t>(a.M) * a.R : 0, mb = b.g ? static_cast<size_t>(b.M) * b.R : 0;
-    const size_t blk = ((ma > mb ? ma : mb) + 255) / 256;
+    const size_t blk = ((ma > mb ? ma : mb) + 1023) / 1024;
     return launch_kernel(true, grad_join_kernel, dim3(static_cast<unsigned>(blk < 512 ? blk : 512), a.n, 2), dim3(256), 0, st, a, b);
 }
 

@@ -2,17 +2,23 @@
 // weights' 16-bit type on 16-byte boundaries: for every adapter, the sum over its tokens of the outer
 // products of a long row (x or dy) and its narrow counterpart (low).
 //
-// A CTA takes 256 columns of the long rows and one item of the plan, 64 tokens a stage; both
-// gradients' CTAs are one grid.  The tensor core sums over the tokens: D[128 columns, RP] +=
-// X^T low, twice.
+// split_kernel writes every row of low as three 16-bit parts side by side: bf16 parts hold fp32 whole;
+// fp16 ones hold 33 bits below the adapter's largest value, by a power of two that the narrow product
+// left behind.  (Splitting within the product, once per column group, held it to a third of what
+// memory gives: the converting warps' instructions.)
+//
+// grad_tc_kernel: a CTA takes 256 columns of the long rows and one item of the plan, 64 tokens a stage;
+// both gradients' CTAs are one grid, the longest items first (a long one that starts last kept a
+// quarter of the GPU waiting).  The tensor core sums over the tokens: D[128 columns, parts] += X^T low.
 //   A  the rows as they lie in memory, [64 tokens][64 columns] panels: an MN-major operand; by TMA
 //      where a stage's tokens are consecutive, else copied
-//   B  low, split into three 16-bit parts and turned to [RP][64 tokens] on the way: K-major
-// bf16 parts hold fp32 whole; fp16 ones hold 33 bits below the adapter's largest value, by a power of
-// two that the narrow product left behind.  The sums go to several accumulators in turn (the pipe
-// truncates what it adds: with four, an eighth of the error of one), which are added at the end.
-// A stage that is not whole is copied with its last row repeated, so that nothing of other rows
-// meets low's zeros.  Bound by reading the long rows.
+//   B  low's parts, [64 tokens][64 values] panels, MN-major as well; by TMA, a short stage's copied
+//      with zeros behind the item's last token
+// One product of N = 3 ranks reads A once for all parts, whose sums stay apart until the end (three
+// products of one rank each cost twice the tensor pipe's time); rank 128 takes three products into two
+// accumulators.  Small ranks have room for several sets of accumulators, which take the stages in
+// turn: the pipe truncates what it adds, and each addition to a shorter sum loses less.  Bound by
+// reading the long rows.
 #include "adapt_tc.cuh"
 
 namespace hymoe {
@@ -20,23 +26,60 @@ namespace {
 
 constexpr int kGtcTok = 64;
 constexpr int kGtcCols = 256;                     // columns per CTA: two products of 128
-constexpr int kGtcConv = 2;                       // groups of four converting warps, in turn
-constexpr int kGtcThreads = 64 + (kGtcConv + 1) * 128;  // TMA, MMA, converting and copying warps
-constexpr int kGtcPanel = kGtcTok * 128;          // 64 columns of the stage's rows
+constexpr int kGtcThreads = 320;                  // TMA, MMA, four warps for the results and four that copy
+constexpr int kGtcPanel = kGtcTok * 128;          // 64 values of the stage's rows
 constexpr int kGtcX = kGtcCols / 64 * kGtcPanel;
 constexpr int kGtcParts = 3;
 
 template <int RP>
 struct GtcTile {
-    static constexpr int kPart = RP * 128;
-    static constexpr int kStage = kGtcX + kGtcParts * kPart;
+    static constexpr int kLow = kGtcParts * RP;                // 16-bit values of a row's parts
+    static constexpr int kWide = adapt_parts(RP);              // the same, in whole panels
+    static constexpr int kB = kWide / 64 * kGtcPanel;
+    static constexpr int kStage = kGtcX + kB;
     static constexpr int kStages = 224 * 1024 / kStage < 4 ? 224 * 1024 / kStage : 4;
-    static_assert(kStages % kGtcConv == 0, "a group of converting warps always meets the same stages");
     static constexpr int kSmem = 1024 + kStages * kStage;
-    static constexpr int kSet = kGtcCols / 128 * RP;           // accumulator columns of a set
+    static constexpr int kAccs = RP < 128 ? kGtcParts : 2;     // sums that stay apart
+    static constexpr int kAcc = kAccs * RP;
+    static constexpr int kSet = kGtcCols / 128 * kAcc;         // accumulator columns of a set
     static constexpr int kSets = 512 / kSet < 4 ? 512 / kSet : 4;
-    static constexpr int kTmem = kSet * kSets;
+    static_assert(kStages >= 2 && kSets >= 1, "a ring, and room for the sums");
 };
+
+// fp16 parts: low times 2^shift puts the adapter's largest value in [2^14, 2^15).
+__device__ __forceinline__ int gtc_exponent(unsigned amax) { return max(16, min(239, static_cast<int>(amax >> 23))); }
+
+template <typename W, int RP>
+__global__ __launch_bounds__(256) void split_kernel(const __grid_constant__ AdaptGradPair pair) {
+    using L = GtcTile<RP>;
+    const AdaptGrad& a = blockIdx.y == 0 ? pair.g[0] : pair.g[1];
+    griddep_wait();
+    griddep_launch_dependents();
+    if (a.g == nullptr || static_cast<int>(blockIdx.x) >= a.plan.n_lists[3]) return;
+    const int4 tile = a.plan.tiles[blockIdx.x];
+    float scale = 1.f;
+    if (AdType<W>::kScaled) {
+        const int e = gtc_exponent(a.plan.amax[blockIdx.y * a.n + tile.x]);
+        scale = __uint_as_float(static_cast<uint32_t>(254 + 14 - e) << 23);
+    }
+    const float4* src = reinterpret_cast<const float4*>(a.low + static_cast<size_t>(tile.y) * RP);
+    uint16_t* dst = static_cast<uint16_t*>(pair.parts[blockIdx.y]) + static_cast<size_t>(tile.y) * L::kWide;
+    for (int i = threadIdx.x; i < tile.z * (RP / 4); i += 256) {
+        const float4 f = src[i];
+        float v[4] = {f.x * scale, f.y * scale, f.z * scale, f.w * scale};
+        uint16_t* to = dst + static_cast<size_t>(i / (RP / 4)) * L::kWide + i % (RP / 4) * 4;
+#pragma unroll
+        for (int p = 0; p < kGtcParts; ++p) {
+            const uint2 w = make_uint2(AdType<W>::pack(v[0], v[1]), AdType<W>::pack(v[2], v[3]));
+            *reinterpret_cast<uint2*>(to + p * RP) = w;
+            const float2 lo = AdType<W>::unpack(w.x), hi = AdType<W>::unpack(w.y);
+            v[0] -= lo.x;
+            v[1] -= lo.y;
+            v[2] -= hi.x;
+            v[3] -= hi.y;
+        }
+    }
+}
 
 template <typename W, int RP>
 __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_constant__ AdaptGradPair pair) {
@@ -46,34 +89,47 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
     __shared__ uint64_t full[L::kStages], empty[L::kStages], done;
     __shared__ uint32_t tmem_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const bool second = static_cast<int>(blockIdx.y) >= pair.groups0;
+    const bool second = static_cast<int>(blockIdx.x) >= pair.groups0;
     const AdaptGrad& a = second ? pair.g[1] : pair.g[0];
-    const CUtensorMap* map = second ? &pair.rows[1] : &pair.rows[0];
-    const int m0 = (static_cast<int>(blockIdx.y) - (second ? pair.groups0 : 0)) * kGtcCols;
+    const CUtensorMap *map_x = second ? &pair.rows[1] : &pair.rows[0], *map_low = second ? &pair.lows[1] : &pair.lows[0];
+    const int m0 = (static_cast<int>(blockIdx.x) - (second ? pair.groups0 : 0)) * kGtcCols;
     griddep_wait();
     griddep_launch_dependents();
-    if (static_cast<int>(blockIdx.x) >= a.plan.n_lists[2]) return;
-    const int4 item = a.plan.items[blockIdx.x];
+    const int n_items = a.plan.n_lists[2];
+    if (static_cast<int>(blockIdx.y) >= n_items) return;
+    // a few items: the longest first (ties in their order)
+    int which = blockIdx.y;
+    if (n_items <= 32) {
+        const int len = lane < n_items ? a.plan.items[lane].z : -1;
+        int rank = 0;
+        for (int j = 0; j < n_items; ++j) {
+            const int other = __shfl_sync(0xffffffffu, len, j);
+            rank += other > len || (other == len && j < lane) ? 1 : 0;
+        }
+        which = __ffs(__ballot_sync(0xffffffffu, lane < n_items && rank == which)) - 1;
+    }
+    const int4 item = a.plan.items[which];
     const int n_st = (item.z + kGtcTok - 1) / kGtcTok;
     const int* perm = a.plan.perm + item.y;
     // Of stages it .. it + 31, one per lane: the first token, and those that TMA takes (whole, of
-    // consecutive tokens); the others are copied.
+    // consecutive tokens); the others' rows are copied.
     const auto look = [&](int it, int* first) {
         const int t = (it + lane) * kGtcTok;
         const bool whole = t + kGtcTok <= item.z;
         *first = whole ? __ldg(perm + t) : 0;
-        return __ballot_sync(0xffffffffu, whole && __ldg(perm + min(t, item.z - kGtcTok) + kGtcTok - 1) - *first == kGtcTok - 1);
+        const int last = whole ? __ldg(perm + t + kGtcTok - 1) : 0;
+        return __ballot_sync(0xffffffffu, whole && last - *first == kGtcTok - 1);
     };
     if (tid == 0) {
         for (int s = 0; s < L::kStages; ++s) {
-            mbar_init(&full[s], 9);  // TMA's thread, a group of converting warps, four copying warps
+            mbar_init(&full[s], 5);  // TMA's thread and four copying warps
             mbar_init(&empty[s], 1);
         }
         mbar_init(&done, 1);
         fence_mbar_init();
     }
     if (warp == 1) {
-        tmem_alloc(&tmem_s, L::kTmem);
+        tmem_alloc(&tmem_s, 512);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -81,13 +137,6 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
     tc_fence_after();
     const uint32_t tmem = tmem_s;
     int* err = a.plan.n_lists;
-    // fp16 parts: low times 2^shift, its largest value (over the adapter) in [2^14, 2^15)
-    float scale = 1.f, unscale = 1.f;
-    if (AdType<W>::kScaled) {
-        const int e = max(16, min(239, static_cast<int>(a.plan.amax[(second ? a.n : 0) + item.x] >> 23)));
-        scale = __uint_as_float(static_cast<uint32_t>(254 + 14 - e) << 23);
-        unscale = __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
-    }
 
     if (warp == 0) {
         int it = 0, firsts = 0;
@@ -99,12 +148,16 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
             if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER))) break;
             if (lane == 0) {
                 uint8_t* sx = smem + s * L::kStage;
-                if (tma >> (it % 32) & 1) {
-                    mbar_arrive_expect_tx(&full[s], kGtcX);
+                const bool rows = tma >> (it % 32) & 1, low = (it + 1) * kGtcTok <= item.z;
+                mbar_arrive_expect_tx(&full[s], (rows ? kGtcX : 0) + (low ? L::kB : 0));
+                if (rows) {
 #pragma unroll
-                    for (int p = 0; p < kGtcCols / 64; ++p) tma_load_2d(sx + p * kGtcPanel, map, &full[s], m0 + p * 64, first);
-                } else {
-                    mbar_arrive(&full[s]);
+                    for (int p = 0; p < kGtcCols / 64; ++p) tma_load_2d(sx + p * kGtcPanel, map_x, &full[s], m0 + p * 64, first);
+                }
+                if (low) {
+#pragma unroll
+                    for (int p = 0; p < L::kWide / 64; ++p)
+                        tma_load_2d(sx + kGtcX + p * kGtcPanel, map_low, &full[s], p * 64, item.y + it * kGtcTok);
                 }
             }
         }
@@ -114,24 +167,31 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr uint32_t idesc = ad_idesc<W>(RP, true, false);
+            constexpr int kN = RP < 128 ? L::kLow : RP;
+            constexpr uint32_t idesc = ad_idesc<W>(kN, true, true);
             for (int it = 0; it < n_st; ++it) {
                 const int s = it % L::kStages, set = it % L::kSets;
                 if (!mbar_wait(&full[s], (it / L::kStages) & 1, err, DEVERR_TIMEOUT_MMA)) break;
                 tc_fence_after();
                 const uint32_t sx = smem_u32(smem + s * L::kStage), sl = sx + kGtcX;
+                const uint32_t started = it >= L::kSets ? 1u : 0u;
 #pragma unroll
                 for (int h = 0; h < kGtcCols / 128; ++h) {
-                    uint32_t more = it >= L::kSets ? 1u : 0u;
+                    const uint32_t acc = tmem + set * L::kSet + h * L::kAcc;
 #pragma unroll
-                    for (int p = kGtcParts - 1; p >= 0; --p)
+                    for (int kk = 0; kk < kGtcTok / 16; ++kk) {
+                        const uint64_t da = sw128_mnmajor_desc(sx + 2 * h * kGtcPanel + kk * 2048, kGtcPanel);
+                        const uint32_t more = kk > 0 ? 1u : started;
+                        if (RP < 128) {
+                            mma_f16_ss(acc, da, sw128_mnmajor_desc(sl + kk * 2048, kGtcPanel), idesc, more);
+                        } else {  // the first part's sum, and that of the other two
 #pragma unroll
-                        for (int kk = 0; kk < kGtcTok / 16; ++kk) {
-                            mma_f16_ss(tmem + set * L::kSet + h * RP,
-                                       sw128_mnmajor_desc(sx + 2 * h * kGtcPanel + kk * 2048, kGtcPanel),
-                                       sw128_kmajor_desc(sl + p * L::kPart + kk * 32), idesc, more);
-                            more = 1u;
+                            for (int p = 0; p < kGtcParts; ++p)
+                                mma_f16_ss(acc + (p == 0 ? 0 : RP), da,
+                                           sw128_mnmajor_desc(sl + p * (RP / 64) * kGtcPanel + kk * 2048, kGtcPanel), idesc,
+                                           p == 2 ? 1u : more);
                         }
+                    }
                 }
                 mma_commit(&empty[s]);
             }
@@ -139,73 +199,32 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
             mbar_drain(&done, 0);
         }
         __syncwarp();
-    } else if (warp < 2 + kGtcConv * 4) {
-        // ------------------------------------------------------------ low's parts, then the results
-        const int ct = (tid - 64) & 127, group = (tid - 64) >> 7;
-        constexpr int kJ = RP < 128 ? RP : 128;             // rank columns side by side over the threads
-        constexpr int kOct = kGtcTok / 8;                   // groups of eight tokens
-        constexpr int kPer = RP * kOct / 128;               // (column, octet) pairs of a thread
-        for (int it = group; it < n_st; it += kGtcConv) {
-            const int s = it % L::kStages;
-            bool ok = true;
-#pragma unroll
-            for (int i0 = 0; i0 < kPer; i0 += 4) {
-                constexpr int kNow = kPer < 4 ? kPer : 4;
-                float v[kNow][8];
-#pragma unroll
-                for (int i = 0; i < kNow; ++i) {
-                    const int idx = ct + (i0 + i) * 128, j = idx % kJ, t0 = it * kGtcTok + idx / kJ * 8;
-#pragma unroll
-                    for (int t = 0; t < 8; ++t)
-                        v[i][t] = t0 + t < item.z ? a.low[static_cast<size_t>(item.y + t0 + t) * RP + j] : 0.f;
-                }
-                if (i0 == 0) ok = mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_DEQUANT);
-                uint8_t* sl = smem + s * L::kStage + kGtcX;
-#pragma unroll
-                for (int i = 0; i < kNow; ++i) {
-                    const int idx = ct + (i0 + i) * 128, j = idx % kJ, oct = idx / kJ;
-                    if (AdType<W>::kScaled) {
-#pragma unroll
-                        for (int t = 0; t < 8; ++t) v[i][t] *= scale;
-                    }
-#pragma unroll
-                    for (int p = 0; p < kGtcParts; ++p) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            w[t] = AdType<W>::pack(v[i][2 * t], v[i][2 * t + 1]);
-                            const float2 b = AdType<W>::unpack(w[t]);
-                            v[i][2 * t] -= b.x;
-                            v[i][2 * t + 1] -= b.y;
-                        }
-                        *reinterpret_cast<uint4*>(sl + p * L::kPart + sw128_offset(j, oct)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
-            }
-            if (!__all_sync(0xffffffffu, ok)) break;
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[s]);
-        }
+    } else if (warp < 6) {
+        // ------------------------------------------------------------ the results
         if (n_st > 0) mbar_wait(&done, 0, err, DEVERR_TIMEOUT_EPILOGUE);
         tc_fence_after();
+        float unscale = 1.f;
+        if (AdType<W>::kScaled)
+            unscale = __uint_as_float(static_cast<uint32_t>(gtc_exponent(a.plan.amax[(second ? a.n : 0) + item.x]) - 14) << 23);
         const int q = warp & 3;
         float* out = item.w >= 0 ? a.part + static_cast<size_t>(item.w) * a.M * a.R : a.g + static_cast<size_t>(item.x) * a.M * a.R;
         const int sets = n_st < L::kSets ? n_st : L::kSets;
 #pragma unroll 1
-        for (int h = group; h < kGtcCols / 128; h += kGtcConv) {
+        for (int h = 0; h < kGtcCols / 128; ++h) {
             const int m = m0 + h * 128 + q * 32 + lane;
 #pragma unroll 1
             for (int c = 0; c < RP; c += 16) {
                 float v[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = 0.f;
-                for (int set = 0; set < sets; ++set) {
-                    uint32_t u[16];
-                    tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + set * L::kSet + h * RP + c, u);
-                    tmem_ld_wait();
+                for (int p = L::kAccs - 1; p >= 0; --p) {  // the small parts first
+                    for (int set = 0; set < sets; ++set) {
+                        uint32_t u[16];
+                        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + set * L::kSet + h * L::kAcc + p * RP + c, u);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(u[j]);
+                        for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(u[j]);
+                    }
                 }
                 if (m < a.M) {
 #pragma unroll
@@ -225,22 +244,33 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
         tc_fence_before();
     } else {
         // ------------------------------------------------------------ rows in any order, and short stages
-        const int ct = tid - 64 - kGtcConv * 128, piece = ct & 31, row0 = ct >> 5;  // pieces of 16 bytes of rows row0 + 4 i
+        const int ct = tid - 192, piece = ct & 31, row0 = ct >> 5;  // pieces of 16 bytes of rows row0 + 4 i
         const bool in = m0 + piece * 8 < a.M;                       // M is a multiple of 8
         int it = 0, firsts;
         uint32_t tma = 0;
         for (; it < n_st; ++it) {
-            const int s = it % L::kStages;
+            const int s = it % L::kStages, left = item.z - it * kGtcTok;
             if (it % 32 == 0) tma = look(it, &firsts);
             if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER))) break;
+            uint8_t* sx = smem + s * L::kStage;
             if (!(tma >> (it % 32) & 1)) {
-                uint8_t* dst = smem + s * L::kStage + piece / 8 * kGtcPanel;
+                uint8_t* dst = sx + piece / 8 * kGtcPanel;
 #pragma unroll
                 for (int i = 0; i < kGtcTok / 4; ++i) {
-                    const int r = row0 + 4 * i, at = min(it * kGtcTok + r, item.z - 1);
+                    const int r = row0 + 4 * i;
+                    const bool have = in && r < left;
                     const char* src = static_cast<const char*>(a.x);
-                    if (in) src += (static_cast<size_t>(__ldg(perm + at)) * a.ldx + m0 + piece * 8) * 2;
-                    cp_async16_part(dst + sw128_offset(r, piece % 8), src, in ? 16 : 0);
+                    if (have) src += (static_cast<size_t>(__ldg(perm + it * kGtcTok + r)) * a.ldx + m0 + piece * 8) * 2;
+                    cp_async16_part(dst + sw128_offset(r, piece % 8), src, have ? 16 : 0);
+                }
+            }
+            if (left < kGtcTok) {
+                const char* low = static_cast<const char*>(second ? pair.parts[1] : pair.parts[0]);
+                for (int i = ct; i < kGtcTok * (L::kLow / 8); i += 128) {
+                    const int r = i / (L::kLow / 8), c = i % (L::kLow / 8);
+                    const bool have = r < left;
+                    const char* src = have ? low + (static_cast<size_t>(item.y + it * kGtcTok + r) * L::kWide + c * 8) * 2 : low;
+                    cp_async16_part(sx + kGtcX + c / 8 * kGtcPanel + sw128_offset(r, c % 8), src, have ? 16 : 0);
                 }
             }
             cp_async_commit();
@@ -259,7 +289,7 @@ __global__ __launch_bounds__(kGtcThreads, 1) void grad_tc_kernel(const __grid_co
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, L::kTmem);
+        tmem_dealloc(tmem, 512);
     }
 }
 
@@ -267,10 +297,11 @@ template <typename W, int RP>
 cudaError_t launch_t(const AdaptGradPair& p, cudaStream_t st) {
     using L = GtcTile<RP>;
     auto kern = grad_tc_kernel<W, RP>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    if (e == cudaSuccess) e = launch_kernel(true, split_kernel<W, RP>, dim3(p.g[0].plan.max_tiles, 2), dim3(256), 0, st, p);
     if (e != cudaSuccess) return e;
     const int groups1 = p.g[1].g ? (p.g[1].M + kGtcCols - 1) / kGtcCols : 0;
-    return launch_kernel(true, kern, dim3(p.g[0].plan.max_items, p.groups0 + groups1), dim3(kGtcThreads), L::kSmem, st, p);
+    return launch_kernel(true, kern, dim3(p.groups0 + groups1, p.g[0].plan.max_items), dim3(kGtcThreads), L::kSmem, st, p);
 }
 
 template <typename W>

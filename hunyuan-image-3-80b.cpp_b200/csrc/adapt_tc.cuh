@@ -27,10 +27,15 @@ cudaError_t launch_adapt_low_tc(const AdaptMaps& maps, const AdaptLow& a, int ty
 cudaError_t launch_adapt_wide_tc(const AdaptMaps& maps, const AdaptWide& a, int type_y, int type_w, bool trans, int n_sms,
                                  cudaStream_t st);
 
+// 16-bit values of a row of low in three parts, in whole panels of 64.
+__host__ __device__ constexpr int adapt_parts(int rp) { return (3 * rp + 63) / 64 * 64; }
+
 // Both gradients of a call (either may be absent: g[i].g == nullptr; plan, R and n are always set).
 struct AdaptGradPair {
     AdaptGrad g[2];
     CUtensorMap rows[2];  // their long rows, box {64 values, 64 rows}
+    CUtensorMap lows[2];  // low in parts, the same box
+    void* parts[2];       // [T, adapt_parts(RP)] 16-bit values: low's parts, in sorted order
     int groups0;          // column groups of the first (set by the launcher)
 };
 cudaError_t launch_adapt_grad_tc(AdaptGradPair p, int type_w, cudaStream_t st);
