@@ -12,19 +12,25 @@
 // which names the expert by itself, and a shift in the lane that held it.
 //
 // What the replaced bits and fp32 hide is then checked.  16-bit logits lose nothing.  The selected
-// experts' values are formed again in fp32 and neighbours compared: with the documented errors of
-// the fp32 functions (__expf 2 + 1.173 |x| ulp times s (1 - s), __fdividef 2 ulp; expf 1 ulp and the
-// roundings of a softmax's sum) a value is off by less than 2^-21 (sigmoid) or 2^-20 (softmax) plus
-// 2^-23 of itself, so values further apart than twice that are in the exact order, and two experts
-// of the same logit and bias tie in any precision; the best key left out is compared as the largest
-// value it can stand for.  A token that cannot be proven is selected again in double precision
-// (route_exact).
+// experts' values are formed again in fp32 and neighbours compared: with the documented errors of the
+// fp32 functions (ex2.approx 2^-22 relative and half a step of its argument, times s (1 - s),
+// rcp.approx 1 ulp; expf 1 ulp and the roundings of a softmax's sum) a value is off by less than 2^-21
+// (sigmoid) or 2^-20 (softmax) plus 2^-23 of itself, so values further apart than twice that are in
+// the exact order, and two experts of the same logit and bias tie in any precision; the best one left
+// out is compared too, and the next one as the most that its key can stand for.
 //
 // Weights come from the selected logits with the largest one's exponent taken out, so a
 // renormalised row is right however small its scores are.
 //
-// Bound by instruction issue: a token of 128 experts and 6 choices takes some 250 warp
-// instructions, while its bf16 logits are 256 bytes.
+// A token whose choices cannot be proven has its K + 1 best ordered in double precision (settle);
+// only where that does not prove them either, or which groups are kept is in doubt, all its experts
+// are (route_exact).
+//
+// Bound by instruction issue, and by latency in short calls: 128 experts and 6 choices with a bias,
+// bf16, take 3.0 us for 256 tokens (a warp each), 27.7 us for 131072 (a thread each; 60.6 by warps,
+// some 400 warp instructions a token, while its logits are 256 bytes); 256 experts in 8 groups 12 us
+// for 8192 tokens (26 before the candidates were settled by themselves: one token selected again in
+// full took longer than all the others).
 #pragma once
 
 #include <math.h>
@@ -133,7 +139,7 @@ __device__ __forceinline__ void store_row(T* row, int E, const float (&v)[EPL]) 
 
 // Best (value, index) of the warp: the larger value, the lower index where they tie.
 __device__ __forceinline__ void warp_best(double& v, int& e) {
-#pragma unroll
+#pragma unroll 1
     for (int o = 16; o; o >>= 1) {
         const double ov = __shfl_xor_sync(kAll, v, o);
         const int oe = __shfl_xor_sync(kAll, e, o);
@@ -165,6 +171,9 @@ __device__ __forceinline__ unsigned order_key(float v) {
 __device__ __forceinline__ float key_value(unsigned k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
+
+// A closed expert's key is 0, or that of -inf: under this one and so under every open expert's.
+constexpr unsigned kOpenKey = 0x00800000u;  // order_key(-FLT_MAX)
 
 // Descending, by Batcher's odd-even merge sort: every index is known at compile time.
 template <int A, int B, int N>
@@ -228,55 +237,59 @@ __device__ __forceinline__ float gate_weight(float z, bool norm, float m, float 
     return w * scale;
 }
 
-template <typename T, int EPL>
+// Selection of one token in double precision by a warp: lane k returns the k-th expert, or -1.  Rare
+// and cold: the loops stay loops, as fetching long straight code took longer than running it (15 us
+// against 6 for 256 experts in 8 groups).
+template <typename T>
 __device__ int select_exact(const T* __restrict__ row, const GateArgs& a) {
-    const int lane = threadIdx.x & 31, E = a.E;
-    float z[EPL];
-    double s[EPL], c[EPL];
-    {
-        Vec<T, EPL> raw;
-        fetch_row<T, EPL, false>(row, E, raw);
-        clean_row(raw, z);
-    }
+    constexpr int kMost = HYMOE_GATE_MAX_EXPERTS / 32;
+    const int lane = threadIdx.x & 31, E = a.E, n = (E + 31) / 32;
+    const bool sig = a.score == HYMOE_SCORE_SIGMOID, two = a.group_score == HYMOE_GROUP_TOP2;
+    double c[kMost], gv[kMost];  // what orders expert lane + 32 i, and what its group counts
     float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) m = fmaxf(m, z[i]);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i)
+        if (lane + 32 * i < E) m = fmaxf(m, clean_logit(gate_value(row[lane + 32 * i])));
     m = warp_max(m);
     double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-        s[i] = 0.0;
-        if (z[i] > -INFINITY)
-            s[i] = a.score == HYMOE_SCORE_SIGMOID ? 1.0 / (1.0 + exp(-static_cast<double>(z[i]))) : exp(static_cast<double>(z[i]) - m);
-        sum += s[i];
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const float z = lane + 32 * i < E ? clean_logit(gate_value(row[lane + 32 * i])) : -INFINITY;
+        double s = 0.0;
+        if (z > -INFINITY && (a.bias != nullptr || two)) {
+            s = exp(sig ? -static_cast<double>(z) : static_cast<double>(z) - m);
+            if (sig) s = 1.0 / (1.0 + s);
+        }
+        sum += s;
+        c[i] = z;
+        gv[i] = s;
     }
     sum = warp_sum(sum);
-    const bool two = a.group_score == HYMOE_GROUP_TOP2;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
         const int e = lane + 32 * i;
-        if (a.score == HYMOE_SCORE_SOFTMAX) s[i] = sum > 0.0 ? s[i] / sum : 0.0;
-        const double b = a.bias != nullptr && e < E ? static_cast<double>(clean_logit(__ldg(a.bias + e))) : 0.0;
-        c[i] = z[i] == -INFINITY ? -INFINITY : a.bias != nullptr ? s[i] + b : static_cast<double>(z[i]);
+        if (c[i] == -INFINITY) {
+            gv[i] = -INFINITY;
+            continue;
+        }
+        const double s = sig ? gv[i] : sum > 0.0 ? gv[i] / sum : 0.0;
+        if (a.bias != nullptr) c[i] = s + static_cast<double>(clean_logit(__ldg(a.bias + e)));
+        gv[i] = two && a.bias == nullptr ? s : c[i];
     }
     if (a.n_group > 0) {
         const int gs = E / a.n_group;
         double val = -INFINITY;  // lane g: group g's value
+#pragma unroll 1
         for (int g = 0; g < a.n_group; ++g) {
             double b1 = -INFINITY, b2 = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < EPL; ++i) {
+#pragma unroll 1
+            for (int i = g * gs / 32; i < n && 32 * i < (g + 1) * gs; ++i) {
                 const int e = lane + 32 * i;
                 if (e < g * gs || e >= (g + 1) * gs) continue;
-                const double v = two && a.bias == nullptr && z[i] != -INFINITY ? s[i] : c[i];
-                if (v > b1) {
-                    b2 = b1;
-                    b1 = v;
-                } else if (v > b2) {
-                    b2 = v;
-                }
+                b2 = fmax(b2, fmin(b1, gv[i]));
+                b1 = fmax(b1, gv[i]);
             }
-#pragma unroll
+#pragma unroll 1
             for (int o = 16; o; o >>= 1) {
                 const double o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
                 b2 = fmax(fmin(b1, o1), fmax(b2, o2));
@@ -284,35 +297,31 @@ __device__ int select_exact(const T* __restrict__ row, const GateArgs& a) {
             }
             if (lane == g) val = two && b2 > -INFINITY ? b1 + b2 : b1;
         }
-        unsigned kept = 0;
-        for (int r = 0; r < a.topk_group; ++r) {
-            double v = lane < a.n_group && !(kept >> lane & 1u) ? val : -INFINITY;
-            int g = v > -INFINITY ? lane : 64;
-            warp_best(v, g);
-            if (v == -INFINITY) break;
-            kept |= 1u << g;
+        int better = 0;
+#pragma unroll 1
+        for (int g = 0; g < a.n_group; ++g) {
+            const double v = __shfl_sync(kAll, val, g);
+            better += v > val || (v == val && g < lane);
         }
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-            const int e = lane + 32 * i;
-            if (e < E && !(kept >> (e / gs) & 1u)) c[i] = -INFINITY;
-        }
+        const unsigned kept = __ballot_sync(kAll, lane < a.n_group && val > -INFINITY && better < a.topk_group);
+#pragma unroll 1
+        for (int i = 0; i < n; ++i)
+            if (lane + 32 * i < E && !(kept >> ((lane + 32 * i) / gs) & 1u)) c[i] = -INFINITY;
     }
     int sel = -1;
+#pragma unroll 1
     for (int k = 0; k < a.K; ++k) {
         double v = -INFINITY;
         int e = 1 << 20;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
+#pragma unroll 1
+        for (int i = 0; i < n; ++i)
             if (c[i] > v) {
                 v = c[i];
                 e = lane + 32 * i;
             }
         warp_best(v, e);
         if (v == -INFINITY) break;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-            if (e == lane + 32 * i) c[i] = -INFINITY;
+        if ((e & 31) == lane) c[e >> 5] = -INFINITY;
         if (lane == k) sel = e;
     }
     return sel;
@@ -328,27 +337,64 @@ __device__ __forceinline__ void put_choice(const GateArgs& a, size_t t, int sel,
     if (cnt != nullptr && sel >= 0) atomicAdd(cnt + sel, 1);
 }
 
-// A token in double precision where its order could not be proven in fp32: outputs and counts.
-template <typename T, int EPL, bool SIG>
-__device__ __noinline__ void route_exact(const T* __restrict__ row, size_t t, const GateArgs& a, int* cnt) {
-    const int sel = select_exact<T, EPL>(row, a);
+// Lane k's weight for its selection and both to memory.
+template <typename T>
+__device__ void finish_choice(const T* __restrict__ row, size_t t, const GateArgs& a, int sel, int* cnt) {
+    const int lane = threadIdx.x & 31;
     const float z = sel >= 0 ? clean_logit(gate_value(row[sel])) : -INFINITY;
-    float m = 0.f, sum = 0.f;
-    if (!SIG && !a.norm) {
-        Vec<T, EPL> raw;
-        float c[EPL];
-        fetch_row<T, EPL, false>(row, a.E, raw);
-        clean_row(raw, c);
-        m = c[0];
-#pragma unroll
-        for (int i = 1; i < EPL; ++i) m = fmaxf(m, c[i]);
+    if (a.score == HYMOE_SCORE_SIGMOID) {
+        put_choice(a, t, sel, gate_weight<true>(z, a.norm, 0.f, 0.f, a.scale), cnt);
+        return;
+    }
+    float m = -INFINITY, sum = 0.f;
+    if (!a.norm) {
+#pragma unroll 1
+        for (int e = lane; e < a.E; e += 32) m = fmaxf(m, clean_logit(gate_value(row[e])));
         m = warp_max(m);
         m = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) sum += expf(c[i] - m);
+#pragma unroll 1
+        for (int e = lane; e < a.E; e += 32) sum += expf(clean_logit(gate_value(row[e])) - m);
         sum = warp_sum(sum);
     }
-    put_choice(a, t, sel, gate_weight<SIG>(z, a.norm, m, sum, a.scale), cnt);
+    put_choice(a, t, sel, gate_weight<false>(z, a.norm, m, sum, a.scale), cnt);
+}
+
+// A token in double precision where its order could not be proven in fp32: outputs and counts.
+template <typename T>
+__device__ __noinline__ void route_exact(const T* __restrict__ row, size_t t, const GateArgs& a, int* cnt) {
+    finish_choice(row, t, a, select_exact(row, a), cnt);
+}
+
+// The order of a few candidates in double precision, by a warp: lane j < K + 1 brings candidate j's
+// key (0: none); second: the largest key among the experts that are no candidates.  Sigmoid scores
+// with a bias, or logits.  Lane k returns the k-th expert, or -1; -2 in every lane where an expert
+// that is no candidate may come in.
+template <typename T>
+__device__ __forceinline__ int settle(const T* __restrict__ row, const GateArgs& a, unsigned cand, unsigned second) {
+    const int lane = threadIdx.x & 31;
+    const bool have = cand >= kOpenKey;
+    int e = have ? static_cast<int>(a.mask - (cand & a.mask)) : (1 << 20) + lane;
+    double d = -INFINITY;
+    if (have) {
+        d = clean_logit(gate_value(row[e]));
+        if (a.bias != nullptr) d = 1.0 / (1.0 + exp(-d)) + static_cast<double>(clean_logit(__ldg(a.bias + e)));
+    }
+    int rank = 0, from = 0;
+#pragma unroll 1
+    for (int j = 0; j <= a.K; ++j) {
+        const double dj = __shfl_sync(kAll, d, j);
+        const int ej = __shfl_sync(kAll, e, j);
+        rank += dj > d || (dj == d && ej < e);
+    }
+#pragma unroll 1
+    for (int j = 0; j <= a.K; ++j)
+        if (__shfl_sync(kAll, rank, j) == lane) from = j;
+    e = __shfl_sync(kAll, e, from);
+    d = __shfl_sync(kAll, d, from);
+    const double last = __shfl_sync(kAll, d, a.K - 1), most = key_value(second | a.mask);
+    const double slack = a.bias != nullptr ? 0x1p-20 + 0x1p-22 * fabs(last) : 0.0;
+    if (second >= kOpenKey && !(last - most > slack)) return -2;
+    return lane < a.K && e < (1 << 20) ? e : -1;
 }
 
 // One token: lane k gets its k-th expert (-1: none left) and weight; false where the selection has
@@ -487,7 +533,7 @@ __device__ __forceinline__ bool route_token(const T* row, const Vec<T, EPL>& raw
         for (int i = 0; i + 1 < EPL; ++i) key[i] = pop ? key[i + 1] : key[i];
         key[EPL - 1] = pop ? 0u : key[EPL - 1];
     }
-    const int sel = chosen != 0 ? static_cast<int>(a.mask - (chosen & a.mask)) : -1;
+    int sel = chosen != 0 ? static_cast<int>(a.mask - (chosen & a.mask)) : -1;
     float z = -INFINITY;
     if (biased || sizeof(T) == 4) {
         if (sel >= 0) z = clean_logit(gate_value(row[sel]));
@@ -500,19 +546,40 @@ __device__ __forceinline__ bool route_token(const T* row, const Vec<T, EPL>& raw
         const float lo = key_value(chosen & ~a.mask), hi = key_value(after | a.mask);
         const float slack = biased ? 2.f * delta + 0x1p-22f * fabsf(lo) : 0.f;
         if (__any_sync(kAll, lane <= last && after != 0 && !(lo - hi > slack))) {
+            // the best one left by its own value, the next by the most that its key can stand for
+            unsigned second = 0;
+            float zl = -INFINITY, bl = 0.f;
+            if (best_left != 0) {
+                second = __reduce_max_sync(kAll, key[0] == best_left ? key[1] : key[0]);
+                const int el = static_cast<int>(a.mask - (best_left & a.mask));
+                zl = clean_logit(gate_value(row[el]));
+                if (biased) bl = clean_logit(__ldg(a.bias + el));
+            }
             const float pz = __shfl_up_sync(kAll, z, 1);
             bool bad = false;
             if (biased) {
-                const float b = sel >= 0 ? clean_logit(__ldg(a.bias + sel)) : 0.f;
-                const float v = (SIG ? quick_sigmoid(z) : sum > 0.f ? expf(z - m) * quick_rcp(sum) : 0.f) + b;
+                const auto value = [&](float zz) { return SIG ? quick_sigmoid(zz) : sum > 0.f ? expf(zz - m) * quick_rcp(sum) : 0.f; };
+                const float b = sel >= 0 ? clean_logit(__ldg(a.bias + sel)) : 0.f, v = value(z) + b;
                 const float pv = __shfl_up_sync(kAll, v, 1), pb = __shfl_up_sync(kAll, b, 1);
                 if (lane > 0 && lane <= last)
                     bad = !(pv - v > 2.f * delta + 0x1p-22f * fabsf(pv)) && !(pz == z && pb == b);
-                if (lane == last && after != 0) bad = bad || !(v - hi > 2.f * delta + 0x1p-22f * fabsf(v));
+                if (lane == last && best_left != 0) {
+                    const float least = 2.f * delta + 0x1p-22f * fabsf(v);
+                    bad = bad || (!(v - (value(zl) + bl) > least) && !(z == zl && b == bl));
+                    bad = bad || (second != 0 && !(v - key_value(second | a.mask) > least));
+                }
             } else {
-                bad = (lane > 0 && lane <= last && pz < z) || (lane == last && after != 0 && ((chosen ^ after) & ~a.mask) == 0);
+                bad = (lane > 0 && lane <= last && pz < z) ||
+                      (lane == last && best_left != 0 && (z < zl || ((chosen ^ second) & ~a.mask) == 0));
             }
-            unsure = __any_sync(kAll, bad) || unsure;
+            if (__any_sync(kAll, bad)) {
+                int e = -2;
+                if ((SIG || !biased) && K < 32)
+                    e = settle(row, a, lane < K ? chosen : lane == K ? best_left : 0u, second);
+                unsure = unsure || __any_sync(kAll, e == -2);
+                sel = e;
+                z = sel >= 0 ? clean_logit(gate_value(row[sel])) : -INFINITY;
+            }
         }
     } else if (sel >= 0) {  // the key is the logit: its replaced bits were those of a 16-bit value
         z = fminf(key_value(chosen & 0x80000000u ? chosen & ~a.mask : chosen | a.mask), kBig);
@@ -563,7 +630,7 @@ __global__ __launch_bounds__(32 * kGateWarps, EPL <= 2 ? 6 : EPL == 4 ? 5 : EPL 
         }
         for (; again != 0; again &= again - 1) {
             const size_t u = first + static_cast<size_t>(__ffs(again) - 1) * step;
-            route_exact<T, EPL, SIG>(logits + u * ld, u, a, a.counts != nullptr ? cnt : nullptr);
+            route_exact<T>(logits + u * ld, u, a, a.counts != nullptr ? cnt : nullptr);
         }
     }
     if (a.counts != nullptr) {
@@ -572,6 +639,272 @@ __global__ __launch_bounds__(32 * kGateWarps, EPL <= 2 ? 6 : EPL == 4 ? 5 : EPL 
             if (gridDim.x == 1) a.counts[e] = cnt[e];
             else if (cnt[e]) atomicAdd(a.counts + e, cnt[e]);  // whole numbers: any order gives the same
         }
+    }
+}
+
+// ---- a token per thread
+//
+// For many tokens, without scores to write: a thread takes its token's experts eight at a time, sorts
+// their keys and merges them into the eight best so far (two sorting networks: some 11 operations per
+// expert, where a warp per token pays a reduction and a shift per choice for one token alone).  Keys,
+// certificates and weights are those of route_token; a thread's sums are its own.  A token that
+// cannot be proven is left to its warp at the end.
+constexpr int kRowsTopk = 8;
+
+// The eight best of l (descending) and of eight keys (descending); rest: the largest key left out.
+__device__ __forceinline__ void merge_best(unsigned (&l)[8], const unsigned (&k)[8], unsigned& rest) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        rest = max(rest, min(l[i], k[7 - i]));
+        l[i] = max(l[i], k[7 - i]);
+    }
+#pragma unroll
+    for (int d = 4; d; d >>= 1)  // what is left rises and falls: halves compared, quarters, pairs
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if ((i & d) == 0) {
+                const unsigned hi = max(l[i], l[i + d]), lo = min(l[i], l[i + d]);
+                l[i] = hi;
+                l[i + d] = lo;
+            }
+}
+
+// Eight values that order the experts (or their groups): s + b, scores or logits; -inf: closed.
+template <typename T, bool BIASED>
+__device__ __forceinline__ void eight_values(const Vec<T, 8>& raw, const float* bias, bool scored, float (&v)[8]) {
+    Vec<float, 8> b;
+    if (BIASED) b = *reinterpret_cast<const Vec<float, 8>*>(bias);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float z = BIASED ? fmaxf(gate_value(raw.v[i]), -INFINITY) : clean_logit(gate_value(raw.v[i]));
+        v[i] = z;
+        if (BIASED) v[i] = z == -INFINITY ? z : quick_sigmoid(z) + b.v[i];
+        else if (scored) v[i] = z == -INFINITY ? z : quick_sigmoid(z);
+    }
+}
+
+template <typename T, bool BIASED, bool GROUPS>
+__global__ __launch_bounds__(128, 8) void gate_rows_kernel(const T* __restrict__ logits, size_t ld, uint32_t n_tok,
+                                                        const __grid_constant__ GateArgs a) {
+    extern __shared__ __align__(16) float rbuf[];  // [E] biases, [n_group][threads] values
+    __shared__ int cnt[HYMOE_GATE_MAX_EXPERTS];
+    const int tid = threadIdx.x, E = a.E, K = a.K;
+    for (int e = tid; e < E; e += blockDim.x) {
+        cnt[e] = 0;
+        if (BIASED) rbuf[e] = clean_logit(__ldg(a.bias + e));
+    }
+    __syncthreads();
+    const size_t t = static_cast<size_t>(blockIdx.x) * blockDim.x + tid;
+    const bool live = t < n_tok, sig = a.score == HYMOE_SCORE_SIGMOID;
+    const T* row = logits + (live ? t : n_tok - 1) * ld;
+    const auto eight = [&](int e) { return *reinterpret_cast<const Vec<T, 8>*>(row + e); };
+    constexpr float delta = 0x1p-21f;
+    bool unsure_groups = false;
+
+    unsigned kept = kAll;
+    if constexpr (GROUPS) {
+        const bool two = a.group_score == HYMOE_GROUP_TOP2;
+        const int gs = E / a.n_group;
+        float* gv = rbuf + (BIASED ? E : 0) + tid;
+        float big = 0.f;
+        for (int g = 0; g < a.n_group; ++g) {
+            float b1 = -INFINITY, b2 = -INFINITY;
+            for (int e = g * gs; e < (g + 1) * gs; e += 8) {
+                float v[8];
+                eight_values<T, BIASED>(eight(e), rbuf + e, two, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    b2 = fmaxf(b2, fminf(b1, v[i]));
+                    b1 = fmaxf(b1, v[i]);
+                }
+            }
+            gv[g * blockDim.x] = two && b2 > -INFINITY ? b1 + b2 : b1;
+            if (b1 > -INFINITY) big = fmaxf(big, fabsf(b1) + (b2 > -INFINITY ? fabsf(b2) : 0.f));
+        }
+        kept = 0;
+        float lowest = INFINITY, first_out = -INFINITY;
+        for (int g = 0; g < a.n_group; ++g) {
+            const float v = gv[g * blockDim.x];
+            int better = 0;
+            for (int h = 0; h < a.n_group; ++h) {
+                const float o = gv[h * blockDim.x];
+                better += o > v || (o == v && h < g);
+            }
+            if (v > -INFINITY && better < a.topk_group) {
+                kept |= 1u << g;
+                lowest = fminf(lowest, v);
+            } else {
+                first_out = fmaxf(first_out, v);
+            }
+        }
+        if (BIASED || two) unsure_groups = first_out > -INFINITY && lowest - first_out <= 4.f * delta + 0x1p-21f * big;
+    }
+
+    unsigned l[8], rest = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l[i] = 0;
+    {
+        const int gs = GROUPS ? E / a.n_group : E;
+        Vec<T, 8> next = eight(0);
+        for (int e0 = 0, g = 0; e0 < E; e0 += gs, ++g) {
+            const bool keep = !GROUPS || (kept >> g & 1u);
+            for (int e = e0; e < e0 + gs; e += 8) {
+                const Vec<T, 8> raw = next;
+                if (e + 8 < E) next = eight(e + 8);
+                float v[8];
+                eight_values<T, BIASED>(raw, rbuf + e, false, v);
+                unsigned key[8];
+                const unsigned id = a.mask - e;  // its lowest three bits are set
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    key[i] = (order_key(BIASED ? v[i] : v[i] + 0.f) & ~a.mask) | (id ^ i);  // -0 is 0
+                    if (GROUPS && !keep) key[i] = 0;
+                }
+                sort_keys(key);
+                merge_best(l, key, rest);
+            }
+        }
+    }
+
+    float m = 0.f, sum = 0.f;
+    if (!BIASED && !sig && !a.norm) {  // a plain softmax: its sum, in trees of 8 and runs of 8 trees
+        m = -INFINITY;
+        for (int e = 0; e < E; e += 8) {
+            float v[8];
+            eight_values<T, false>(eight(e), nullptr, false, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, v[i]);
+        }
+        m = m == -INFINITY ? 0.f : m;
+        float part = 0.f;
+        for (int e = 0; e < E; e += 8) {
+            float v[8];
+            eight_values<T, false>(eight(e), nullptr, false, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = expf(v[i] - m);
+            part += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            if ((e & 56) == 56 || e + 8 == E) {
+                sum += part;
+                part = 0.f;
+            }
+        }
+    }
+
+    // the choices' logits, and whether their order is certain
+    bool unsure = unsure_groups;
+    int sel[8];
+    float z[8], w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const bool have = k < K && l[k] >= kOpenKey;
+        sel[k] = have ? static_cast<int>(a.mask - (l[k] & a.mask)) : -1;
+        z[k] = -INFINITY;
+        if (!have) continue;
+        if (BIASED || sizeof(T) == 4) {
+            z[k] = clean_logit(gate_value(row[sel[k]]));
+        } else {  // the key is the logit: its replaced bits were those of a 16-bit value
+            z[k] = fminf(key_value(l[k] & 0x80000000u ? l[k] & ~a.mask : l[k] | a.mask), kBig);
+            if (z[k] >= 3.38953138e38f) z[k] = clean_logit(gate_value(row[sel[k]]));  // +inf became FLT_MAX
+        }
+    }
+    if (BIASED || sizeof(T) == 4) {
+        bool close = false;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const unsigned after = k < 7 ? l[k < 7 ? k + 1 : 7] : rest;
+            const float lo = key_value(l[k] & ~a.mask), hi = key_value(after | a.mask);
+            const float slack = BIASED ? 2.f * delta + 0x1p-22f * fabsf(lo) : 0.f;
+            close = close || (k < K && after >= kOpenKey && !(lo - hi > slack));
+        }
+        if (close) {
+            float pv = 0.f, pb = 0.f, pz = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (sel[k] < 0) continue;
+                const unsigned after = k < 7 ? l[k < 7 ? k + 1 : 7] : rest;
+                const bool last = k + 1 == K && after >= kOpenKey;  // the best one left is next
+                if (BIASED) {
+                    const float b = rbuf[sel[k]], v = quick_sigmoid(z[k]) + b;
+                    if (k > 0) unsure = unsure || (!(pv - v > 2.f * delta + 0x1p-22f * fabsf(pv)) && !(pz == z[k] && pb == b));
+                    if (last) unsure = unsure || !(v - key_value(after | a.mask) > 2.f * delta + 0x1p-22f * fabsf(v));
+                    pv = v;
+                    pb = b;
+                } else {
+                    unsure = unsure || (k > 0 && pz < z[k]) || (last && ((l[k] ^ after) & ~a.mask) == 0);
+                }
+                pz = z[k];
+            }
+        }
+    }
+
+    if (a.norm) {
+        float mm = z[0], tot = 0.f;
+#pragma unroll
+        for (int k = 1; k < 8; ++k) mm = fmaxf(mm, z[k]);
+        if (sig) mm = fminf(mm, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            w[k] = 0.f;
+            if (sel[k] >= 0) w[k] = sig ? expf(fminf(z[k], 0.f) - mm) * quick_rcp(1.f + expf(-fabsf(z[k]))) : expf(z[k] - mm);
+            tot += w[k];
+        }
+        const float inv = tot > 0.f ? quick_rcp(tot) * a.scale : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] *= inv;
+    } else {
+        const float inv = sum > 0.f ? quick_rcp(sum) : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            w[k] = 0.f;
+            if (sel[k] >= 0) w[k] = (sig ? __fdiv_rn(1.f, 1.f + expf(-z[k])) : expf(z[k] - m) * inv) * a.scale;
+        }
+    }
+    if (live && !unsure) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (k >= K) break;
+            a.idx[t * K + k] = sel[k];
+            a.weights[t * K + k] = w[k];
+            if (a.counts != nullptr && sel[k] >= 0) atomicAdd(cnt + sel[k], 1);
+        }
+    }
+    // tokens in doubt, one after another by the whole warp: whichever groups are kept, the candidates'
+    // order is settled among themselves
+    int* c = a.counts != nullptr ? cnt : nullptr;
+    for (unsigned again = __ballot_sync(kAll, live && unsure); again != 0; again &= again - 1) {
+        const int who = __ffs(again) - 1, lane = tid & 31;
+        const size_t u = t - lane + who;
+        const T* row_u = logits + u * ld;
+        unsigned cand = 0, second = __shfl_sync(kAll, rest, who);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned v = __shfl_sync(kAll, l[i], who);
+            if (i <= K && lane == i) cand = v;
+            if (i == K + 1) second = v;
+        }
+        if (K == 8) {  // the ninth is the last candidate: look for the tenth
+            const unsigned keep = __shfl_sync(kAll, kept, who);
+            if (lane == 8) cand = second;
+            unsigned most = 0;
+#pragma unroll 1
+            for (int e = lane; e < E; e += 32) {
+                if (GROUPS && !(keep >> (e / (E / a.n_group)) & 1u)) continue;
+                const float zz = clean_logit(gate_value(row_u[e]));
+                const float v = !BIASED ? zz + 0.f : zz == -INFINITY ? zz : quick_sigmoid(zz) + rbuf[e];
+                const unsigned k = (order_key(v) & ~a.mask) | (a.mask - e);
+                if (k < second) most = max(most, k);
+            }
+            second = __reduce_max_sync(kAll, most);
+        }
+        int e = -2;
+        if (!__shfl_sync(kAll, unsure_groups, who)) e = settle(row_u, a, cand, second);
+        if (__any_sync(kAll, e == -2)) route_exact<T>(row_u, u, a, c);
+        else finish_choice(row_u, u, a, e, c);
+    }
+    if (a.counts != nullptr) {
+        __syncthreads();
+        for (int e = tid; e < E; e += blockDim.x)
+            if (cnt[e]) atomicAdd(a.counts + e, cnt[e]);  // whole numbers: any order gives the same
     }
 }
 
@@ -688,7 +1021,7 @@ inline bool row_runs(const void* p, size_t ld, size_t es, int E) {
     return entry_aligned(p, unit) && ld * es % unit == 0;
 }
 
-inline int gate_grid(size_t n_tok) {
+inline int gate_grid(size_t n_tok) {  // (one wave of what fits was 4 to 15% slower)
     const size_t chunks = (n_tok + kGateWarps - 1) / kGateWarps;
     return static_cast<int>(chunks < 148 * 8 ? chunks : 148 * 8);
 }
@@ -718,6 +1051,31 @@ cudaError_t launch_grad_epl(const T* x, size_t ld, T* d, size_t ldd, uint32_t n_
     return cudaGetLastError();
 }
 
+// Whether a thread per token takes the call: pieces of eight experts on 16-byte boundaries, at most
+// eight choices, nothing to sum over the experts for their order, and tokens enough to fill the GPU
+// with threads.  By warps against by threads, us, bf16: 128 experts, 6 choices, bias: 6.8 / 10.9 at
+// 8192 tokens, 10.8 / 9.6 at 16384, 60.6 / 27.7 at 131072; 64 experts, 8 choices: 4.2 / 4.9, 6.5 / 5.5,
+// 37.8 / 16.6; 512 experts, 8 choices: 9.0 / 16.2, 15.8 / 17.0, 114 / 81.  Groups cost a second pass
+// (256 experts, 8 groups): 44.9 / 46.4 at 32768, 136 / 88 at 131072.
+constexpr uint32_t kGateRowsMin = 16384, kGateRowsMinGroups = 65536;
+inline bool gate_by_rows(const hymoe_mat& x, size_t es, uint32_t n_tok, const GateArgs& a) {
+    const bool sig = a.score == HYMOE_SCORE_SIGMOID, two = a.n_group > 0 && a.group_score == HYMOE_GROUP_TOP2;
+    return n_tok >= (a.n_group > 0 ? kGateRowsMinGroups : kGateRowsMin) && a.K <= kRowsTopk && a.E % 8 == 0 && entry_aligned(x.data, 16) &&
+           static_cast<size_t>(x.ld) * es % 16 == 0 && a.scores == nullptr && (sig || (a.bias == nullptr && !two)) &&
+           (a.n_group == 0 || a.E / a.n_group % 8 == 0);
+}
+template <typename T>
+cudaError_t launch_gate_rows(const T* x, size_t ld, uint32_t n_tok, const GateArgs& a, cudaStream_t st) {
+    const int block = n_tok < 148u * 512u ? 32 : 128;
+    const size_t smem = sizeof(float) * ((a.bias ? a.E : 0) + static_cast<size_t>(a.n_group) * block);
+    const unsigned grid = (n_tok + block - 1) / block;
+    if (a.bias && a.n_group) gate_rows_kernel<T, true, true><<<grid, block, smem, st>>>(x, ld, n_tok, a);
+    else if (a.bias) gate_rows_kernel<T, true, false><<<grid, block, smem, st>>>(x, ld, n_tok, a);
+    else if (a.n_group) gate_rows_kernel<T, false, true><<<grid, block, smem, st>>>(x, ld, n_tok, a);
+    else gate_rows_kernel<T, false, false><<<grid, block, smem, st>>>(x, ld, n_tok, a);
+    return cudaGetLastError();
+}
+
 // EPL: the smallest of 2, 4, 8, 16 that holds the experts; runs where the rows allow it.
 template <typename T>
 cudaError_t launch_gate(const hymoe_mat& x, uint32_t n_tok, const GateArgs& a, cudaStream_t st) {
@@ -726,6 +1084,7 @@ cudaError_t launch_gate(const hymoe_mat& x, uint32_t n_tok, const GateArgs& a, c
                      (a.n_group == 0 || 32 % a.n_group == 0);
     const T* p = static_cast<const T*>(x.data);
     const size_t ld = static_cast<size_t>(x.ld);
+    if (gate_by_rows(x, sizeof(T), n_tok, a)) return launch_gate_rows<T>(p, ld, n_tok, a, st);
     auto go = [&](auto kern_run, auto kern_spread) { return run ? kern_run(p, ld, n_tok, a, st) : kern_spread(p, ld, n_tok, a, st); };
     if (a.E <= 64) return go(launch_gate_epl<T, 2, true>, launch_gate_epl<T, 2, false>);
     if (a.E <= 128) return go(launch_gate_epl<T, 4, true>, launch_gate_epl<T, 4, false>);

@@ -32,7 +32,7 @@ __global__ __launch_bounds__(32 * kRouterTok) void route_block_kernel(const floa
                                                   a, bias, gbuf[warp], sel, w))
             put_choice(a, t, sel, w, cnt);
         else
-            route_exact<float, 2, SIG>(row, t, a, cnt);
+            route_exact<float>(row, t, a, cnt);
     }
     __syncthreads();
     if (threadIdx.x < static_cast<unsigned>(a.E)) chunk_counts[static_cast<size_t>(blockIdx.x) * a.E + threadIdx.x] = cnt[threadIdx.x];
