@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
     };
     fetch(t_lo);
     for (int i = tid; i < W * nb; i += kPlanThreads) cnt[i] = 0;
-    for (int i = tid; i < p.max_tiles * (p.tile_rows / kAdRows); i += kPlanThreads) p.counters[i] = 0u;
+    for (int i = tid; i < (p.items ? 2 : 1) * p.max_tiles * (p.tile_rows / kAdRows); i += kPlanThreads) p.counters[i] = 0u;
     __syncthreads();
     int* mine = cnt + (warp < W ? warp : 0) * nb;
     auto rate = [&](int i) {
@@ -188,7 +188,7 @@ cudaError_t launch_plan_adapt(const int* ids, int T, int n, const AdaptPlan& p, 
 
 // The workspace: every part starts on 256 bytes.
 struct AdaptLayout {
-    size_t perm, tiles, items, pieces, amax, lists, counters, low, low2, low_part, part, slots, low16[2], bytes;
+    size_t perm, tiles, items, pieces, amax, lists, counters, low, low2, low_part, low_part2, part, slots, low16[2], bytes;
     int tile_rows, max_tiles, spare_tiles, max_items;
 };
 // (the sizes do not depend on tile_rows)
@@ -211,14 +211,16 @@ AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward, int 
     l.lists = take(4 * sizeof(int));
     l.perm = take(T * sizeof(int));
     l.tiles = take(tiles64 * sizeof(int4));
-    l.counters = take(half_tiles * sizeof(unsigned));
+    l.counters = take((backward ? 2 : 1) * half_tiles * sizeof(unsigned));
     l.low = take(T * adapt_rp(ad->rank) * sizeof(float));
     const size_t shared_tiles = half_tiles * kAdMaxSplits;
-    l.low_part = take((shared_tiles < kAdMaxSlots ? shared_tiles : kAdMaxSlots) * kAdRows * adapt_rp(ad->rank) * sizeof(float));
+    const size_t low_part = (shared_tiles < kAdMaxSlots ? shared_tiles : kAdMaxSlots) * kAdRows * adapt_rp(ad->rank) * sizeof(float);
+    l.low_part = take(low_part);
     if (backward) {
         l.items = take(static_cast<size_t>(l.max_items) * sizeof(int4));
         l.pieces = take((n + 1) * sizeof(int));
         l.amax = take(2 * n * sizeof(unsigned));
+        l.low_part2 = take(low_part);
         l.low2 = take(T * adapt_rp(ad->rank) * sizeof(float));
         for (size_t& at : l.low16) at = take(T > kTcRows ? T * adapt_parts(adapt_rp(ad->rank)) * 2 : 0);
         l.slots = 2 * long_pieces;  // an adapter of c tokens in p > 1 pieces: p < 2 c / chunk
@@ -364,8 +366,8 @@ bool weights_tma(const hymoe_adapters* ad) {
            entry_aligned(ad->b, 16);
 }
 
-cudaError_t run_low(const AdaptPlan& plan, const hymoe_mat& x, const void* w, int type_w, bool trans, const float* scale,
-                    float* low, float* part, unsigned* amax, int R, int K, int T, int n, bool tc, int n_sms, cudaStream_t st) {
+AdaptLow low_args(const AdaptPlan& plan, const hymoe_mat& x, const void* w, bool trans, const float* scale, float* low,
+                  float* part, unsigned* amax, int R, int K) {
     AdaptLow a{};
     a.plan = plan;
     a.x = x.data;
@@ -377,16 +379,18 @@ cudaError_t run_low(const AdaptPlan& plan, const hymoe_mat& x, const void* w, in
     a.amax = amax;
     a.K = K;
     a.R = R;
-    if (tc) {
-        AdaptMaps m;
-        if (!encode_rows(&m.rows, x, T, K, kTcRows) ||
-            !(trans ? encode_weights(&m, w, type_w, n, K, R, 64) : encode_weights(&m, w, type_w, n, R, K, adapt_rp(R))))
-            return cudaErrorInvalidValue;
-        return launch_adapt_low_tc(m, a, type_w, trans, n_sms, st);
-    }
     a.vec_x = rows_vec(x.data, a.ldx, elem_bytes(x.type));
     a.vec_w = rows_vec(w, trans ? R : K, 2);
-    return launch_adapt_low(a, x.type, type_w, trans, n_sms, st);
+    return a;
+}
+
+cudaError_t run_low(const AdaptLow& a, const hymoe_mat& x, int type_w, bool trans, int T, int n, bool tc, int n_sms, cudaStream_t st) {
+    if (!tc) return launch_adapt_low(a, x.type, type_w, trans, n_sms, st);
+    AdaptMaps m;
+    if (!encode_rows(&m.rows, x, T, a.K, kTcRows) ||
+        !(trans ? encode_weights(&m, a.w, type_w, n, a.K, a.R, 64) : encode_weights(&m, a.w, type_w, n, a.R, a.K, adapt_rp(a.R))))
+        return cudaErrorInvalidValue;
+    return launch_adapt_low_tc(m, a, type_w, trans, n_sms, st);
 }
 
 cudaError_t run_wide(const AdaptPlan& plan, const float* low, const void* w, int type_w, bool trans, const hymoe_mat* base,
@@ -509,7 +513,7 @@ extern "C" hymoe_status hymoe_adapt(const hymoe_adapters* ad, const hymoe_mat* x
     float* low = reinterpret_cast<float*>(ws + l.low);
     float* low_part = reinterpret_cast<float*>(ws + l.low_part);
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
-    if (e == cudaSuccess) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low, low_part, nullptr, R, static_cast<int>(I), t, n, tc_low, n_sms, st);
+    if (e == cudaSuccess) e = run_low(low_args(plan, *x, ad->a, false, ad->scale, low, low_part, nullptr, R, static_cast<int>(I)), *x, ad->type, false, t, n, tc_low, n_sms, st);
     if (e == cudaSuccess) e = run_wide(plan, low, ad->b, ad->type, false, base, *out, R, static_cast<int>(O), t, n, tc_wide, n_sms, st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt: kernel launch failed");
     return HYMOE_OK;
@@ -576,14 +580,20 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
     const AdaptPlan plan = plan_in(l, ws, true);
     float* low_dy = reinterpret_cast<float*>(ws + l.low);
     float* low_x = reinterpret_cast<float*>(ws + l.low2);
-    float* low_part = reinterpret_cast<float*>(ws + l.low_part);
+    float *low_part = reinterpret_cast<float*>(ws + l.low_part), *low_part2 = reinterpret_cast<float*>(ws + l.low_part2);
     float* part = reinterpret_cast<float*>(ws + l.part);
     const int i = static_cast<int>(I), o = static_cast<int>(O);
     unsigned* amax = tc_grad && ad->type == HYMOE_TYPE_F16 ? plan.amax : nullptr;
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
-    if (e == cudaSuccess && (dx || da)) e = run_low(plan, *dy, ad->b, ad->type, true, ad->scale, low_dy, low_part, amax, R, o, t, n, tc_dy, n_sms, st);
+    // the narrow products, dy's for dx and da and x's for db; as one launch where both are mma.sync's
+    const AdaptLow by_dy = low_args(plan, *dy, ad->b, true, ad->scale, low_dy, low_part, amax, R, o);
+    AdaptLow by_x = low_args(plan, *x, ad->a, false, ad->scale, low_x, low_part2, amax ? amax + n : nullptr, R, i);
+    by_x.plan.counters += l.max_tiles * (l.tile_rows / kAdRows);
+    const bool pair = (dx || da) && db && !tc_dy && !tc_x && x->type == dy->type;
+    if (e == cudaSuccess && pair) e = launch_adapt_lows(by_dy, by_x, x->type, ad->type, n_sms, st);
+    if (e == cudaSuccess && !pair && (dx || da)) e = run_low(by_dy, *dy, ad->type, true, t, n, tc_dy, n_sms, st);
     if (e == cudaSuccess && dx) e = run_wide(plan, low_dy, ad->a, ad->type, true, base, *dx, R, i, t, n, tc_dx, n_sms, st);
-    if (e == cudaSuccess && db) e = run_low(plan, *x, ad->a, ad->type, false, ad->scale, low_x, low_part, amax ? amax + n : nullptr, R, i, t, n, tc_x, n_sms, st);
+    if (e == cudaSuccess && !pair && db) e = run_low(by_x, *x, ad->type, false, t, n, tc_x, n_sms, st);
     // dA from x and dy's narrow rows, dB from dy and x's; long adapters in pieces
     AdaptGradPair grads;
     grads.g[0] = grad_args(plan, low_dy, *x, da, part, n, R, i, 1, i);
@@ -597,9 +607,12 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
                 e = cudaErrorInvalidValue;
         }
         if (e == cudaSuccess && (da || db)) e = launch_adapt_grad_tc(grads, ad->type, st);
+    } else if (x->type == dy->type) {
+        if (e == cudaSuccess && (da || db)) e = launch_adapt_grad(grads.g[0], grads.g[1], x->type, st);
     } else {
-        if (e == cudaSuccess && da) e = launch_adapt_grad(grads.g[0], x->type, st);
-        if (e == cudaSuccess && db) e = launch_adapt_grad(grads.g[1], dy->type, st);
+        const AdaptGrad none{};
+        if (e == cudaSuccess && da) e = launch_adapt_grad(grads.g[0], none, x->type, st);
+        if (e == cudaSuccess && db) e = launch_adapt_grad(grads.g[1], none, dy->type, st);
     }
     if (e == cudaSuccess && (da || db) && t > adapt_chunk(t, n)) e = launch_adapt_join(grads.g[0], grads.g[1], st);
     if (e != cudaSuccess) return entry_fail(HYMOE_ERR_CUDA, "hymoe_adapt_backward: kernel launch failed");

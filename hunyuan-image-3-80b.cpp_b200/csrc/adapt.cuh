@@ -64,7 +64,7 @@ struct AdaptPlan {
                      // [3] tiles that have an adapter (the first ones)
     int tile_rows;   // 64 or 128
     unsigned* amax;  // gradients of fp16 rows: [2 n] largest |low| of every adapter (bits), of dy's then of x's
-    unsigned* counters;  // [max_tiles] CTAs of a tile that have left their partial sums (0 between launches)
+    unsigned* counters;  // [max_tiles] (backward: twice) CTAs of a tile that have left their partial sums (0 between launches)
     int max_tiles, max_items;
     int spare_tiles; // of max_tiles, those for adapters' last, part-filled tiles
 };
@@ -121,8 +121,11 @@ cudaError_t launch_adapt_decode(const AdaptDecode& d, int type_x, int type_w, in
 // type_x: HYMOE_TYPE_F32 or type_w; trans: the weight matrix has the rank as its fast dimension
 // (low) or the columns as its fast dimension (wide).
 cudaError_t launch_adapt_low(const AdaptLow& a, int type_x, int type_w, bool trans, int n_sms, cudaStream_t st);
+// Two narrow products as one launch: trans and then not, x of one type.
+cudaError_t launch_adapt_lows(const AdaptLow& a, const AdaptLow& b, int type_x, int type_w, int n_sms, cudaStream_t st);
 cudaError_t launch_adapt_wide(const AdaptWide& a, int type_y, int type_w, bool trans, int n_sms, cudaStream_t st);
-cudaError_t launch_adapt_grad(const AdaptGrad& a, int type_x, cudaStream_t st);
+// One or two gradients over long rows of one type (g == nullptr: none).
+cudaError_t launch_adapt_grad(const AdaptGrad& a, const AdaptGrad& b, int type_x, cudaStream_t st);
 // Adds the pieces of long adapters in one or two gradients (g == nullptr: none).
 cudaError_t launch_adapt_join(const AdaptGrad& a, const AdaptGrad& b, cudaStream_t st);
 

@@ -4,9 +4,10 @@
 // A CTA takes 128 columns of the long rows and one item of the plan (an adapter's tokens, or a
 // piece of a long adapter's), 32 tokens at a time; the matrix pipe sums over the 32 tokens, and
 // the sums of the blocks are added in fp32 outside it: the pipe truncates what it adds, which over
-// a thousand tokens cost 5e-6 of the result instead of 1e-6.  low is held in two bf16 parts beside
-// bf16 rows (2^-17 of each value), in two tf32 parts beside others.  Items that are pieces of one
-// adapter write partial sums, which a second kernel adds in order.
+// a thousand tokens cost 5e-6 of the result instead of 1e-6.  low is held in three bf16 parts beside
+// bf16 rows (all its bits; two left 2.4e-6 of a gradient), in two tf32 parts beside others.  Both
+// gradients are one launch (a launch after the other took 10 us more for 77 tokens).  Items that are
+// pieces of one adapter write partial sums, which a second kernel adds in order.
 #include <type_traits>
 
 #include "adapt.cuh"
@@ -29,16 +30,18 @@ struct GradTile {
     static constexpr bool kParts = std::is_same<X, __nv_bfloat16>::value;  // 16-bit parts of low
     static constexpr int kPRow = ad_pad16(RP * 2);
     static constexpr int kPBytes = kGradTok * kPRow;  // one part of a block
-    static constexpr int kSmem = kStage * kGradStages + (kParts ? 2 * kPBytes : 0);
+    static constexpr int kSmem = kStage * kGradStages + (kParts ? 3 * kPBytes : 0);
 };
 
 template <typename X, int RP>
-__global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant__ AdaptGrad a) {
+__global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant__ AdaptGrad a0,
+                                                           const __grid_constant__ AdaptGrad a1) {
     using L = GradTile<X, RP>;
     extern __shared__ __align__(128) char smem[];
     griddep_wait();
     griddep_launch_dependents();
-    if (static_cast<int>(blockIdx.x) >= a.plan.n_lists[2]) return;
+    const AdaptGrad& a = blockIdx.z == 0 ? a0 : a1;
+    if (a.g == nullptr || static_cast<int>(blockIdx.y) * kAdGradCols >= a.M || static_cast<int>(blockIdx.x) >= a.plan.n_lists[2]) return;
     const int4 item = a.plan.items[blockIdx.x];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int m0 = blockIdx.y * kAdGradCols;
@@ -103,12 +106,14 @@ __global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant_
 #pragma unroll
             for (int i = 0; i < kGradTok * RP / 4 / kAdThreads; ++i) {
                 const int p = tid + i * kAdThreads, r = p / (RP / 4), c = p % (RP / 4) * 4;
-                const float4 v = *reinterpret_cast<const float4*>(ls + r * (RP + 4) + c);
-                const uint32_t h0 = AdType<X>::pack(v.x, v.y), h1 = AdType<X>::pack(v.z, v.w);
-                const float2 b0 = AdType<X>::unpack(h0), b1 = AdType<X>::unpack(h1);
-                *reinterpret_cast<uint2*>(ps + r * L::kPRow + c * 2) = make_uint2(h0, h1);
-                *reinterpret_cast<uint2*>(ps + L::kPBytes + r * L::kPRow + c * 2) =
-                    make_uint2(AdType<X>::pack(v.x - b0.x, v.y - b0.y), AdType<X>::pack(v.z - b1.x, v.w - b1.y));
+                float4 v = *reinterpret_cast<const float4*>(ls + r * (RP + 4) + c);
+#pragma unroll
+                for (int part = 0; part < 3; ++part) {
+                    const uint32_t h0 = AdType<X>::pack(v.x, v.y), h1 = AdType<X>::pack(v.z, v.w);
+                    const float2 b0 = AdType<X>::unpack(h0), b1 = AdType<X>::unpack(h1);
+                    *reinterpret_cast<uint2*>(ps + part * L::kPBytes + r * L::kPRow + c * 2) = make_uint2(h0, h1);
+                    v = make_float4(v.x - b0.x, v.y - b0.y, v.z - b1.x, v.w - b1.y);
+                }
             }
             __syncthreads();
 #pragma unroll
@@ -121,7 +126,7 @@ __global__ __launch_bounds__(kAdThreads) void grad_kernel(const __grid_constant_
 #pragma unroll
                 for (int j = 0; j < RP / 16; ++j)
 #pragma unroll
-                    for (int part = 1; part >= 0; --part) {
+                    for (int part = 2; part >= 0; --part) {
                         uint32_t bf[4];
                         ldsm4_t(bf, smem_u32(ps) + part * L::kPBytes + (kk * 16 + (lane & 15)) * L::kPRow + (j * 16 + (lane >> 4) * 8) * 2);
 #pragma unroll
@@ -233,21 +238,23 @@ __global__ __launch_bounds__(256) void grad_join_kernel(const __grid_constant__ 
 }
 
 template <typename X, int RP>
-cudaError_t launch_t(const AdaptGrad& a, cudaStream_t st) {
+cudaError_t launch_t(const AdaptGrad& a, const AdaptGrad& b, cudaStream_t st) {
     using L = GradTile<X, RP>;
     auto kern = grad_kernel<X, RP>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
-    return launch_kernel(true, kern, dim3(a.plan.max_items, (a.M + kAdGradCols - 1) / kAdGradCols), dim3(kAdThreads), L::kSmem, st, a);
+    const int ma = a.g ? a.M : 0, mb = b.g ? b.M : 0;
+    return launch_kernel(true, kern, dim3(a.plan.max_items, ((ma > mb ? ma : mb) + kAdGradCols - 1) / kAdGradCols, b.g ? 2 : 1),
+                         dim3(kAdThreads), L::kSmem, st, a, b);
 }
 
 template <typename X>
-cudaError_t launch_x(const AdaptGrad& a, cudaStream_t st) {
+cudaError_t launch_x(const AdaptGrad& a, const AdaptGrad& b, cudaStream_t st) {
     switch (adapt_rp(a.R)) {
-        case 16: return launch_t<X, 16>(a, st);
-        case 32: return launch_t<X, 32>(a, st);
-        case 64: return launch_t<X, 64>(a, st);
-        default: return launch_t<X, 128>(a, st);
+        case 16: return launch_t<X, 16>(a, b, st);
+        case 32: return launch_t<X, 32>(a, b, st);
+        case 64: return launch_t<X, 64>(a, b, st);
+        default: return launch_t<X, 128>(a, b, st);
     }
 }
 
@@ -259,10 +266,10 @@ cudaError_t launch_adapt_join(const AdaptGrad& a, const AdaptGrad& b, cudaStream
     return launch_kernel(true, grad_join_kernel, dim3(static_cast<unsigned>(blk < 512 ? blk : 512), a.n, 2), dim3(256), 0, st, a, b);
 }
 
-cudaError_t launch_adapt_grad(const AdaptGrad& a, int type_x, cudaStream_t st) {
-    if (type_x == HYMOE_TYPE_F32) return launch_x<float>(a, st);
-    if (type_x == HYMOE_TYPE_F16) return launch_x<__half>(a, st);
-    return launch_x<__nv_bfloat16>(a, st);
+cudaError_t launch_adapt_grad(const AdaptGrad& a, const AdaptGrad& b, int type_x, cudaStream_t st) {
+    if (type_x == HYMOE_TYPE_F32) return launch_x<float>(a, b, st);
+    if (type_x == HYMOE_TYPE_F16) return launch_x<__half>(a, b, st);
+    return launch_x<__nv_bfloat16>(a, b, st);
 }
 
 }  // namespace hymoe

@@ -27,12 +27,8 @@ struct LowTile {
 };
 
 template <typename X, typename W, int RP, bool TRANS>
-__global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void low_kernel(
-    const __grid_constant__ AdaptLow a, int S) {
+__device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
     using L = LowTile<X, W, RP, TRANS>;
-    extern __shared__ __align__(128) char smem[];
-    griddep_wait();
-    griddep_launch_dependents();
     const int tile_id = blockIdx.x / S, rank = blockIdx.x % S;
     const int4 tile = ad_part_tile(a.plan, tile_id);
     if (tile.x < 0) return;  // none, or rows without an adapter
@@ -220,6 +216,52 @@ __global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void 
 }
 
 template <typename X, typename W, int RP, bool TRANS>
+__global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void low_kernel(
+    const __grid_constant__ AdaptLow a, int S) {
+    extern __shared__ __align__(128) char smem[];
+    griddep_wait();
+    griddep_launch_dependents();
+    low_tile<X, W, RP, TRANS>(a, S, smem);
+}
+
+// Grid (tiles x the larger S, 2).
+template <typename X, typename W, int RP>
+__global__ __launch_bounds__(kAdThreads) void low_pair_kernel(const __grid_constant__ AdaptLow a, int Sa,
+                                                              const __grid_constant__ AdaptLow b, int Sb, int tiles) {
+    extern __shared__ __align__(128) char smem[];
+    griddep_wait();
+    griddep_launch_dependents();
+    if (static_cast<int>(blockIdx.x) >= tiles * (blockIdx.y == 0 ? Sa : Sb)) return;
+    if (blockIdx.y == 0) low_tile<X, W, RP, true>(a, Sa, smem);
+    else low_tile<X, W, RP, false>(b, Sb, smem);
+}
+
+template <typename X, typename W, int RP>
+cudaError_t launch_pair(const AdaptLow& a, const AdaptLow& b, int n_sms, cudaStream_t st) {
+    using La = LowTile<X, W, RP, true>;
+    using Lb = LowTile<X, W, RP, false>;
+    constexpr int smem = La::kSmem > Lb::kSmem ? La::kSmem : Lb::kSmem;
+    constexpr int per_sm = La::kPerSm < Lb::kPerSm ? La::kPerSm : Lb::kPerSm;
+    auto kern = low_pair_kernel<X, W, RP>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const int tiles = a.plan.max_tiles * (a.plan.tile_rows / kAdRows);
+    const int Sa = adapt_splits(tiles, a.K, per_sm * n_sms / 2), Sb = adapt_splits(tiles, b.K, per_sm * n_sms / 2);
+    return launch_kernel(true, kern, dim3(static_cast<unsigned>(tiles) * (Sa > Sb ? Sa : Sb), 2), dim3(kAdThreads), smem, st, a, Sa,
+                         b, Sb, tiles);
+}
+
+template <typename X, typename W>
+cudaError_t launch_pair_x(const AdaptLow& a, const AdaptLow& b, int n_sms, cudaStream_t st) {
+    switch (adapt_rp(a.R)) {
+        case 16: return launch_pair<X, W, 16>(a, b, n_sms, st);
+        case 32: return launch_pair<X, W, 32>(a, b, n_sms, st);
+        case 64: return launch_pair<X, W, 64>(a, b, n_sms, st);
+        default: return launch_pair<X, W, 128>(a, b, n_sms, st);
+    }
+}
+
+template <typename X, typename W, int RP, bool TRANS>
 cudaError_t launch_t(const AdaptLow& a, int n_sms, cudaStream_t st) {
     using L = LowTile<X, W, RP, TRANS>;
     auto kern = low_kernel<X, W, RP, TRANS>;
@@ -241,6 +283,14 @@ cudaError_t launch_x(const AdaptLow& a, bool trans, int n_sms, cudaStream_t st) 
 }
 
 }  // namespace
+
+cudaError_t launch_adapt_lows(const AdaptLow& a, const AdaptLow& b, int type_x, int type_w, int n_sms, cudaStream_t st) {
+    if (type_w == HYMOE_TYPE_F16)
+        return type_x == HYMOE_TYPE_F32 ? launch_pair_x<float, __half>(a, b, n_sms, st)
+                                        : launch_pair_x<__half, __half>(a, b, n_sms, st);
+    return type_x == HYMOE_TYPE_F32 ? launch_pair_x<float, __nv_bfloat16>(a, b, n_sms, st)
+                                    : launch_pair_x<__nv_bfloat16, __nv_bfloat16>(a, b, n_sms, st);
+}
 
 cudaError_t launch_adapt_low(const AdaptLow& a, int type_x, int type_w, bool trans, int n_sms, cudaStream_t st) {
     if (type_w == HYMOE_TYPE_F16)
