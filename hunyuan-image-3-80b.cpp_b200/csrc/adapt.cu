@@ -235,7 +235,7 @@ AdaptPlan plan_in(const AdaptLayout& l, char* ws, bool backward) {
     p.items = backward ? reinterpret_cast<int4*>(ws + l.items) : nullptr;
     p.pieces = backward ? reinterpret_cast<int*>(ws + l.pieces) : nullptr;
     p.amax = backward ? reinterpret_cast<unsigned*>(ws + l.amax) : nullptr;
-    p.n_lists = reinterpret_cast<int*>(ws + l.lists);
+    p.err = p.n_lists = reinterpret_cast<int*>(ws + l.lists);  // the workspace's first word
     p.counters = reinterpret_cast<unsigned*>(ws + l.counters);
     p.tile_rows = l.tile_rows;
     p.max_tiles = l.max_tiles;
@@ -450,6 +450,12 @@ bool all_on(int dev, std::initializer_list<const void*> ps) {
 extern "C" hymoe_status hymoe_adapt(const hymoe_adapters* ad, const hymoe_mat* x, const int32_t* ids, uint32_t n_tokens,
                                     const hymoe_mat* base, const hymoe_mat* out, void* workspace,
                                     size_t workspace_bytes, void* stream) {
+    return adapt_call(ad, x, ids, n_tokens, base, out, workspace, workspace_bytes, stream, nullptr);
+}
+
+hymoe_status hymoe::adapt_call(const hymoe_adapters* ad, const hymoe_mat* x, const int32_t* ids, uint32_t n_tokens,
+                               const hymoe_mat* base, const hymoe_mat* out, void* workspace, size_t workspace_bytes,
+                               void* stream, int* err) {
     set_thread_error("");
     if (const char* why = adapters_problem(ad)) return entry_fail(HYMOE_ERR_INVALID_ARG, why);
     if (n_tokens == 0) return HYMOE_OK;
@@ -509,7 +515,8 @@ extern "C" hymoe_status hymoe_adapt(const hymoe_adapters* ad, const hymoe_mat* x
     const bool tc_wide = aligned && rows_tma(out, O) && (!base || rows_tma(base, O));
     const AdaptLayout l = adapt_layout(ad, T, false, tc_low || tc_wide ? kTcRows : kAdRows);
     char* ws = static_cast<char*>(workspace);
-    const AdaptPlan plan = plan_in(l, ws, false);
+    AdaptPlan plan = plan_in(l, ws, false);
+    if (err) plan.err = err;
     float* low = reinterpret_cast<float*>(ws + l.low);
     float* low_part = reinterpret_cast<float*>(ws + l.low_part);
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);

@@ -60,7 +60,8 @@ struct AdaptPlan {
     int4* tiles;     // {adapter or -1, first row, rows, 0} of at most tile_rows rows
     int4* items;     // gradients: {adapter, first row, rows, partial slot or -1}; every adapter has one
     int* pieces;     // gradients: [n + 1] first item of each adapter (items are adapter-major)
-    int* n_lists;    // [0] status (0, or DevErr bits of a wait that expired), [1] tiles, [2] items,
+    int* err;        // DevErr bits of a bounded wait that expired: n_lists, or the caller's word
+    int* n_lists;    // [0] status, [1] tiles, [2] items,
                      // [3] tiles that have an adapter (the first ones)
     int tile_rows;   // 64 or 128
     unsigned* amax;  // gradients of fp16 rows: [2 n] largest |low| of every adapter (bits), of dy's then of x's

@@ -24,7 +24,11 @@ struct LtcTile {
     static constexpr int kStages = kN == 128 ? 3 : 4;
     static constexpr int kSmem = 1024 + kStages * (kA + kB);
     static_assert(kStages * (kA + kB) >= kLtcRows * (RP + 4) * 4, "the stages hold the partial sums");
-    static constexpr int kCols = kN < 32 ? 32 : kN;
+    // Accumulators that take the columns in turn: the pipe truncates what it adds, 4e-8 of the running
+    // sum each time (over 2048 columns that made 2e-6 of low; a quarter with four).
+    static constexpr int kSets = kN == 128 ? 2 : 4;
+    static constexpr int kSet = kN < 32 ? 32 : kN;  // columns of one
+    static constexpr int kCols = kSets * kSet;      // two CTAs share the 512 of an SM
 };
 
 template <typename W, int RP, bool TRANS>
@@ -65,7 +69,7 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
     const int nk = (a.K + 63) / 64;
     const int k_lo = static_cast<int>(static_cast<int64_t>(nk) * rank / S);
     const int k_hi = static_cast<int>(static_cast<int64_t>(nk) * (rank + 1) / S);
-    int* err = a.plan.n_lists;  // the status word
+    int* err = a.plan.err;  // the status word
 
     if (warp == 0) {
         if (lane == 0) {
@@ -101,9 +105,9 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
                 const uint32_t sa = smem_u32(smem + s * (L::kA + L::kB)), sb = sa + L::kA;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                    mma_f16_ss(tmem, sw128_kmajor_desc(sa + kk * 32),
+                    mma_f16_ss(tmem + kk % L::kSets * L::kSet, sw128_kmajor_desc(sa + kk * 32),
                                TRANS ? sw128_mnmajor_desc(sb + kk * 2048, 8192) : sw128_kmajor_desc(sb + kk * 32), idesc,
-                               (it | kk) != 0 ? 1u : 0u);
+                               it != 0 || kk >= L::kSets ? 1u : 0u);
                 mma_commit(&empty[s]);
             }
             mma_commit(&done);
@@ -146,12 +150,19 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
         float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
         for (int c = 0; c < RP; c += 32) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, v);
-            tmem_ld_wait();
+            constexpr int kNow = RP < 32 ? RP : 32;
+            float sum[kNow];
 #pragma unroll
-            for (int j = 0; j < (RP < 32 ? RP : 32); j += 4)
-                *reinterpret_cast<uint4*>(red + r * (RP + 4) + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            for (int set = 0; set < L::kSets; ++set) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + set * L::kSet + c, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < kNow; ++j) sum[j] = set == 0 ? __uint_as_float(v[j]) : sum[j] + __uint_as_float(v[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < kNow; j += 4)
+                *reinterpret_cast<float4*>(red + r * (RP + 4) + c + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
         }
         tc_fence_before();
         if (S == 1) {

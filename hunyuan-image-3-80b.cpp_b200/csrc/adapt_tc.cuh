@@ -27,8 +27,10 @@ cudaError_t launch_adapt_low_tc(const AdaptMaps& maps, const AdaptLow& a, int ty
 cudaError_t launch_adapt_wide_tc(const AdaptMaps& maps, const AdaptWide& a, int type_y, int type_w, bool trans, int n_sms,
                                  cudaStream_t st);
 
-// 16-bit values of a row of low in three parts, in whole panels of 64.
-__host__ __device__ constexpr int adapt_parts(int rp) { return (3 * rp + 63) / 64 * 64; }
+// 16-bit values of a row of low in three parts: the first, in whole panels of 64, and the other two
+// from adapt_rest on.
+__host__ __device__ constexpr int adapt_rest(int rp) { return rp < 64 ? 64 : rp; }
+__host__ __device__ constexpr int adapt_parts(int rp) { return adapt_rest(rp) + (rp < 32 ? 64 : 2 * rp); }
 
 // Both gradients of a call (either may be absent: g[i].g == nullptr; plan, R and n are always set).
 struct AdaptGradPair {

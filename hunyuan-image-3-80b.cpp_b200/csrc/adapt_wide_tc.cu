@@ -97,7 +97,7 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
     // narrow product, only its readers do.
     if (warp >= 2 && warp < 10) griddep_wait();
     griddep_launch_dependents();
-    int* err = a.plan.n_lists;
+    int* err = a.plan.err;
     const int n_blk = (a.N + L::kCols - 1) / L::kCols;
     const int n_tiles = a.plan.n_lists[a.in_place ? 3 : 1];  // in place, rows without an adapter stay
     const int64_t units = static_cast<int64_t>(n_tiles) * n_blk;

@@ -55,4 +55,9 @@ inline EntrySpan entry_span(const hymoe_mat* m, uint32_t rows, uint32_t cols) {
 }
 inline bool entry_overlap(EntrySpan a, EntrySpan b) { return a.lo < b.hi && b.lo < a.hi; }
 
+// hymoe_adapt with the word that an expired device-side wait sets (nullptr: the workspace's first).
+hymoe_status adapt_call(const hymoe_adapters* ad, const hymoe_mat* x, const int32_t* ids, uint32_t n_tokens,
+                        const hymoe_mat* base, const hymoe_mat* out, void* workspace, size_t workspace_bytes,
+                        void* stream, int* err);
+
 }  // namespace hymoe

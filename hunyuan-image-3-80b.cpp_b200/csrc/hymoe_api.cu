@@ -46,6 +46,7 @@
 
 #include "../../include/hymoe.h"
 #include "common.cuh"
+#include "entry.h"
 #include "kernels.h"
 
 using namespace hymoe;
@@ -2058,7 +2059,7 @@ static hymoe_status forward_call(hymoe_ctx* c, uint32_t layer, const float* x, c
         // the sums before the SwiGLU, down's onto its result.
         auto adapt = [&](const hymoe_adapters* ad, __half* in, int n_in, const float* base, float* res, int n_out) -> hymoe_status {
             const hymoe_mat mx{in, HYMOE_TYPE_F16, n_in}, mb{const_cast<float*>(base), HYMOE_TYPE_F32, n_out}, mo{res, HYMOE_TYPE_F32, n_out};
-            const hymoe_status sa = hymoe_adapt(ad, &mx, ids, n_tokens, base ? &mb : nullptr, &mo, c->ad_ws, c->ad_ws_bytes, st);
+            const hymoe_status sa = adapt_call(ad, &mx, ids, n_tokens, base ? &mb : nullptr, &mo, c->ad_ws, c->ad_ws_bytes, st, c->err_word);
             return sa == HYMOE_OK ? sa : c->fail(sa, "adapters: %s", hymoe_last_error(nullptr));
         };
         if (ad_gu) {

@@ -4,6 +4,7 @@ and without an adapter beside one another, widths that end inside a tile, gradie
 in pieces.  The tolerances are those of test_gpu_adapt.py."""
 import pytest
 
+import hymoe
 from test_gpu_adapt import Problem, check, near
 
 pytestmark = pytest.mark.gpu
@@ -151,3 +152,27 @@ def test_other_types_beside_the_weights():
     for x, y in (("f32", "bf16"), ("bf16", "f32")):
         p = with_ids(runs(*MIXES["both"]), 256, 264, 16, 4, x=x, y=y)
         check(p)
+
+
+@pytest.mark.parametrize("T", [100, 300])
+def test_workspace_as_it_comes(T):
+    """Whatever the workspace holds before the call; its first word says afterwards that no wait expired."""
+    p = Problem(T, 256, 264, 16, 4)
+    ad = p.adapters
+    want, grads = ad.apply(p.x, p.ids, base=p.base), ad.backward(p.x, p.dy, p.ids, base=p.base_x)
+    mat = lambda t: hymoe.Mat(t.data_ptr(), 30, t.shape[1])
+    for fill in (0, 0xFF, 0x7F):
+        ws = torch.full((ad._workspace_bytes(T, True),), fill, dtype=torch.uint8, device="cuda")
+        out = torch.full_like(want, float("nan"))
+        n = ad._workspace_bytes(T, False)
+        stream = torch.cuda.current_stream().cuda_stream
+        assert ad.L.hymoe_adapt(ad._spec, mat(p.x), p.ids.data_ptr(), T, mat(p.base), mat(out), ws.data_ptr(), n, stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and not bool(ws[:4].any()) and bool((ws[n:] == fill).all())
+        ws.fill_(fill)
+        dx, da, db = (torch.full_like(grads[k], float("nan")) for k in ("dx", "da", "db"))
+        assert ad.L.hymoe_adapt_backward(ad._spec, mat(p.x), mat(p.dy), p.ids.data_ptr(), T, mat(p.base_x), mat(dx), da.data_ptr(),
+                                         db.data_ptr(), ws.data_ptr(), ws.numel(), stream) == 0
+        torch.cuda.synchronize()
+        assert not bool(ws[:4].any())
+        assert all(torch.equal(a, grads[k]) for k, a in (("dx", dx), ("da", da), ("db", db)))
