@@ -7,7 +7,9 @@
 // a thousand tokens cost 5e-6 of the result instead of 1e-6.  low is held in three bf16 parts beside
 // bf16 rows (all its bits; two left 2.4e-6 of a gradient), in two tf32 parts beside others.  Both
 // gradients are one launch (a launch after the other took 10 us more for 77 tokens).  Items that are
-// pieces of one adapter write partial sums, which a second kernel adds in order.
+// pieces of one adapter write partial sums, which a second kernel adds in order.  77 tokens, 4096 and
+// 4096 columns, rank 16: 9.8 us, latency; 4096 tokens of F32 rows of 4 adapters: 76 us, bound by the
+// matrix pipe and by splitting the rows into tf32 parts.
 #include <type_traits>
 
 #include "adapt.cuh"

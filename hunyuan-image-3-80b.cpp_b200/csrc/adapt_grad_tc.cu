@@ -18,7 +18,8 @@
 // The pipe truncates what it adds, some 4e-8 of the running sum each time: over 1600 tokens that made
 // 2e-6 of a gradient.  So the first part's sums go to two accumulators in turn, 256 tokens each, which
 // are added in registers; the other two parts' sums, 2^-8 of them, have one accumulator.  Bound by
-// reading the long rows.
+// reading the long rows: 8192 tokens of 4096 and 6144 columns, rank 64, 8 adapters take 60 us (2.8
+// TB/s; 54 with one accumulator and four times the error), split_kernel 3.
 #include "adapt_tc.cuh"
 
 namespace hymoe {

@@ -17,7 +17,8 @@
 //              round once and write pieces of 128 bytes.  Two warps share 32 rows (a quarter of the
 //              accumulator's lanes), each with half of the columns.
 // One lane owns one row, so fp16 parts can carry a power of two per row.  Bound by reading and
-// writing the rows of out.
+// writing the rows of out: 4160 tokens of requests to 4096 F32 columns, rank 16, 26.5 us (5.1 TB/s);
+// 8192 tokens in any order to 6144 bf16 columns, rank 64, 52 us (3.9 TB/s, in pieces of 256 bytes).
 #include "adapt_tc.cuh"
 
 namespace hymoe {
