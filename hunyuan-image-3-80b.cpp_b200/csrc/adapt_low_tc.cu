@@ -150,19 +150,21 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
         // the sums through shared memory (the stages are free): rows padded by four floats
         float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (int c = 0; c < RP; c += 32) {
-            constexpr int kNow = RP < 32 ? RP : 32;
-            float sum[kNow];
+        for (int c = 0; c < RP; c += 16) {
+            uint32_t v[L::kSets][16];
 #pragma unroll
-            for (int set = 0; set < L::kSets; ++set) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + set * L::kSet + c, v);
-                tmem_ld_wait();
+            for (int set = 0; set < L::kSets; ++set)
+                tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + set * L::kSet + c, v[set]);
+            tmem_ld_wait();
+            float sum[16];
 #pragma unroll
-                for (int j = 0; j < kNow; ++j) sum[j] = set == 0 ? __uint_as_float(v[j]) : sum[j] + __uint_as_float(v[j]);
+            for (int j = 0; j < 16; ++j) {
+                sum[j] = __uint_as_float(v[0][j]);
+#pragma unroll
+                for (int set = 1; set < L::kSets; ++set) sum[j] += __uint_as_float(v[set][j]);
             }
 #pragma unroll
-            for (int j = 0; j < kNow; j += 4)
+            for (int j = 0; j < 16; j += 4)
                 *reinterpret_cast<float4*>(red + r * (RP + 4) + c + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
         }
         tc_fence_before();

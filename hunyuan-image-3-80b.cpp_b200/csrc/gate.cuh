@@ -1068,7 +1068,7 @@ template <typename T>
 cudaError_t launch_gate_rows(const T* x, size_t ld, uint32_t n_tok, const GateArgs& a, cudaStream_t st) {
     const int block = n_tok < 148u * 512u ? 32 : 128;
     const size_t smem = sizeof(float) * ((a.bias ? a.E : 0) + static_cast<size_t>(a.n_group) * block);
-    const unsigned grid = (n_tok + block - 1) / block;
+    const unsigned grid = static_cast<unsigned>((static_cast<size_t>(n_tok) + block - 1) / block);
     if (a.bias && a.n_group) gate_rows_kernel<T, true, true><<<grid, block, smem, st>>>(x, ld, n_tok, a);
     else if (a.bias) gate_rows_kernel<T, true, false><<<grid, block, smem, st>>>(x, ld, n_tok, a);
     else if (a.n_group) gate_rows_kernel<T, false, true><<<grid, block, smem, st>>>(x, ld, n_tok, a);
