@@ -176,3 +176,15 @@ def test_workspace_as_it_comes(T):
         torch.cuda.synchronize()
         assert not bool(ws[:4].any())
         assert all(torch.equal(a, grads[k]) for k, a in (("dx", dx), ("da", da), ("db", db)))
+
+
+@pytest.mark.parametrize("shape,kw", [
+    ((5000, 72, 64, 8, 4096), {}),                                        # most adapters, about a token each
+    ((200, 128, 136, 128, 4096), dict(x="f16", w="f16", y="f32")),        # fewer tokens than adapters
+    ((130, 1 << 20, 64, 8, 2), {}),                                       # the longest rows to read
+    ((130, 64, 1 << 20, 8, 2), dict(x="f16", w="f16", y="f16")),          # and to write
+    ((90, 1 << 20, 72, 1, 1), dict(ids="one")),
+    ((33000, 64, 72, 16, 2), dict(ids="requests")),                       # long sums
+    ((70001, 64, 64, 8, 9), dict(x="f32", y="f32"))])
+def test_largest_sizes(shape, kw):
+    check(Problem(*shape, **kw))
