@@ -218,6 +218,22 @@ __device__ __forceinline__ void two_best(float& b1, float& b2, float o1, float o
     b1 = fmaxf(b1, o1);
 }
 
+// A group's value from its two best: half of their sum (which itself can lie beyond fp32, as with
+// experts that a bias of the lowest value masks: still open), its only one by half as well, or its
+// best; -inf: closed.  And a bound on its error.  An expert's value is off by less than delta plus
+// 2^-23 of itself (above), so half a sum by delta + 2^-23 of half the magnitudes, and its own rounding
+// and that of value -+ error by 2^-24 of the same each.  A magnitude belongs to its group alone: one
+// masked group does not make the others doubtful.
+__device__ __forceinline__ float group_value(bool two, float b1, float b2) {
+    return !two ? b1 : b2 > -INFINITY ? 0.5f * b1 + 0.5f * b2 : 0.5f * b1;
+}
+template <bool SIG>
+__device__ __forceinline__ float group_error(bool two, float b1, float b2) {
+    constexpr float delta = SIG ? 0x1p-21f : 0x1p-20f;
+    const float mag = !two ? fabsf(b1) : b2 > -INFINITY ? 0.5f * fabsf(b1) + 0.5f * fabsf(b2) : 0.5f * fabsf(b1);
+    return 1.25f * delta + 0x1p-22f * mag;
+}
+
 // Weight of a selected logit z (-inf: none selected in this lane): all lanes of the warp.  m, sum: a
 // plain softmax's largest logit and sum.
 template <bool SIG>
@@ -491,19 +507,19 @@ __device__ __forceinline__ bool route_token(const T* row, const Vec<T, EPL>& raw
                 }
             __syncwarp();
         }
-        val = two && b2 > -INFINITY ? b1 + b2 : b1;
+        val = group_value(two, b1, b2);
         const bool is_group = RUN || lane < a.n_group;
         int better = 0;
         for (int g = 0; g < a.n_group; ++g) {
             const float v = __shfl_sync(kAll, val, g * lanes);
             better += v > val || (v == val && g < mine);
         }
-        const bool keep = is_group && val > -INFINITY && better < a.topk_group;
+        const bool open = is_group && val > -INFINITY, keep = open && better < a.topk_group;
         if (biased || two) {
-            const float lowest = -warp_max(keep ? -val : -INFINITY);
-            const float first_out = warp_max(is_group && !keep ? val : -INFINITY);
-            const float big = warp_max(is_group && b1 > -INFINITY ? fabsf(b1) + (b2 > -INFINITY ? fabsf(b2) : 0.f) : 0.f);
-            unsure = first_out > -INFINITY && lowest - first_out <= 4.f * delta + 0x1p-21f * big;
+            const float err = group_error<SIG>(two, b1, b2);
+            const float lowest = -warp_max(keep ? err - val : -INFINITY);
+            const float first_out = warp_max(open && !keep ? val + err : -INFINITY);
+            unsure = first_out > -INFINITY && !(lowest > first_out);
         }
         if constexpr (RUN) {
             if (!keep) {
@@ -686,7 +702,7 @@ __device__ __forceinline__ void eight_values(const Vec<T, 8>& raw, const float* 
 template <typename T, bool BIASED, bool GROUPS>
 __global__ __launch_bounds__(128, 8) void gate_rows_kernel(const T* __restrict__ logits, size_t ld, uint32_t n_tok,
                                                         const __grid_constant__ GateArgs a) {
-    extern __shared__ __align__(16) float rbuf[];  // [E] biases, [n_group][threads] values
+    extern __shared__ __align__(16) float rbuf[];  // [E] biases, [n_group][threads] values and, with biases, errors
     __shared__ int cnt[HYMOE_GATE_MAX_EXPERTS];
     const int tid = threadIdx.x, E = a.E, K = a.K;
     for (int e = tid; e < E; e += blockDim.x) {
@@ -705,8 +721,8 @@ __global__ __launch_bounds__(128, 8) void gate_rows_kernel(const T* __restrict__
     if constexpr (GROUPS) {
         const bool two = a.group_score == HYMOE_GROUP_TOP2;
         const int gs = E / a.n_group;
-        float* gv = rbuf + (BIASED ? E : 0) + tid;
-        float big = 0.f;
+        // with a bias a group's error too, by its magnitude; scores alone are at most 1
+        float *gv = rbuf + (BIASED ? E : 0) + tid, *ge = gv + a.n_group * blockDim.x;
         for (int g = 0; g < a.n_group; ++g) {
             float b1 = -INFINITY, b2 = -INFINITY;
             for (int e = g * gs; e < (g + 1) * gs; e += 8) {
@@ -718,13 +734,13 @@ __global__ __launch_bounds__(128, 8) void gate_rows_kernel(const T* __restrict__
                     b1 = fmaxf(b1, v[i]);
                 }
             }
-            gv[g * blockDim.x] = two && b2 > -INFINITY ? b1 + b2 : b1;
-            if (b1 > -INFINITY) big = fmaxf(big, fabsf(b1) + (b2 > -INFINITY ? fabsf(b2) : 0.f));
+            gv[g * blockDim.x] = group_value(two, b1, b2);
+            if (BIASED) ge[g * blockDim.x] = group_error<true>(two, b1, b2);
         }
         kept = 0;
         float lowest = INFINITY, first_out = -INFINITY;
         for (int g = 0; g < a.n_group; ++g) {
-            const float v = gv[g * blockDim.x];
+            const float v = gv[g * blockDim.x], err = BIASED ? ge[g * blockDim.x] : group_error<true>(two, 1.f, 1.f);
             int better = 0;
             for (int h = 0; h < a.n_group; ++h) {
                 const float o = gv[h * blockDim.x];
@@ -732,12 +748,12 @@ __global__ __launch_bounds__(128, 8) void gate_rows_kernel(const T* __restrict__
             }
             if (v > -INFINITY && better < a.topk_group) {
                 kept |= 1u << g;
-                lowest = fminf(lowest, v);
-            } else {
-                first_out = fmaxf(first_out, v);
+                lowest = fminf(lowest, v - err);
+            } else if (v > -INFINITY) {
+                first_out = fmaxf(first_out, v + err);
             }
         }
-        if (BIASED || two) unsure_groups = first_out > -INFINITY && lowest - first_out <= 4.f * delta + 0x1p-21f * big;
+        if (BIASED || two) unsure_groups = first_out > -INFINITY && !(lowest > first_out);
     }
 
     unsigned l[8], rest = 0;
@@ -1067,7 +1083,7 @@ inline bool gate_by_rows(const hymoe_mat& x, size_t es, uint32_t n_tok, const Ga
 template <typename T>
 cudaError_t launch_gate_rows(const T* x, size_t ld, uint32_t n_tok, const GateArgs& a, cudaStream_t st) {
     const int block = n_tok < 148u * 512u ? 32 : 128;
-    const size_t smem = sizeof(float) * ((a.bias ? a.E : 0) + static_cast<size_t>(a.n_group) * block);
+    const size_t smem = sizeof(float) * ((a.bias ? a.E : 0) + static_cast<size_t>(a.n_group) * (a.bias ? 2 : 1) * block);
     const unsigned grid = static_cast<unsigned>((static_cast<size_t>(n_tok) + block - 1) / block);
     if (a.bias && a.n_group) gate_rows_kernel<T, true, true><<<grid, block, smem, st>>>(x, ld, n_tok, a);
     else if (a.bias) gate_rows_kernel<T, true, false><<<grid, block, smem, st>>>(x, ld, n_tok, a);
