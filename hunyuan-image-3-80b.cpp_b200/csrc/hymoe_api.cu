@@ -390,6 +390,16 @@ cudaError_t dalloc(T** p, size_t count) {
     return cudaMalloc(reinterpret_cast<void**>(p), sizeof(T) * (count ? count : 1));
 }
 
+// Copies a layer's small parameters and waits for the copy: a plain cudaMemcpy may return before it
+// has landed (device to device always, small host copies too), and the context's streams do not wait
+// for the legacy stream.  On that stream all the same: the copy follows what the caller queued on it
+// (and on the streams that it orders).
+cudaError_t copy_now(void* dst, const void* src, size_t bytes, bool host) {
+    const cudaError_t e = cudaMemcpyAsync(dst, src, bytes, host ? cudaMemcpyHostToDevice : cudaMemcpyDeviceToDevice,
+                                          cudaStreamLegacy);
+    return e != cudaSuccess ? e : cudaStreamSynchronize(cudaStreamLegacy);
+}
+
 hymoe_status make_tmap(hymoe_ctx* c, CUtensorMap* map, void* base, uint64_t K, uint64_t rows,
                        uint32_t box_rows_) {
     EncodeTiledFn enc = get_encode_fn();
@@ -1361,9 +1371,7 @@ hymoe_status hymoe_set_norm(hymoe_ctx* c, uint32_t layer, const float* weight, f
     }
     if (!c->rms_buf) HY_CUDA(c, dalloc(&c->rms_buf, static_cast<size_t>(c->cfg.max_tokens)));
     if (!c->norm_w[layer]) HY_CUDA(c, dalloc(&c->norm_w[layer], static_cast<size_t>(c->H)));
-    const bool host = (flags & HYMOE_HOST_PTRS) != 0;
-    HY_CUDA(c, cudaMemcpy(c->norm_w[layer], weight, sizeof(float) * c->H,
-                          host ? cudaMemcpyHostToDevice : cudaMemcpyDeviceToDevice));
+    HY_CUDA(c, copy_now(c->norm_w[layer], weight, sizeof(float) * c->H, (flags & HYMOE_HOST_PTRS) != 0));
     c->norm_eps[layer] = eps;
     return HYMOE_OK;
 }
@@ -1435,9 +1443,7 @@ hymoe_status hymoe_set_balance_bias(hymoe_ctx* c, uint32_t layer, const float* b
         c->clear_graphs();  // captured launches have no bias
         HY_CUDA(c, dalloc(&c->gate_bias[layer], static_cast<size_t>(c->E)));
     }
-    const bool host = (flags & HYMOE_HOST_PTRS) != 0;
-    HY_CUDA(c, cudaMemcpy(c->gate_bias[layer], bias, sizeof(float) * c->E,
-                          host ? cudaMemcpyHostToDevice : cudaMemcpyDeviceToDevice));
+    HY_CUDA(c, copy_now(c->gate_bias[layer], bias, sizeof(float) * c->E, (flags & HYMOE_HOST_PTRS) != 0));
     return HYMOE_OK;
 }
 
