@@ -1431,7 +1431,12 @@ hymoe_status hymoe_set_gate(hymoe_ctx* c, const hymoe_gate* gate) {
 hymoe_status hymoe_set_balance_bias(hymoe_ctx* c, uint32_t layer, const float* bias, int flags) {
     if (!c) return HYMOE_ERR_INVALID_ARG;
     if (layer >= c->layers.size()) return c->fail(HYMOE_ERR_INVALID_ARG, "layer %u out of range", layer);
+    if (bias && c->cfg.ep_size > 1) return c->fail(HYMOE_ERR_UNSUPPORTED, "hymoe_set_balance_bias: one GPU only");
     HY_CUDA(c, cudaSetDevice(c->cfg.device));
+    const bool host = (flags & HYMOE_HOST_PTRS) != 0;
+    if (bias && !host && !entry_on_device(bias, c->cfg.device))
+        return c->fail(HYMOE_ERR_INVALID_ARG, "hymoe_set_balance_bias: bias must be memory of the context's device "
+                                              "(or HYMOE_HOST_PTRS given)");
     HY_CUDA(c, cudaStreamSynchronize(c->stream));  // no call still reads the old bias
     if (!bias) {
         c->clear_graphs();
@@ -1439,11 +1444,19 @@ hymoe_status hymoe_set_balance_bias(hymoe_ctx* c, uint32_t layer, const float* b
         c->gate_bias[layer] = nullptr;
         return HYMOE_OK;
     }
-    if (!c->gate_bias[layer]) {
-        c->clear_graphs();  // captured launches have no bias
-        HY_CUDA(c, dalloc(&c->gate_bias[layer], static_cast<size_t>(c->E)));
+    if (c->gate_bias[layer]) {
+        HY_CUDA(c, copy_now(c->gate_bias[layer], bias, sizeof(float) * c->E, host));
+        return HYMOE_OK;
     }
-    HY_CUDA(c, copy_now(c->gate_bias[layer], bias, sizeof(float) * c->E, (flags & HYMOE_HOST_PTRS) != 0));
+    float* fresh = nullptr;
+    HY_CUDA(c, dalloc(&fresh, static_cast<size_t>(c->E)));
+    const cudaError_t e = copy_now(fresh, bias, sizeof(float) * c->E, host);
+    if (e != cudaSuccess) {
+        cudaFree(fresh);
+        HY_CUDA(c, e);
+    }
+    c->clear_graphs();  // captured launches have no bias
+    c->gate_bias[layer] = fresh;
     return HYMOE_OK;
 }
 

@@ -435,7 +435,8 @@ hymoe_status hymoe_adapt_backward(const hymoe_adapters* adapters, const hymoe_ma
 hymoe_status hymoe_set_gate(hymoe_ctx* ctx, const hymoe_gate* gate);
 
 /* The gate's selection bias of one layer: [E] F32 (host memory with HYMOE_HOST_PTRS, else device),
- * copied; NULL removes it.  Used while a gate is set. */
+ * copied before the call returns, after what is queued on the default stream; NULL removes it.  Used
+ * while a gate is set.  A refused call leaves the layer's bias as it was. */
 hymoe_status hymoe_set_balance_bias(hymoe_ctx* ctx, uint32_t layer, const float* bias, int flags);
 
 /* Adapters of one layer's shared expert for hymoe_forward_adapted, HYMOE_TYPE_F16: gate_up (H ->

@@ -95,3 +95,18 @@ def test_norm_has_landed(orc):
 
         np.testing.assert_array_equal(run(before)["out"], want)
     b.m.close()
+
+
+def test_balance_bias_of_the_wrong_memory_is_refused(orc):
+    """A host pointer given as device memory: refused, and the layer has no bias (or the one it had)."""
+    b = Block(orc)
+    b.m.set_gate(gate_of(b.E, b.K, GATES[0]))
+    L, wrong = hymoe.lib(), np.full(b.E, 7.0, np.float32)
+    wrong[::2] = -7.0
+    x, bias = b.x(20), np.random.default_rng(14).standard_normal(b.E).astype(np.float32)
+    for use in (None, bias):
+        b.m.set_balance_bias(0, use)
+        assert L.hymoe_set_balance_bias(b.m.h, 0, wrong.ctypes.data, 0) == 1
+        assert "device" in L.hymoe_last_error(b.m.h).decode()
+        check_gate(b.m.forward_host(0, x, debug=True), None if use is None else use.astype(np.float64), b.K, **GATES[0])
+    b.m.close()
