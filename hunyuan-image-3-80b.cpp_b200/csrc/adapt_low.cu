@@ -2,7 +2,9 @@
 //
 // A tile of 64 sorted rows of one adapter is shared by S CTAs, each over a part of the long
 // dimension.  Every CTA leaves its partial sums [64, RP] in the workspace; the last one of a tile to
-// arrive adds them in the order of the parts.  Bound by reading x (the weights, RP / 64 of its
+// arrive adds them in the order of the parts.  The matrix pipe truncates what it adds, so a stage's
+// products (16 additions for F32 rows, 4 for others) start from zero and join fp32 sums outside it: left
+// in its accumulators, 4096 columns of a CTA cost 2e-5 of low, and more the longer the rows.  Bound by reading x (the weights, RP / 64 of its
 // bytes per tile, come from L2): four stages of 64 columns are in flight per CTA, and S is chosen
 // so that the CTAs fill the GPU once.  77 tokens of 4096 columns, rank 16, both narrow products of a
 // backward pass: 9.4 us.  Long batches of F32 rows are bound by the tf32 pipe (two products for x's
@@ -20,6 +22,11 @@ constexpr int kLowStages = 4;
 template <typename X, typename W, int RP, bool TRANS>
 struct LowTile {
     static constexpr bool kF32 = sizeof(X) == 4;
+    // Groups of four warps that share the rank: the sums and a stage's accumulators of all 128 columns
+    // beside two tf32 parts do not fit one warp's registers (and one warp a scheduler, as large stages
+    // leave, waited for its own products).
+    static constexpr int kGroups = kF32 && RP == 128 ? 2 : 1;
+    static constexpr int kThreads = kGroups * kAdThreads, kOwn = RP / kGroups;  // columns of a warp
     static constexpr int kXRow = kF32 ? kLowK * 4 + 32 : kLowK * 2 + 16;
     static constexpr int kWRow = TRANS ? ad_pad16(RP * 2) : kLowK * 2 + 16;
     static constexpr int kXBytes = kAdRows * kXRow;
@@ -35,7 +42,8 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
     const int tile_id = blockIdx.x / S, rank = blockIdx.x % S;
     const int4 tile = ad_part_tile(a.plan, tile_id);
     if (tile.x < 0) return;  // none, or rows without an adapter
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5 & 3, lane = tid & 31;
+    const int c0 = L::kGroups == 1 ? 0 : (tid >> 7) * L::kOwn;  // this warp's columns of the rank
     const int nk = (a.K + kLowK - 1) / kLowK;
     const int k_lo = static_cast<int>(static_cast<int64_t>(nk) * rank / S);
     const int k_hi = static_cast<int>(static_cast<int64_t>(nk) * (rank + 1) / S);
@@ -43,16 +51,16 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
     // this thread's pieces of every stage: piece xc of rows xr0 + i * (128 / pieces) of x, and piece
     // p % kWPieces of row p / kWPieces of the weights, p = tid + i * 128
     constexpr int P = 16 / static_cast<int>(sizeof(X));
-    constexpr int kXPieces = kLowK / P, kXIter = kAdRows * kXPieces / kAdThreads;
+    constexpr int kXPieces = kLowK / P, kXIter = kAdRows * kXPieces / L::kThreads;
     constexpr int kWPieces = TRANS ? RP / 8 : kLowK / 8, kWAll = (TRANS ? kLowK : RP) * kWPieces;
-    constexpr int kWIter = kWAll / kAdThreads;
-    static_assert(kWAll % kAdThreads == 0, "whole rounds of pieces");
+    constexpr int kWIter = kWAll / L::kThreads;
+    static_assert(kWAll % L::kThreads == 0, "whole rounds of pieces");
     const int xc = tid % kXPieces, xr0 = tid / kXPieces;
     const char* xp[kXIter];  // the piece in column 0; rows that do not exist have no bytes
     int xn[kXIter];
 #pragma unroll
     for (int i = 0; i < kXIter; ++i) {
-        const int r = xr0 + i * (kAdThreads / kXPieces);
+        const int r = xr0 + i * (L::kThreads / kXPieces);
         const bool ok = r < tile.z;
         const int tok = ok ? __ldg(a.plan.perm + tile.y + r) : 0;
         xp[i] = static_cast<const char*>(a.x) + (static_cast<size_t>(tok) * a.ldx + (ok ? xc * P : 0)) * sizeof(X);
@@ -63,7 +71,7 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
     int wn[kWIter];
 #pragma unroll
     for (int i = 0; i < kWIter; ++i) {
-        const int p = tid + i * kAdThreads, r = p / kWPieces, c = p % kWPieces * 8;
+        const int p = tid + i * L::kThreads, r = p / kWPieces, c = p % kWPieces * 8;
         const bool ok = TRANS ? c < a.R : r < a.R;  // trans: row = k, columns = rank; else row = rank, columns = k
         wp[i] = ok ? wbase + (static_cast<size_t>(r) * (TRANS ? a.R : a.K) + c) * 2 : wbase;
         wn[i] = !ok ? 0 : TRANS ? min(16, (a.R - c) * 2) : 16;
@@ -76,36 +84,36 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
         if (vec && k0 + kLowK <= a.K) {  // a whole block of aligned rows
 #pragma unroll
             for (int i = 0; i < kXIter; ++i)
-                cp_async16_part(xs + (xr0 + i * (kAdThreads / kXPieces)) * L::kXRow + xc * 16,
+                cp_async16_part(xs + (xr0 + i * (L::kThreads / kXPieces)) * L::kXRow + xc * 16,
                                 xp[i] + static_cast<size_t>(k0) * sizeof(X), xn[i]);
             const size_t adv = static_cast<size_t>(k0) * (TRANS ? a.R : 1) * 2;
 #pragma unroll
             for (int i = 0; i < kWIter; ++i) {
-                const int p = tid + i * kAdThreads;
+                const int p = tid + i * L::kThreads;
                 cp_async16_part(ws + p / kWPieces * L::kWRow + p % kWPieces * 16, wn[i] ? wp[i] + adv : wbase, wn[i]);
             }
             return;
         }
 #pragma unroll
         for (int i = 0; i < kXIter; ++i) {
-            const int r = xr0 + i * (kAdThreads / kXPieces), n = xn[i] ? a.K - (k0 + xc * P) : 0;
+            const int r = xr0 + i * (L::kThreads / kXPieces), n = xn[i] ? a.K - (k0 + xc * P) : 0;
             ad_copy_piece<sizeof(X)>(xs + r * L::kXRow + xc * 16,
                                      n > 0 ? xp[i] + static_cast<size_t>(k0) * sizeof(X) : static_cast<const char*>(a.x), n, a.vec_x);
         }
 #pragma unroll
         for (int i = 0; i < kWIter; ++i) {
-            const int p = tid + i * kAdThreads, r = p / kWPieces, c = p % kWPieces;
+            const int p = tid + i * L::kThreads, r = p / kWPieces, c = p % kWPieces;
             const int n = wn[i] == 0 ? 0 : TRANS ? (k0 + r < a.K ? a.R - c * 8 : 0) : a.K - (k0 + c * 8);
             ad_copy_piece<2>(ws + r * L::kWRow + c * 16,
                              n > 0 ? wp[i] + static_cast<size_t>(k0) * (TRANS ? a.R : 1) * 2 : wbase, n, a.vec_w);
         }
     };
 
-    float acc[RP / 8][4];
+    float sum[L::kOwn / 8][4];
 #pragma unroll
-    for (int i = 0; i < RP / 8; ++i)
+    for (int i = 0; i < L::kOwn / 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+        for (int j = 0; j < 4; ++j) sum[i][j] = 0.f;
 
 #pragma unroll
     for (int s = 0; s < kLowStages - 1; ++s) {
@@ -121,21 +129,26 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
         cp_async_commit();
         const char* xs = smem + stage * L::kStage;
         const uint32_t xa = smem_u32(xs), wa = xa + L::kXBytes;
+        float acc[L::kOwn / 8][4];  // this stage's products
+#pragma unroll
+        for (int i = 0; i < L::kOwn / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < kLowK / 16; ++kk) {
-            uint32_t bf[RP / 16][4];
+            uint32_t bf[L::kOwn / 16][4];
 #pragma unroll
-            for (int j = 0; j < RP / 16; ++j) {
+            for (int j = 0; j < L::kOwn / 16; ++j) {
                 if (TRANS)  // blocks (k 0-7, n 0-7), (k 8-15, n 0-7), (k 0-7, n 8-15), (k 8-15, n 8-15)
-                    ldsm4_t(bf[j], wa + (kk * 16 + (lane & 15)) * L::kWRow + (j * 16 + (lane >> 4) * 8) * 2);
+                    ldsm4_t(bf[j], wa + (kk * 16 + (lane & 15)) * L::kWRow + (c0 + j * 16 + (lane >> 4) * 8) * 2);
                 else
-                    ldsm4(bf[j], wa + (j * 16 + (lane >> 4) * 8 + (lane & 7)) * L::kWRow + (kk * 16 + (lane >> 3 & 1) * 8) * 2);
+                    ldsm4(bf[j], wa + (c0 + j * 16 + (lane >> 4) * 8 + (lane & 7)) * L::kWRow + (kk * 16 + (lane >> 3 & 1) * 8) * 2);
             }
             if constexpr (!L::kF32) {
                 uint32_t af[4];
                 ldsm4(af, xa + (warp * 16 + (lane & 15)) * L::kXRow + (kk * 16 + (lane >> 4) * 8) * 2);
 #pragma unroll
-                for (int j = 0; j < RP / 16; ++j) {
+                for (int j = 0; j < L::kOwn / 16; ++j) {
                     AdType<W>::mma(acc[2 * j], af, bf[j][0], bf[j][1]);
                     AdType<W>::mma(acc[2 * j + 1], af, bf[j][2], bf[j][3]);
                 }
@@ -156,7 +169,7 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
                     split_tf32(v[h][0].y, hi[2], lo[2]);
                     split_tf32(v[h][1].y, hi[3], lo[3]);
 #pragma unroll
-                    for (int j = 0; j < RP / 16; ++j)
+                    for (int j = 0; j < L::kOwn / 16; ++j)
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             const float2 b = AdType<W>::unpack(bf[j][2 * q + h]);
@@ -166,6 +179,10 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
                 }
             }
         }
+#pragma unroll
+        for (int i = 0; i < L::kOwn / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[i][j] += acc[i][j];
     }
     cp_async_wait<0>();
     const float f = a.scale != nullptr ? __ldg(a.scale + tile.x) : 1.f;
@@ -179,10 +196,10 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
         const int r = warp * 16 + g + 8 * q;
         if (r >= tile.z) continue;
 #pragma unroll
-        for (int j = 0; j < RP / 8; ++j) {
-            const float2 v = make_float2(acc[j][2 * q] * f1, acc[j][2 * q + 1] * f1);
+        for (int j = 0; j < L::kOwn / 8; ++j) {
+            const float2 v = make_float2(sum[j][2 * q] * f1, sum[j][2 * q + 1] * f1);
             top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
-            *reinterpret_cast<float2*>(dst + static_cast<size_t>(r) * RP + j * 8 + 2 * t) = v;
+            *reinterpret_cast<float2*>(dst + static_cast<size_t>(r) * RP + c0 + j * 8 + 2 * t) = v;
         }
     }
     __syncwarp();
@@ -200,7 +217,7 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
     __threadfence();
     const float* part = a.part + static_cast<size_t>(tile_id) * S * (kAdRows * RP);
     top = 0.f;
-    for (int p = tid; p < tile.z * (RP / 4); p += kAdThreads) {
+    for (int p = tid; p < tile.z * (RP / 4); p += L::kThreads) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int q = 0; q < S; ++q) {
@@ -219,7 +236,7 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
 }
 
 template <typename X, typename W, int RP, bool TRANS>
-__global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void low_kernel(
+__global__ __launch_bounds__(LowTile<X, W, RP, TRANS>::kThreads, LowTile<X, W, RP, TRANS>::kPerSm) void low_kernel(
     const __grid_constant__ AdaptLow a, int S) {
     extern __shared__ __align__(128) char smem[];
     griddep_wait();
@@ -229,7 +246,7 @@ __global__ __launch_bounds__(kAdThreads, LowTile<X, W, RP, TRANS>::kPerSm) void 
 
 // Grid (tiles x the larger S, 2).
 template <typename X, typename W, int RP>
-__global__ __launch_bounds__(kAdThreads) void low_pair_kernel(const __grid_constant__ AdaptLow a, int Sa,
+__global__ __launch_bounds__(LowTile<X, W, RP, true>::kThreads) void low_pair_kernel(const __grid_constant__ AdaptLow a, int Sa,
                                                               const __grid_constant__ AdaptLow b, int Sb, int tiles) {
     extern __shared__ __align__(128) char smem[];
     griddep_wait();
@@ -250,7 +267,7 @@ cudaError_t launch_pair(const AdaptLow& a, const AdaptLow& b, int n_sms, cudaStr
     if (e != cudaSuccess) return e;
     const int tiles = a.plan.max_tiles * (a.plan.tile_rows / kAdRows);
     const int Sa = adapt_splits(tiles, a.K, per_sm * n_sms / 2), Sb = adapt_splits(tiles, b.K, per_sm * n_sms / 2);
-    return launch_kernel(true, kern, dim3(static_cast<unsigned>(tiles) * (Sa > Sb ? Sa : Sb), 2), dim3(kAdThreads), smem, st, a, Sa,
+    return launch_kernel(true, kern, dim3(static_cast<unsigned>(tiles) * (Sa > Sb ? Sa : Sb), 2), dim3(La::kThreads), smem, st, a, Sa,
                          b, Sb, tiles);
 }
 
@@ -272,7 +289,7 @@ cudaError_t launch_t(const AdaptLow& a, int n_sms, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const int tiles = a.plan.max_tiles * (a.plan.tile_rows / kAdRows);
     const int S = adapt_splits(tiles, a.K, L::kPerSm * n_sms);
-    return launch_kernel(true, kern, dim3(static_cast<unsigned>(tiles) * S), dim3(kAdThreads), L::kSmem, st, a, S);
+    return launch_kernel(true, kern, dim3(static_cast<unsigned>(tiles) * S), dim3(L::kThreads), L::kSmem, st, a, S);
 }
 
 template <typename X, typename W>
