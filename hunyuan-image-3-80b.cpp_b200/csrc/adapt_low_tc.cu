@@ -7,7 +7,16 @@
 // copied by the four later epilogue warps, eight lanes to a row (gather4 loads of four rows were
 // tried: they top out at 2.5 TB/s).  One thread issues the products (M = 128 rows, N = RP) into
 // tensor memory.  The parts are added in distributed shared memory, every CTA taking its share of
-// the rows, in the order of the parts.  Bound by reading x: 8192 tokens of 4096 columns, rank 64, in
+// the rows, in the order of the parts.
+//
+// The pipe truncates what it adds, up to 1.4 times 2^-23 of the running sum each time, so a CTA's
+// columns take turns in four accumulators (two at rank 128), as long as that makes 64 stages at most:
+// 64 additions each (128).  Longer rows (LONG) go in segments of 8 stages, 32 additions to one
+// accumulator, which the epilogue's warps add in fp32 to totals in tensor memory while the next
+// segment goes to another (at rank 128 there is room for one and the totals: the next segment's loads
+// go on, its products wait).  Without segments 2^20 columns lost 1.5e-4 of low (rank 128: 3.4e-4).
+//
+// Bound by reading x: 8192 tokens of 4096 columns, rank 64, in
 // any order 21 us (3.2 TB/s; some 8 us pass before the loads are in full flow and after they end).
 #include "adapt_tc.cuh"
 
@@ -16,6 +25,8 @@ namespace {
 
 constexpr int kLtcRows = kTcRows;
 constexpr int kLtcThreads = 192;  // TMA, MMA, four copying and epilogue warps
+constexpr int kLtcMostStages = 64;  // of a CTA without segments
+constexpr int kLtcSegment = 8;      // stages of a segment
 
 // N: columns of the product; an MN-major weight tile has whole blocks of 64.
 template <int RP, bool TRANS>
@@ -25,20 +36,21 @@ struct LtcTile {
     static constexpr int kStages = kN == 128 ? 3 : 4;
     static constexpr int kSmem = 1024 + kStages * (kA + kB);
     static_assert(kStages * (kA + kB) >= kLtcRows * (RP + 4) * 4, "the stages hold the partial sums");
-    // Accumulators that take the columns in turn: the pipe truncates what it adds, 4e-8 of the running
-    // sum each time (over 2048 columns that made 2e-6 of low; a quarter with four).
-    static constexpr int kSets = kN == 128 ? 2 : 4;
-    static constexpr int kSet = kN < 32 ? 32 : kN;  // columns of one
-    static constexpr int kCols = kSets * kSet;      // two CTAs share the 512 of an SM
+    static constexpr int kAccs = kN == 128 ? 2 : 4;  // accumulators
+    static constexpr int kSet = kN < 32 ? 32 : kN;   // columns of one
+    static constexpr int kCols = kAccs * kSet;       // two CTAs share the 512 of an SM
+    static constexpr int kBufs = kAccs / 2;          // LONG: those of segments, and behind them the totals
 };
 
-template <typename W, int RP, bool TRANS>
+template <typename W, int RP, bool TRANS, bool LONG>
 __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_constant__ AdaptMaps maps,
                                                                 const __grid_constant__ AdaptLow a, int S) {
     using L = LtcTile<RP, TRANS>;
+    constexpr int kSets = LONG ? 1 : L::kAccs;  // accumulators that a stage's products take in turn
+    static_assert(L::kStages < kLtcSegment, "the copying warps add up a segment amid the next");
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    __shared__ uint64_t full[L::kStages], empty[L::kStages], done;
+    __shared__ uint64_t full[L::kStages], empty[L::kStages], done, seg_done[L::kBufs], seg_free[L::kBufs];
     __shared__ uint32_t tmem_s;
     __shared__ int tok[kLtcRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -57,6 +69,12 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
             mbar_init(&empty[s], 1);
         }
         mbar_init(&done, 1);
+        if (LONG) {
+            for (int b = 0; b < L::kBufs; ++b) {
+                mbar_init(&seg_done[b], 1);
+                mbar_init(&seg_free[b], 4);  // the epilogue's warps
+            }
+        }
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -70,6 +88,7 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
     const int nk = (a.K + 63) / 64;
     const int k_lo = static_cast<int>(static_cast<int64_t>(nk) * rank / S);
     const int k_hi = static_cast<int>(static_cast<int64_t>(nk) * (rank + 1) / S);
+    const int n_seg = (k_hi - k_lo + kLtcSegment - 1) / kLtcSegment;
     int* err = a.plan.err;  // the status word
 
     if (warp == 0) {
@@ -100,16 +119,19 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
             int it = 0;
             for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
                 const int s = it % L::kStages;
+                const int seg = it / kLtcSegment, b = LONG ? seg % L::kBufs : 0, seg_it = LONG ? it % kLtcSegment : it;
+                if (LONG && seg_it == 0 && seg >= L::kBufs && !mbar_wait(&seg_free[b], (seg / L::kBufs - 1) & 1, err, DEVERR_TIMEOUT_MMA)) break;
                 if (!mbar_wait(&full[s], (it / L::kStages) & 1, err, DEVERR_TIMEOUT_MMA)) break;
                 if (!run) fence_proxy_async_smem();  // the copied rows, before the tensor core reads them
                 tc_fence_after();
                 const uint32_t sa = smem_u32(smem + s * (L::kA + L::kB)), sb = sa + L::kA;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                    mma_f16_ss(tmem + kk % L::kSets * L::kSet, sw128_kmajor_desc(sa + kk * 32),
+                    mma_f16_ss(tmem + (b + kk % kSets) * L::kSet, sw128_kmajor_desc(sa + kk * 32),
                                TRANS ? sw128_mnmajor_desc(sb + kk * 2048, 8192) : sw128_kmajor_desc(sb + kk * 32), idesc,
-                               it != 0 || kk >= L::kSets ? 1u : 0u);
+                               seg_it != 0 || kk >= kSets ? 1u : 0u);
                 mma_commit(&empty[s]);
+                if (LONG && seg_it == kLtcSegment - 1 && seg + 1 < n_seg) mma_commit(&seg_done[b]);
             }
             mma_commit(&done);
             mbar_drain(&done, 0);  // every product has ended before tensor memory is freed
@@ -117,6 +139,45 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
         __syncwarp();
     } else {
         const int q = warp & 3, et = tid - 64;
+        const uint32_t mine = tmem + (static_cast<uint32_t>(q * 32) << 16);  // this warp's rows
+        // Sixteen columns of accumulators b .. b + kSets and, with `more`, of the totals.
+        const auto gather = [&](int b, int c, bool more, float (&sum)[16]) {
+            uint32_t v[kSets + LONG][16];
+#pragma unroll
+            for (int set = 0; set < kSets; ++set) tmem_ld_32x32b_x16(mine + (b + set) * L::kSet + c, v[set]);
+            if (LONG && more) tmem_ld_32x32b_x16(mine + L::kBufs * L::kSet + c, v[kSets - 1 + LONG]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                sum[j] = __uint_as_float(v[0][j]);
+#pragma unroll
+                for (int set = 1; set < kSets; ++set) sum[j] += __uint_as_float(v[set][j]);
+                if (LONG && more) sum[j] += __uint_as_float(v[kSets - 1 + LONG][j]);
+            }
+        };
+        // The sums of the next segment but the last, when it has ended, into the totals.
+        int folded = 0;
+        const auto fold = [&]() {
+            const int b = folded % L::kBufs;
+            if (!__all_sync(0xffffffffu, mbar_wait(&seg_done[b], (folded / L::kBufs) & 1, err, DEVERR_TIMEOUT_EPILOGUE))) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < RP; c += 16) {
+                float sum[16];
+                gather(b, c, folded > 0, sum);
+                uint32_t v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(sum[j]);
+                tmem_st_32x32b_x16(mine + L::kBufs * L::kSet + c, v);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_free[b]);
+            ++folded;
+            return true;
+        };
+        bool ok = true;
         if (!run) {
             // this thread's piece of rows et / 8 + 16 i
             const int piece = et & 7;
@@ -129,8 +190,10 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
                 dst[i] = sw128_offset(r, piece);
             }
             int it = 0;
-            for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
+            for (int kb = k_lo; ok && kb < k_hi; ++kb, ++it) {
                 const int s = it % L::kStages;
+                // the ring is full of the next segment's stages (which may wait for this): time for the last one's sums
+                if (LONG && it >= kLtcSegment && it % kLtcSegment == L::kStages && !(ok = fold())) break;
                 if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / L::kStages) & 1) ^ 1, err, DEVERR_TIMEOUT_PRODUCER))) break;
                 uint8_t* sa = smem + s * (L::kA + L::kB);
                 const int left = a.K - kb * 64 - piece * 8;
@@ -140,8 +203,11 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
                     cp_async16_part(sa + dst[i], bytes ? src[i] + static_cast<size_t>(kb) * 128 : static_cast<const char*>(a.x), bytes);
                 cp_async_arrive(&full[s]);
             }
+            ok = ok && it == k_hi - k_lo;
             cp_async_wait_all();
         }
+        if (LONG)
+            while (ok && folded + 1 < n_seg) ok = fold();
         // on an expired wait the status word says that the results are not valid
         mbar_wait(&done, 0, err, DEVERR_TIMEOUT_EPILOGUE);
         tc_fence_after();
@@ -151,18 +217,8 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
         float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
         for (int c = 0; c < RP; c += 16) {
-            uint32_t v[L::kSets][16];
-#pragma unroll
-            for (int set = 0; set < L::kSets; ++set)
-                tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + set * L::kSet + c, v[set]);
-            tmem_ld_wait();
             float sum[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                sum[j] = __uint_as_float(v[0][j]);
-#pragma unroll
-                for (int set = 1; set < L::kSets; ++set) sum[j] += __uint_as_float(v[set][j]);
-            }
+            gather(LONG ? (n_seg - 1) % L::kBufs : 0, c, n_seg > 1, sum);
 #pragma unroll
             for (int j = 0; j < 16; j += 4)
                 *reinterpret_cast<float4*>(red + r * (RP + 4) + c + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
@@ -212,14 +268,14 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
 template <typename W, int RP, bool TRANS>
 cudaError_t launch_t(const AdaptMaps& maps, const AdaptLow& a, int n_sms, cudaStream_t st) {
     using L = LtcTile<RP, TRANS>;
-    auto kern = low_tc_kernel<W, RP, TRANS>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
-    if (e != cudaSuccess) return e;
     // as many CTAs as two to an SM allow (for the tiles that are likely: half of the adapters' last
     // ones are short of the bound), each with two stages of columns at least
     const int nk = (a.K + 63) / 64, tiles = a.plan.max_tiles - a.plan.spare_tiles / 2;
     int S = 1;
     while (S < 8 && tiles * 2 * S <= 2 * n_sms && nk >= 4 * S) S *= 2;
+    auto kern = (nk + S - 1) / S > kLtcMostStages ? low_tc_kernel<W, RP, TRANS, true> : low_tc_kernel<W, RP, TRANS, false>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(a.plan.max_tiles) * S);
     cfg.blockDim = dim3(kLtcThreads);

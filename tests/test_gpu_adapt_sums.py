@@ -20,6 +20,7 @@ torch = pytest.importorskip("torch")
 
 T16 = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 BLOCK = 64          # columns of a block's sum in the mma.sync kernels
+SEGMENT = 512       # the fewest columns of a segment on the 5th-generation tensor cores
 SPLITS = 16
 
 
@@ -59,6 +60,17 @@ CASES = [  # tokens, columns, rank, x, weights, additions of one accumulator, co
     (300, (1 << 18) + 1, 5, "bf16", "bf16", 4, BLOCK),    # off 16-byte boundaries
     (300, (1 << 18) + 4, 40, "f16", "f16", 4, BLOCK),
     (100, 1 << 18, 8, "bf16", "bf16", 4, BLOCK),          # few tokens
+    # the 5th-generation tensor cores: 64 additions (rank 128: 128) where the accumulators take all of a CTA's columns
+    (300, 1 << 15, 8, "bf16", "bf16", 64, 1 << 12),
+    (300, 1 << 15, 128, "f16", "f16", 128, 1 << 12),
+    # longer rows in segments of 32
+    (300, 1 << 20, 8, "bf16", "bf16", 32, SEGMENT),
+    (300, 1 << 20, 128, "bf16", "bf16", 32, SEGMENT),
+    (300, 1 << 18, 64, "f16", "f16", 32, SEGMENT),
+    (300, 200 * 1024 + 72, 32, "bf16", "bf16", 32, SEGMENT),
+    (300, (1 << 15) + 64, 24, "f16", "f16", 32, SEGMENT),   # one stage more in some CTAs
+    (300, (1 << 15) + 520, 128, "bf16", "bf16", 32, SEGMENT),
+    (2000, 1 << 16, 16, "f16", "f16", 32, SEGMENT),
 ]
 NAMES = ["-".join(map(str, c[:5])) for c in CASES]
 
