@@ -238,6 +238,8 @@ __device__ __forceinline__ void split_tf32(float v, uint32_t& hi, uint32_t& lo) 
     hi = __float_as_uint(v) & 0xffffe000u;
     lo = __float_as_uint(v - __uint_as_float(hi));
 }
+// What is left of v beside its first part: nothing of an infinity (inf - inf would make the row NaN).
+__device__ __forceinline__ float part_rest(float v, float part) { return fabsf(v) == INFINITY ? 0.f : v - part; }
 
 #endif  // __CUDACC__
 

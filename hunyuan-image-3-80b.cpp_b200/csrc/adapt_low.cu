@@ -164,10 +164,12 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t hi[4], lo[4];
-                    split_tf32(v[h][0].x, hi[0], lo[0]);
-                    split_tf32(v[h][1].x, hi[1], lo[1]);
-                    split_tf32(v[h][0].y, hi[2], lo[2]);
-                    split_tf32(v[h][1].y, hi[3], lo[3]);
+                    const float part[4] = {v[h][0].x, v[h][1].x, v[h][0].y, v[h][1].y};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        split_tf32(part[i], hi[i], lo[i]);
+                        lo[i] = __float_as_uint(part_rest(part[i], __uint_as_float(hi[i])));
+                    }
 #pragma unroll
                     for (int j = 0; j < L::kOwn / 16; ++j)
 #pragma unroll
@@ -197,9 +199,10 @@ __device__ __forceinline__ void low_tile(const AdaptLow& a, int S, char* smem) {
         if (r >= tile.z) continue;
 #pragma unroll
         for (int j = 0; j < L::kOwn / 8; ++j) {
-            const float2 v = make_float2(sum[j][2 * q] * f1, sum[j][2 * q + 1] * f1);
+            const int c = c0 + j * 8 + 2 * t;  // (columns behind the rank: 0 times an infinity is none of the result's)
+            const float2 v = make_float2(c < a.R ? sum[j][2 * q] * f1 : 0.f, c + 1 < a.R ? sum[j][2 * q + 1] * f1 : 0.f);
             top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
-            *reinterpret_cast<float2*>(dst + static_cast<size_t>(r) * RP + c0 + j * 8 + 2 * t) = v;
+            *reinterpret_cast<float2*>(dst + static_cast<size_t>(r) * RP + c) = v;
         }
     }
     __syncwarp();

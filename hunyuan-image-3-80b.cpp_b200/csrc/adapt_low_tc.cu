@@ -243,7 +243,8 @@ __global__ __launch_bounds__(kLtcThreads, 2) void low_tc_kernel(const __grid_con
                 s.z += v.z;
                 s.w += v.w;
             }
-            s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+            // (columns behind the rank: 0 times an infinity is none of the result's)
+            s = make_float4(c < a.R ? s.x * f : 0.f, c + 1 < a.R ? s.y * f : 0.f, c + 2 < a.R ? s.z * f : 0.f, c + 3 < a.R ? s.w * f : 0.f);
             top = fmaxf(top, fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w))));
             *reinterpret_cast<float4*>(a.low + static_cast<size_t>(tile.y + row) * RP + c) = s;
         }

@@ -36,8 +36,8 @@ __device__ __forceinline__ void split16(float x, float y, uint32_t (&p)[NP]) {
     for (int i = 0; i < NP; ++i) {
         p[i] = AdType<W>::pack(x, y);
         const float2 b = AdType<W>::unpack(p[i]);
-        x -= b.x;
-        y -= b.y;
+        x = part_rest(x, b.x);
+        y = part_rest(y, b.y);
     }
 }
 

@@ -302,8 +302,8 @@ __global__ __launch_bounds__(kWtcThreads, 1) void wide_tc_kernel(const __grid_co
                             for (int j = 0; j < 4; ++j) {
                                 w[j] = AdType<W>::pack(v[2 * j], v[2 * j + 1]);
                                 const float2 b = AdType<W>::unpack(w[j]);
-                                v[2 * j] -= b.x;
-                                v[2 * j + 1] -= b.y;
+                                v[2 * j] = part_rest(v[2 * j], b.x);
+                                v[2 * j + 1] = part_rest(v[2 * j + 1], b.y);
                             }
                             *reinterpret_cast<uint4*>(sA + (p * L::kKBlocks + c / 8) * kWtcPanel + sw128_offset(r, c % 8)) =
                                 make_uint4(w[0], w[1], w[2], w[3]);

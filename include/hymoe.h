@@ -405,8 +405,9 @@ hymoe_status hymoe_adapt_workspace(const hymoe_adapters* adapters, uint32_t n_to
  *   workspace: hymoe_adapt_workspace bytes, 256-byte aligned, used by this call alone until it
  *     has run (NULL where none is needed).  Its first 4 bytes are then 0; anything else says that a
  *     bounded device-side wait expired and the results are not whole
- * Products are summed in fp32, the intermediate A x is kept in fp32 or in parts that add up to
- * it, and the result is rounded once. */
+ * Products are summed in fp32, the intermediate A x is kept in fp32 or in parts that add up to it
+ * (to 16 bits beside a 16-bit result, 21 beside an F32 one), and the result is rounded once.
+ * Infinities and NaN in x or base stay in their token's row and come out as the formula has them. */
 hymoe_status hymoe_adapt(const hymoe_adapters* adapters, const hymoe_mat* x, const int32_t* ids,
                          uint32_t n_tokens, const hymoe_mat* base, const hymoe_mat* out, void* workspace,
                          size_t workspace_bytes, void* stream);
@@ -417,7 +418,10 @@ hymoe_status hymoe_adapt(const hymoe_adapters* adapters, const hymoe_mat* x, con
  *   da[a]  = scale[a] * sum over a's tokens of (B_a^T dy[t]) x[t]^T   [n_adapters, rank, in_features]
  *   db[a]  = scale[a] * sum over a's tokens of dy[t] (A_a x[t])^T     [n_adapters, out_features, rank]
  * da and db are F32, overwritten for every adapter (0 where it has no tokens), nullable.  The
- * sums' order depends on the ids alone: equal inputs give equal bits. */
+ * sums' order depends on the ids alone: equal inputs give equal bits.  Infinities and NaN come out of
+ * dx as of hymoe_adapt's out; da and db are infinite or NaN where they take part.  For F16 adapters,
+ * more than 128 tokens and rows that TMA takes (16-byte boundaries), da and db hold B_a^T dy and A_a x
+ * to 33 bits below the adapter's largest of them. */
 hymoe_status hymoe_adapt_backward(const hymoe_adapters* adapters, const hymoe_mat* x, const hymoe_mat* dy,
                                   const int32_t* ids, uint32_t n_tokens, const hymoe_mat* base,
                                   const hymoe_mat* dx, float* da, float* db, void* workspace,
