@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kDecThreads, 4) void decode_adapt_kernel(const __gr
                 const W* row[kDecRows];
 #pragma unroll
                 for (int i = 0; i < kDecRows; ++i) row[i] = wa + static_cast<size_t>(min(g * kDecRows + i, R - 1)) * K;
-                if (d.vec_x && d.vec_a) {
+                if (d.vec_x && d.vec_a) {  // (K and k_lo .. k_hi are whole pieces of 8 then)
 #pragma unroll 2
                     for (int k = k_lo + (kp * 32 + lane) * 8; k + 8 <= k_hi; k += kparts * 256) {
                         float xv[8];
@@ -93,11 +93,6 @@ __global__ __launch_bounds__(kDecThreads, 4) void decode_adapt_kernel(const __gr
                             for (int j = 0; j < 8; ++j) s[i] = fmaf(xv[j], wv[j], s[i]);
                         }
                     }
-                    // a last piece that is not whole (K not a multiple of 8)
-                    const int tail = k_hi / 8 * 8 > k_lo ? k_hi / 8 * 8 : k_lo;
-                    if (kp == 0 && tail + lane < k_hi)
-#pragma unroll
-                        for (int i = 0; i < kDecRows; ++i) s[i] = fmaf(dec_f(x[tail + lane]), dec_f(row[i][tail + lane]), s[i]);
                 } else {
                     for (int k = k_lo + kp * 32 + lane; k < k_hi; k += kparts * 32) {
                         const float xv = dec_f(x[k]);
