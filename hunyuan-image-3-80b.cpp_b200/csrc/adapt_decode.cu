@@ -130,34 +130,33 @@ __global__ __launch_bounds__(kDecThreads, 4) void decode_adapt_kernel(const __gr
     const Y* base = static_cast<const Y*>(d.base);
     Y* out = static_cast<Y*>(d.out) + static_cast<size_t>(t) * d.ldo;
     for (int o = n_lo + tid; o < n_hi; o += kDecThreads) {
-        const Y* from = base != nullptr ? base + static_cast<size_t>(t) * d.ldb + o : nullptr;
-        if (!has) {  // the base's row as it is (0 + -0 would be 0)
-            if (from != nullptr) out[o] = *from;
-            else dec_store(out + o, 0.f);
-            continue;
-        }
         float s = 0.f;
-        const W* row = wb + static_cast<size_t>(o) * R;
-        if (d.vec_b) {
+        if (has) {
+            const W* row = wb + static_cast<size_t>(o) * R;
+            if (d.vec_b) {
 #pragma unroll 4
-            for (int j = 0; j < R; j += 8) {
-                float wv[8];
-                dec_load8(row + j, wv);
-                const float4 l0 = *reinterpret_cast<const float4*>(low + j), l1 = *reinterpret_cast<const float4*>(low + j + 4);
-                s = fmaf(l0.x, wv[0], s);
-                s = fmaf(l0.y, wv[1], s);
-                s = fmaf(l0.z, wv[2], s);
-                s = fmaf(l0.w, wv[3], s);
-                s = fmaf(l1.x, wv[4], s);
-                s = fmaf(l1.y, wv[5], s);
-                s = fmaf(l1.z, wv[6], s);
-                s = fmaf(l1.w, wv[7], s);
+                for (int j = 0; j < R; j += 8) {
+                    float wv[8];
+                    dec_load8(row + j, wv);
+                    const float4 l0 = *reinterpret_cast<const float4*>(low + j), l1 = *reinterpret_cast<const float4*>(low + j + 4);
+                    s = fmaf(l0.x, wv[0], s);
+                    s = fmaf(l0.y, wv[1], s);
+                    s = fmaf(l0.z, wv[2], s);
+                    s = fmaf(l0.w, wv[3], s);
+                    s = fmaf(l1.x, wv[4], s);
+                    s = fmaf(l1.y, wv[5], s);
+                    s = fmaf(l1.z, wv[6], s);
+                    s = fmaf(l1.w, wv[7], s);
+                }
+            } else {
+                for (int j = 0; j < R; ++j) s = fmaf(low[j], dec_f(row[j]), s);
             }
-        } else {
-            for (int j = 0; j < R; ++j) s = fmaf(low[j], dec_f(row[j]), s);
         }
-        if (from != nullptr) s += dec_f(*from);
-        dec_store(out + o, s);
+        Y v;
+        dec_store(&v, 0.f);
+        if (base != nullptr) v = base[static_cast<size_t>(t) * d.ldb + o];
+        if (has) dec_store(&v, s + dec_f(v));  // else the base's value as it is (0 + -0 would be 0)
+        out[o] = v;
     }
     if (has) cluster_sync();  // no CTA leaves while another reads its partial result
 }
