@@ -582,6 +582,8 @@ class Adapters:
         if got is None:
             n = C.c_size_t()
             _check_entry(self.L.hymoe_adapt_workspace(C.byref(self.spec), T, 1 if backward else 0, C.byref(n)))
+            if len(self._bytes) >= 256:  # batches of many sizes
+                self._bytes.clear()
             got = self._bytes[(T, backward)] = n.value
         return got
 
