@@ -587,6 +587,32 @@ class Adapters:
             got = self._bytes[(T, backward)] = n.value
         return got
 
+    def workspace(self, T: int, backward: bool = False):
+        """Device memory for apply() (backward()) of up to T tokens; None where none is needed.  Passed as
+        a call's workspace it is that call's alone until the call has run, and check() then tells
+        whether the results are whole.  Calls without one take memory of their own and drop it."""
+        import torch
+        n = self._workspace_bytes(T, backward)
+        return torch.empty((n,), dtype=torch.uint8, device=self.device) if n else None
+
+    def check(self, workspace) -> None:
+        """Waits for the call that was given this workspace (on the current stream) and raises HymoeError
+        (TIMEOUT) if a bounded device-side wait expired in it: its results are not whole then."""
+        if workspace is not None and bool(workspace[:4].any()):
+            raise HymoeError(STATUS_TIMEOUT, "hymoe_adapt: a bounded device-side wait expired, the results are not whole")
+
+    def _memory(self, workspace, like, T: int, backward: bool):
+        """(tensor, pointer, bytes) of the given workspace, or of a new one."""
+        torch = _torch()[0]
+        if workspace is None:
+            n = self._workspace_bytes(T, backward)
+            ws = like.new_empty((n,), dtype=torch.uint8) if n else None
+            return ws, ws.data_ptr() if n else None, n
+        if workspace.dtype != torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous uint8 tensor on {self.device}, got {workspace.dtype} on "
+                             f"{workspace.device}")
+        return workspace, workspace.data_ptr(), workspace.numel()
+
     def _rows(self, t, T: int, cols: int, what: str):
         if t is None:
             return None
@@ -594,10 +620,10 @@ class Adapters:
             raise ValueError(f"{what} must be on {self.device}, got {t.device}")
         return _mat(t, T, cols, what)
 
-    def apply(self, x, ids=None, base=None, out=None):
+    def apply(self, x, ids=None, base=None, out=None, workspace=None):
         """out[t] = base[t] + scale * B (A x[t]) of adapter ids[t] (int32; outside [0, n): none; None:
         adapter 0).  base None: zeros.  out: written in place (may be base); None: a new tensor of
-        base's type, x's without a base."""
+        base's type, x's without a base.  workspace: of workspace(), for its status."""
         torch = _torch()[0]
         T = x.shape[0]
         mx, mb = self._rows(x, T, self.n_in, "x"), self._rows(base, T, self.n_out, "base")
@@ -605,14 +631,13 @@ class Adapters:
         if out is None:
             out = (x if base is None else base).new_empty((T, self.n_out))
         mo = self._rows(out, T, self.n_out, "out")
-        n = self._workspace_bytes(T, False)
-        ws = x.new_empty((n,), dtype=torch.uint8) if n else None
-        _call(self.device, self.L.hymoe_adapt, self._spec, mx, i, T, mb, mo, ws.data_ptr() if n else None, n)
+        ws, ptr, n = self._memory(workspace, x, T, False)
+        _call(self.device, self.L.hymoe_adapt, self._spec, mx, i, T, mb, mo, ptr, n)
         return out
 
-    def backward(self, x, dy, ids=None, base=None, want=("dx", "da", "db")) -> dict:
+    def backward(self, x, dy, ids=None, base=None, want=("dx", "da", "db"), workspace=None) -> dict:
         """Gradients for dy [T, out]: dx (x's type, base added where given), da and db (float32, every
-        adapter's).  want: the ones to compute."""
+        adapter's).  want: the ones to compute.  workspace: of workspace(backward=True), for its status."""
         torch = _torch()[0]
         T = x.shape[0]
         mx, my = self._rows(x, T, self.n_in, "x"), self._rows(dy, T, self.n_out, "dy")
@@ -625,11 +650,10 @@ class Adapters:
         if "db" in want:
             res["db"] = x.new_empty((self.n, self.n_out, self.rank), dtype=torch.float32)
         md = self._rows(res.get("dx"), T, self.n_in, "dx")
-        n = self._workspace_bytes(T, True)
-        ws = x.new_empty((n,), dtype=torch.uint8) if n else None
+        ws, ptr, n = self._memory(workspace, x, T, True)
         _call(self.device, self.L.hymoe_adapt_backward, self._spec, mx, my, i, T, mb, md,
               res["da"].data_ptr() if "da" in res else None, res["db"].data_ptr() if "db" in res else None,
-              ws.data_ptr() if n else None, n)
+              ptr, n)
         return res
 
 
