@@ -2076,13 +2076,17 @@ static hymoe_status forward_call(hymoe_ctx* c, uint32_t layer, const float* x, c
         }
         // The shared expert's adapters (rows [0, T) of xp and hbuf are its inputs): gate_up's go into
         // the sums before the SwiGLU, down's onto its result.
-        auto adapt = [&](const hymoe_adapters* ad, __half* in, int n_in, const float* base, float* res, int n_out) -> hymoe_status {
+        auto adapt = [&](int phase, const hymoe_adapters* ad, __half* in, int n_in, const float* base, float* res, int n_out) -> hymoe_status {
             const hymoe_mat mx{in, HYMOE_TYPE_F16, n_in}, mb{const_cast<float*>(base), HYMOE_TYPE_F32, n_out}, mo{res, HYMOE_TYPE_F32, n_out};
+            size_t need = 0;  // a call that needs no workspace is one launch; else plan, narrow and wide product
+            if (c->prof) hymoe_adapt_workspace(ad, n_tokens, 0, &need);
+            c->phase_begin();
             const hymoe_status sa = adapt_call(ad, &mx, ids, n_tokens, base ? &mb : nullptr, &mo, c->ad_ws, c->ad_ws_bytes, st, c->err_word);
+            c->phase_end(phase, need ? 3 : 1);
             return sa == HYMOE_OK ? sa : c->fail(sa, "adapters: %s", hymoe_last_error(nullptr));
         };
         if (ad_gu) {
-            const hymoe_status sa = adapt(ad_gu, c->xp, H, nullptr, c->ad_delta, 2 * I);
+            const hymoe_status sa = adapt(HYMOE_PHASE_GATE_UP, ad_gu, c->xp, H, nullptr, c->ad_delta, 2 * I);
             if (sa != HYMOE_OK) return sa;
         }
         const float* glu_add = ad_gu ? c->ad_delta : nullptr;
@@ -2169,7 +2173,7 @@ static hymoe_status forward_call(hymoe_ctx* c, uint32_t layer, const float* x, c
         }
         if (shared_apart) HY_CUDA(c, cudaStreamWaitEvent(st, c->ev_join, 0));  // the shared expert's rows of y
         if (ad_dn) {
-            const hymoe_status sa = adapt(ad_dn, c->hbuf, I, c->y, c->y, H);
+            const hymoe_status sa = adapt(HYMOE_PHASE_DOWN, ad_dn, c->hbuf, I, c->y, c->y, H);
             if (sa != HYMOE_OK) return sa;
         }
         if (T > 0) {

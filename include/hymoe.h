@@ -266,8 +266,8 @@ enum {
     HYMOE_PHASE_ROUTER = 0,   /* router GEMV (+ softmax + top-K when T > 16) */
     HYMOE_PHASE_PLAN = 1,     /* prefix scan + work lists (+ top-K, T <= 16) */
     HYMOE_PHASE_DISPATCH = 2, /* scatter / gather of token rows              */
-    HYMOE_PHASE_GATE_UP = 3,  /* grouped gate_up GEMM + SwiGLU               */
-    HYMOE_PHASE_DOWN = 4,     /* grouped down GEMM                           */
+    HYMOE_PHASE_GATE_UP = 3,  /* grouped gate_up GEMM + SwiGLU, and the shared expert's adapters */
+    HYMOE_PHASE_DOWN = 4,     /* grouped down GEMM, and the shared expert's adapters */
     HYMOE_PHASE_COMBINE = 5,  /* weighted combine + residual                 */
     HYMOE_PHASE_EP_DISPATCH = 6, /* expert-parallel token exchange           */
     HYMOE_PHASE_EP_COMBINE = 7,  /* expert-parallel result exchange          */
