@@ -332,7 +332,8 @@ __device__ void ep_finish(const EpFuse& f, int ct, int n_ctas, int flag_off, int
     }
 }
 
-template <int WT, int STAGES, bool EP>
+// ADD: glu_add is there (an instance of its own, so that other calls keep their code).
+template <int WT, int STAGES, bool EP, bool ADD>
 __global__ void __launch_bounds__(EP ? kEpThreads : kThreads, 1)
     gemm_tc_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs a, const __grid_constant__ EpFuse ep) {
     constexpr int RAW = tile_bytes(WT);
@@ -526,7 +527,7 @@ __global__ void __launch_bounds__(EP ? kEpThreads : kThreads, 1)
                 // matching up rows.  Lanes < 16 finish tokens 0-15 of the chunk, lanes >= 16
                 // tokens 16-31; one shuffle per token pair swaps the missing halves.
                 const bool gate_lane = lane < 16;
-                if (a.glu_add != nullptr && row0 < a.shared_rows) {
+                if (ADD && row0 < a.shared_rows) {
                     // the shared expert's adapters: this lane's gate or up column of every token
                     const float* add = a.glu_add + static_cast<size_t>(row0 + ch * 32) * 2 * a.out_ld +
                                        (gate_lane ? 0 : a.out_ld) + rb * kGluHalf + 16 * q + (lane & 15);
@@ -625,11 +626,11 @@ constexpr size_t smem_bytes() {
            (3 * STAGES + 5) * 8 + 8 + 4 * (kEpMaxRanks + 1);
 }
 
-template <int WT, int STAGES, bool EP>
+template <int WT, int STAGES, bool EP, bool ADD = false>
 cudaError_t launch_typed(const GemmMaps& maps, const GemmArgs& a, const EpFuse& ep, int n_sms, cudaStream_t st) {
     constexpr size_t smem = smem_bytes<WT, STAGES>();
     static_assert(smem <= 232448, "shared memory budget");
-    auto kern = gemm_tc_kernel<WT, STAGES, EP>;
+    auto kern = gemm_tc_kernel<WT, STAGES, EP, ADD>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
@@ -674,6 +675,14 @@ cudaError_t launch_gemm_tc(const GemmMaps& maps, const GemmArgs& a, int n_sms, c
         }
     }
     const EpFuse none{};
+    if (a.glu_add != nullptr) {
+        switch (a.wtype) {
+            case W_Q4_0: return launch_typed<W_Q4_0, 6, false, true>(maps, a, none, n_sms, st);
+            case W_Q8_0: return launch_typed<W_Q8_0, 5, false, true>(maps, a, none, n_sms, st);
+            case W_F16: return launch_typed<W_F16, 4, false, true>(maps, a, none, n_sms, st);
+            default: return cudaErrorInvalidValue;
+        }
+    }
     switch (a.wtype) {
         case W_Q4_0: return launch_typed<W_Q4_0, 6, false>(maps, a, none, n_sms, st);
         case W_Q8_0: return launch_typed<W_Q8_0, 5, false>(maps, a, none, n_sms, st);
