@@ -1485,10 +1485,10 @@ hymoe_status hymoe_set_adapters(hymoe_ctx* c, uint32_t layer, const hymoe_adapte
     HY_CUDA(c, cudaStreamSynchronize(c->stream));  // no call still uses the old ones
     c->clear_graphs();
     if (need > c->ad_ws_bytes) {
+        char* more = nullptr;  // (other layers keep theirs where this fails)
+        HY_CUDA(c, dalloc(&more, need));
         cudaFree(c->ad_ws);
-        c->ad_ws = nullptr;
-        c->ad_ws_bytes = 0;
-        HY_CUDA(c, dalloc(&c->ad_ws, need));
+        c->ad_ws = more;
         c->ad_ws_bytes = need;
     }
     if ((gate_up || down) && !c->ad_ids) HY_CUDA(c, dalloc(&c->ad_ids, static_cast<size_t>(c->cfg.max_tokens)));

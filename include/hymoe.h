@@ -446,8 +446,9 @@ hymoe_status hymoe_set_balance_bias(hymoe_ctx* ctx, uint32_t layer, const float*
 /* Adapters of one layer's shared expert for hymoe_forward_adapted, HYMOE_TYPE_F16: gate_up (H ->
  * 2I: gate rows, then up rows) joins the projection before the SwiGLU, down (I -> H) its result;
  * either may be NULL, both NULL remove them.  The weights are read where they are, in device memory
- * of the context's device: keep them until they are replaced or the context is destroyed.  The first
- * calls allocate the context's scratch for them. */
+ * of the context's device: keep them until they are replaced or the context is destroyed.  Calls
+ * allocate the context's scratch for them, anew where larger ones come: a CUDA graph of the caller's own
+ * that holds calls of this context is captured again after hymoe_set_*. */
 hymoe_status hymoe_set_adapters(hymoe_ctx* ctx, uint32_t layer, const hymoe_adapters* gate_up,
                                 const hymoe_adapters* down);
 
