@@ -190,7 +190,7 @@ cudaError_t launch_plan_adapt(const int* ids, int T, int n, const AdaptPlan& p, 
 
 // The workspace: every part starts on 256 bytes.
 struct AdaptLayout {
-    size_t perm, tiles, items, pieces, amax, lists, counters, low, low2, low_part, low_part2, part, slots, low16[2], bytes;
+    size_t perm, tiles, items, pieces, amax, lists, counters, low, low2, low_part, low_part2, part[2], slots, low16[2], bytes;
     int tile_rows, max_tiles, spare_tiles, max_items;
 };
 // (the sizes do not depend on tile_rows)
@@ -226,7 +226,9 @@ AdaptLayout adapt_layout(const hymoe_adapters* ad, size_t T, bool backward, int 
         l.low2 = take(T * adapt_rp(ad->rank) * sizeof(float));
         for (size_t& at : l.low16) at = take(T > kTcRows ? T * adapt_parts(adapt_rp(ad->rank)) * 2 : 0);
         l.slots = 2 * long_pieces;  // an adapter of c tokens in p > 1 pieces: p < 2 c / chunk
-        l.part = take(l.slots * ad->rank * (static_cast<size_t>(ad->in_features) + ad->out_features) * sizeof(float));
+        // one part each: behind da's odd number of pieces' elements db's would not be on 16 bytes, as the join loads them
+        l.part[0] = take(l.slots * ad->rank * ad->in_features * sizeof(float));
+        l.part[1] = take(l.slots * ad->rank * ad->out_features * sizeof(float));
     }
     return l;
 }
@@ -590,7 +592,7 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
     float* low_dy = reinterpret_cast<float*>(ws + l.low);
     float* low_x = reinterpret_cast<float*>(ws + l.low2);
     float *low_part = reinterpret_cast<float*>(ws + l.low_part), *low_part2 = reinterpret_cast<float*>(ws + l.low_part2);
-    float* part = reinterpret_cast<float*>(ws + l.part);
+    float *part_a = reinterpret_cast<float*>(ws + l.part[0]), *part_b = reinterpret_cast<float*>(ws + l.part[1]);
     const int i = static_cast<int>(I), o = static_cast<int>(O);
     unsigned* amax = tc_grad && ad->type == HYMOE_TYPE_F16 ? plan.amax : nullptr;
     cudaError_t e = launch_plan_adapt(ids, t, n, plan, st);
@@ -605,8 +607,8 @@ extern "C" hymoe_status hymoe_adapt_backward(const hymoe_adapters* ad, const hym
     if (e == cudaSuccess && !pair && db) e = run_low(by_x, *x, ad->type, false, t, n, tc_x, n_sms, st);
     // dA from x and dy's narrow rows, dB from dy and x's; long adapters in pieces
     AdaptGradPair grads;
-    grads.g[0] = grad_args(plan, low_dy, *x, da, part, n, R, i, 1, i);
-    grads.g[1] = grad_args(plan, low_x, *dy, db, part + l.slots * R * I, n, R, o, R, 1);
+    grads.g[0] = grad_args(plan, low_dy, *x, da, part_a, n, R, i, 1, i);
+    grads.g[1] = grad_args(plan, low_x, *dy, db, part_b, n, R, o, R, 1);
     if (tc_grad) {
         const int wide = adapt_parts(adapt_rp(R));
         for (int k = 0; k < 2; ++k) {
