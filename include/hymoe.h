@@ -418,8 +418,9 @@ hymoe_status hymoe_adapt(const hymoe_adapters* adapters, const hymoe_mat* x, con
  *   da[a]  = scale[a] * sum over a's tokens of (B_a^T dy[t]) x[t]^T   [n_adapters, rank, in_features]
  *   db[a]  = scale[a] * sum over a's tokens of dy[t] (A_a x[t])^T     [n_adapters, out_features, rank]
  * da and db are F32, overwritten for every adapter (0 where it has no tokens), nullable.  The
- * sums' order depends on the ids alone: equal inputs give equal bits.  Infinities and NaN come out of
- * dx as of hymoe_adapt's out; da and db are infinite or NaN where they take part.  For F16 adapters,
+ * sums' order depends on the ids, sizes, types, alignment and outputs of a call: equal calls give equal
+ * bits.  Infinities and NaN come out of dx as of hymoe_adapt's out; da and db are infinite or NaN where
+ * they take part.  For F16 adapters,
  * more than 128 tokens and rows that TMA takes (16-byte boundaries), da and db hold B_a^T dy and A_a x
  * to 33 bits below the adapter's largest of them. */
 hymoe_status hymoe_adapt_backward(const hymoe_adapters* adapters, const hymoe_mat* x, const hymoe_mat* dy,
