@@ -25,9 +25,10 @@ constexpr int kAdGradCols = 128;    // columns of a gradient tile
 // Rank padded to the kernels' sizes.
 __host__ __device__ constexpr int adapt_rp(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
-// Tokens of one gradient item.  An adapter of up to twice the average length stays whole; a long one is cut into
-// pieces that run side by side (their sums are added in order by a second kernel), five where it
-// has all the tokens, at most eight.
+// Tokens of one gradient item.  An adapter of up to twice the average length, and of up to a fifth of
+// all tokens, stays whole (with fewer than ten adapters the fifth decides), as does one of up to 512
+// tokens; a longer one is cut into pieces that run side by side (their sums are added in order by a
+// second kernel), five where it has all the tokens, at most eight.
 constexpr int kAdMinChunk = 512, kAdMaxPieces = 8;
 __host__ __device__ constexpr int adapt_chunk(int T, int n) {
     const int avg = static_cast<int>(static_cast<int64_t>(T) * 2 / n), fifth = T / 5;

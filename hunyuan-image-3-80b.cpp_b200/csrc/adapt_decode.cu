@@ -8,7 +8,7 @@
 // read its weights from L2 again.  Four CTAs fit an SM, so 64 tokens' 512 run at once (with three,
 // rank 32 went from 9.1 us at 48 tokens to 16.2 at 64).  Bound by the latency of its two passes over the weights
 // (about 5 us with the launch) up to some 20 MB of distinct adapters, then by reading them:
-// 64 tokens of 32 adapters, 4096 to 6144, rank 32 (21 MB), 9 us with them in L2, 14 without.
+// 64 tokens of 32 adapters, 4096 to 6144, rank 32 (21 MB), 10.5 us with them in L2, 15 without.
 #include "adapt.cuh"
 #include "kernels.h"
 

@@ -7,9 +7,9 @@
 // in its accumulators, 4096 columns of a CTA cost 2e-5 of low, and more the longer the rows.  Bound by reading x (the weights, RP / 64 of its
 // bytes per tile, come from L2): four stages of 64 columns are in flight per CTA, and S is chosen
 // so that the CTAs fill the GPU once.  77 tokens of 4096 columns, rank 16, both narrow products of a
-// backward pass: 9.4 us.  Long batches of F32 rows are bound by the tf32 pipe (two products for x's
-// two parts): 8192 tokens of 4096 columns, rank 64, 76 us; bf16 rows off 16-byte boundaries by their
-// copies of 2 bytes: 84 us.
+// backward pass: 8.8 us.  Long batches of F32 rows are bound by the tf32 pipe (two products for x's
+// two parts): 8192 tokens of 4096 columns, rank 64, 78 us; bf16 rows off 16-byte boundaries by their
+// copies of 2 bytes: 85 us (125 with the weights off them too).
 #include "adapt.cuh"
 #include "kernels.h"
 

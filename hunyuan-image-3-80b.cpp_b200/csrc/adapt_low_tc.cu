@@ -9,7 +9,8 @@
 // tensor memory.  The parts are added in distributed shared memory, every CTA taking its share of
 // the rows, in the order of the parts.
 //
-// The pipe truncates what it adds, up to 1.4 times 2^-23 of the running sum each time, so a CTA's
+// The pipe truncates what it adds, up to 1.4 times 2^-23 of the running sum each time (terms of one
+// sign; some 4e-8 of it on average over terms of both), so a CTA's
 // columns take turns in four accumulators (two at rank 128), as long as that makes 64 stages at most:
 // 64 additions each (128).  Longer rows (LONG) go in segments of 8 stages, 32 additions to one
 // accumulator, which the epilogue's warps add in fp32 to totals in tensor memory while the next

@@ -7,7 +7,8 @@
 // whole 16-byte pieces.  The intermediate rows are read once per CTA into registers, as 16-bit parts
 // (two for a 16-bit result, enough to hold fp32 for an fp32 one), so the products run on the
 // 16-bit matrix pipe.  Bound by reading and writing out's rows: 77 tokens to 4096 columns, rank 16,
-// take 5 us; 8192 to 6144, rank 64, off 16-byte boundaries 138 us, by their copies of 2 bytes.
+// take 5 us; 8192 bf16 rows to 6144 off 16-byte boundaries, rank 64, 261 us, by their copies of 2 bytes
+// (300 with the weights off them too; 124 with the weights alone).
 #include "adapt.cuh"
 #include "kernels.h"
 

@@ -26,10 +26,10 @@
 // only where that does not prove them either, or which groups are kept is in doubt, all its experts
 // are (route_exact).
 //
-// Bound by instruction issue, and by latency in short calls: 128 experts and 6 choices with a bias,
-// bf16, take 3.0 us for 256 tokens (a warp each), 27.7 us for 131072 (a thread each; 60.6 by warps,
-// some 400 warp instructions a token, while its logits are 256 bytes); 256 experts in 8 groups 12 us
-// for 8192 tokens (26 before the candidates were settled by themselves: one token selected again in
+// Bound by instructions, and by latency in short calls: 128 experts and 6 choices with a bias,
+// bf16, take 3.0 us for 256 tokens (a warp each), 27.6 us for 131072 (a thread each, some 39 instructions
+// an expert: issue slots 55% busy; 60.6 by warps, some 400 warp instructions a token, while its logits
+// are 256 bytes); 256 experts in 8 groups 12 us for 8323 tokens (26 before the candidates were settled by themselves: one token selected again in
 // full took longer than all the others).
 #pragma once
 
