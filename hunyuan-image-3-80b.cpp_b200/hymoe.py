@@ -593,10 +593,14 @@ class Adapters:
         whether the results are whole.  Calls without one take memory of their own and drop it."""
         import torch
         n = self._workspace_bytes(T, backward)
-        return torch.empty((n,), dtype=torch.uint8, device=self.device) if n else None
+        if n == 0:
+            return None
+        ws = torch.empty((n,), dtype=torch.uint8, device=self.device)
+        ws[:4].zero_()  # calls of a few tokens need none and leave the status alone
+        return ws
 
     def check(self, workspace) -> None:
-        """Waits for the call that was given this workspace (on the current stream) and raises HymoeError
+        """Waits for the last call that used this workspace() (on the current stream) and raises HymoeError
         (TIMEOUT) if a bounded device-side wait expired in it: its results are not whole then."""
         if workspace is not None and bool(workspace[:4].any()):
             raise HymoeError(STATUS_TIMEOUT, "hymoe_adapt: a bounded device-side wait expired, the results are not whole")

@@ -403,8 +403,9 @@ hymoe_status hymoe_adapt_workspace(const hymoe_adapters* adapters, uint32_t n_to
  *   base, out [n_tokens, out_features], both of the adapters' type or both F32.  base == NULL
  *     counts as zeros; out may be base itself (same data and ld), else nothing may overlap
  *   workspace: hymoe_adapt_workspace bytes, 256-byte aligned, used by this call alone until it
- *     has run (NULL where none is needed).  Its first 4 bytes are then 0; anything else says that a
- *     bounded device-side wait expired and the results are not whole
+ *     has run (NULL where none is needed; a call that needs none does not touch it).  Its first 4
+ *     bytes are then 0; anything else says that a bounded device-side wait expired and the results
+ *     are not whole
  * Products are summed in fp32, the intermediate A x is kept in fp32 or in parts that add up to it
  * (to 16 bits beside a 16-bit result, 21 beside an F32 one), and the result is rounded once.
  * Infinities and NaN in x or base stay in their token's row and come out as the formula has them. */

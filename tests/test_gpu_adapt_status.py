@@ -64,3 +64,16 @@ def test_captured_with_its_own_workspace():
         graph.replay()
         ad.check(ws)
         assert torch.equal(out, want)
+
+
+def test_few_tokens_leave_the_status_alone():
+    """A serving loop's one workspace for batches of every size: steps of a few tokens do not use it."""
+    p = Problem(300, 256, 264, 16, 4)
+    ad = p.adapters
+    for _ in range(3):
+        junk = torch.full((ad.workspace(300).numel(),), 0xFF, dtype=torch.uint8, device="cuda")
+        del junk  # the next workspace is likely to be this memory
+        ws = ad.workspace(300)
+        for T in (5, 64, 300, 5):
+            ad.apply(p.x[:T], p.ids[:T], base=p.base[:T], workspace=ws)
+            ad.check(ws)
